@@ -559,6 +559,45 @@ int pm_gemm_swiglu_bwd_bf16(const void* dy_bf16, int64_t lddy, const void* w_dow
 int pm_gemm_debug_set_variant(int32_t value);
 
 /* --------------------------------------------------------------------------------------------
+ * Low-rank adapters of many runs beside a shared projection, and their gradients' norm.  Stands where the reference keeps one LoRA adapter per run in its
+ * linear layers (models/layers/lora/*, rows split by the micro-batch's lora_num_tokens, trainer/rl/data.py:18-52) and clips each run's gradients
+ * (trainer/utils.py:88-98).
+ *
+ * Rows are grouped by adapter: adapter g owns the POSITIONS [offsets[g], offsets[g+1]) (int32 [n_adapters + 1] on the device, offsets[0] = 0, not decreasing);
+ * position p is row row_ids[p] of the row tensors (row_ids int32 [n_rows], each row at most once; NULL: position p is row p).  Positions behind the last offset belong to
+ * no adapter: their rows of the result are the base's.  Both factors are rank-major: a [n_adapters, rank, d_in], b [n_adapters, rank, d_out] (bf16, contiguous), scales f32.
+ * Row tensors are bf16 with their own row strides (elements, multiples of 8, rows 16-byte aligned).  d_in, d_out multiples of 8, rank 1 .. 128 (zero rows of both
+ * factors give a smaller rank).  Offsets and row ids out of range are clamped: such a table gives wrong results, never an access out of range.  Deterministic.
+ *   fwd:   z[p] = scales[g] * x[row] . a[g]^T (f32, [n_rows, pm_lora_z_columns(rank)] in the order of the positions, the columns past the rank zero; rows of no adapter are
+ *          not written); out[row] = bf16(base[row] + z[p] . b[g]).  out may be base (in place); base NULL = zeros.
+ *   bwd:   dz[p] = scales[g] * grad_out[row] . b[g]^T; grad_x[row] = bf16(base[row] + dz[p] . a[g]) (grad_x NULL: not wanted; base as above);
+ *          grad_a[g] (+)= dz^T . x, grad_b[g] (+)= z^T . grad_out, f32 in the factors' layout, written (accumulate 0; zero for an adapter without rows) or added to (1); both
+ *          NULL: not wanted, then x and z may be NULL.  z is what the forward left.
+ *   merge: out = bf16(weight + scale * b^T . a) for a weight [d_out, d_in] and ONE adapter a [rank, d_in], b [rank, d_out]: what the weight push sends.  out may be weight.
+ * ------------------------------------------------------------------------------------------ */
+int64_t pm_lora_z_columns(int32_t rank);
+int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank);
+int pm_lora_fwd(const void* x_bf16, int64_t ldx, const void* a_bf16, const void* b_bf16, const float* scales, const int32_t* offsets, const int32_t* row_ids /* nullable */,
+                int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base_bf16 /* nullable */, int64_t ldbase, void* out_bf16, int64_t ldout,
+                float* z, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank);
+int pm_lora_bwd(const void* grad_out_bf16, int64_t ldg, const void* x_bf16, int64_t ldx, const float* z, const void* a_bf16, const void* b_bf16, const float* scales,
+                const int32_t* offsets, const int32_t* row_ids /* nullable */, int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank,
+                const void* base_bf16 /* nullable */, int64_t ldbase, void* grad_x_bf16 /* nullable */, int64_t ldgx, float* grad_a /* nullable */, float* grad_b /* nullable */,
+                int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream);
+int pm_lora_merge(const void* weight_bf16, int64_t ldw, const void* a_bf16, const void* b_bf16, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out_bf16, int64_t ldo,
+                  void* stream);
+/* Gradient norms of many tensors by group, and clipping (torch clip_grad_norm_ over each group; trainer/utils.py:88-98).  `chunks`: int64 [n_chunks][4] on the device, rows
+ * {source address, destination address (0: none), elements, (group << 8) | source is bf16 (bit 0) | destination is bf16 (bit 1)}, f32 where a bit is clear; the chunks of one group
+ * stand together, group g's at [group_offsets[g], group_offsets[g+1]) (int32 [n_groups + 1]).  Destinations are their source (same type) or memory of their own.
+ *   sumsq_out[g] = sum of squares in 64 bits (nullable); norms[g] = sqrt of it; coefs[g] = min(1, max_norm / (norms[g] + 1e-6)), 1 for max_norm <= 0 (max_norms [n_groups], where it
+ *   is not NULL, in the place of max_norm); with scale != 0, destination = source * coefs[group].  sumsq_in (nullable) stands in for the sums: what an all-reduce over ranks made of
+ *   them.  norms and coefs may both be NULL where only sumsq_out is wanted.  partials: f64 [n_chunks] of the caller's. */
+int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32_t* group_offsets, int32_t n_groups, const double* sumsq_in /* nullable */, float max_norm,
+                 const float* max_norms /* nullable */, double* partials, double* sumsq_out /* nullable */, float* norms /* nullable */, float* coefs /* nullable */, int32_t scale,
+                 void* stream);
+
+/* --------------------------------------------------------------------------------------------
  * Diagnostics used by tests/ to pin the MFMA fragment layouts the attention kernels assume.
  * C[16,16] = A[16,32] @ B[32,16]^T-free form: c = sum_k a[i][k]*b[j][k]  (both operands K-contiguous, bf16). */
 int pm_mfma_probe_16x16x32(const void* a_bf16, const void* b_bf16, float* c_f32, void* stream);

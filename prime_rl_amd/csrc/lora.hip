@@ -1,0 +1,666 @@
+// lora.hip — the low-rank updates of many runs' adapters beside a shared projection: forward, backward, and an adapter merged into its projection.
+//
+// Rows (tokens) sorted by adapter: adapter a owns the positions [offsets[a], offsets[a+1]); position p is row row_ids[p] of the row tensors (row p itself
+// without row_ids), so packed runs need no permutation and requests in arrival order need no copy.  With s = scales[a], A = a[a] [r, in], B = b[a] [r, out],
+// both rank-major (the factors' long axis is contiguous), every step is one of three products:
+//   shrink   z[p, :]  = s * x[row(p), :] . A^T            the long axis is contracted: both operands are K-contiguous, fragments straight from global memory
+//   expand   y[row, :] = base[row, :] + z[p, :] . B         the short axis (rank) is contracted; the factor tile is read transposed out of LDS
+//   outer    dW[r, c]  = sum_p z[p, r] * t[row(p), c]       the rows are contracted: both operands are read transposed out of LDS (ds_read_b64_tr_b16)
+//   forward  = shrink(x, A), expand(base, z, B);   backward: dz = shrink(dy, B), dx = expand(base_dx, dz, A), dB = outer(z, dy), dA = outer(dz, x)
+//   merge    = expand(W, s B^T, A) with the rows of W in the place of tokens.
+//
+// All of it is bound by HBM traffic of the row tensors up to rank 128 (2 r operations per 2-byte element, far under the MFMA rate), so each kernel makes one
+// pass over its row tensor with 16-byte accesses, and the matrix cores are there to keep the arithmetic out of the way.
+//
+// Numerics: z and dz are f32 in memory.  Where they feed the matrix cores they are split into bf16 terms that add up to the f32 value: two terms (16 bits)
+// in expand, whose result is rounded to bf16 (8 bits) anyway, three terms (24 bits: all of it) in outer, whose results are f32 gradients.  Everything else in
+// the products is bf16 by type and every sum is f32, in a fixed order (no atomics: the same inputs give the same bits).
+#include "common.hip.h"
+
+namespace pm {
+namespace lora {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+
+constexpr int kMaxRank = 128;
+constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
+constexpr int kOuterCols = 256;  // columns per outer tile
+
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ u32x2 tr_read(const unsigned char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_ptr)p));
+}
+
+// The leading bf16 terms of 4 values, which are replaced by what they leave.  An infinite term leaves nothing (not inf - inf).
+__device__ __forceinline__ u32x2 take_terms(f32x4& v) {
+  const u32x2 t = {pack_bf16_hw(v[0], v[1]), pack_bf16_hw(v[2], v[3])};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float lead = q & 1 ? bf16hi(t[q >> 1]) : bf16lo(t[q >> 1]);
+    v[q] = __builtin_isfinite(lead) ? v[q] - lead : 0.f;
+  }
+  return t;
+}
+__device__ __forceinline__ u32x2 to_bf16(const f32x4& v) { return u32x2{pack_bf16_hw(v[0], v[1]), pack_bf16_hw(v[2], v[3])}; }
+
+// Tile `t` of `rows` positions each -> its adapter and positions [p0, p1).  A tile never straddles two adapters.  Positions outside every adapter (behind the last
+// offset, before the first) come after all adapters' tiles as adapter -1.  Offsets are clamped into [0, n] and never run backwards, so no table makes an access out of range.
+__device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int n_adapters, int n, int rows, int t, int lane, int& adapter, int& p0, int& p1) {
+  int base = 0;
+  for (int e0 = 0; e0 < n_adapters + 2; e0 += 64) {
+    const int e = e0 + lane;
+    int lo = 0, hi = 0;
+    if (e < n_adapters) {
+      lo = min(max(offsets[e], 0), n);
+      hi = min(max(offsets[e + 1], lo), n);
+    } else if (e == n_adapters) {
+      lo = min(max(offsets[n_adapters], 0), n);
+      hi = n;
+    } else if (e == n_adapters + 1) {
+      hi = min(max(offsets[0], 0), n);
+    }
+    const int tiles = (hi - lo + rows - 1) / rows;
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    const unsigned long long hit = __ballot(base + incl > t);
+    if (hit) {
+      const int src = __ffsll((long long)hit) - 1;
+      const int first = base + __shfl(incl, src, 64) - __shfl(tiles, src, 64);
+      adapter = e0 + src < n_adapters ? e0 + src : -1;
+      p0 = __shfl(lo, src, 64) + (t - first) * rows;
+      p1 = min(p0 + rows, __shfl(hi, src, 64));
+      return true;
+    }
+    base += __shfl(incl, 63, 64);
+  }
+  return false;
+}
+// Tiles that any offsets of n positions can need.
+static inline int64_t max_tiles(int64_t n, int64_t n_adapters, int64_t rows) {
+  const int64_t t = n / rows + n_adapters + 2;
+  return t < n ? t : n;
+}
+
+__device__ __forceinline__ int64_t row_of(const int32_t* __restrict__ row_ids, int p, int n) {
+  return row_ids ? min(max(row_ids[p], 0), n - 1) : p;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// shrink: z[part][p][r] = scale * sum over the part's columns of t[row(p)][k] * w[adapter][r][k].
+// A workgroup takes 16 * MT positions and one part of the long axis; its four waves take every fourth 64-column step (128 bytes of each row: whole cache
+// lines) and wave 0 adds the four results up through LDS.  The fragments of v_mfma_f32_16x16x32_bf16 come straight from global memory: rows of the factor
+// (from L2, where it stays) as the A operand, rows of t as the B operand.  Positions past the tile's end repeat its first row and are not stored.
+template <int RT, int MT, int U>
+__global__ __launch_bounds__(256) void shrink_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
+                                                     const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank, int rp,
+                                                     int steps_per_part, float* __restrict__ z) {
+  constexpr int kStride = RT * 16 + 4;
+  __shared__ __attribute__((aligned(16))) float red[3][MT * 16][kStride];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+  int adapter, p0, p1;
+  if (!locate(offsets, n_adapters, n, 16 * MT, blockIdx.x, lane, adapter, p0, p1) || adapter < 0) return;
+  const bf16_t* tp[MT];
+  const bf16_t* wp[RT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int p = p0 + i * 16 + lr;
+    tp[i] = t + row_of(row_ids, p < p1 ? p : p0, n) * ldt + lq * 8;
+  }
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const int r = j * 16 + lr;
+    wp[j] = w + ((int64_t)adapter * rank + (r < rank ? r : 0)) * d + lq * 8;
+  }
+  f32x4 acc[MT][RT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int s0 = blockIdx.y * steps_per_part;
+  const int s1 = min(s0 + steps_per_part, (d + 63) >> 6);
+  const int full = min(s1, d >> 6);  // steps whose 64 columns all exist
+  int s = s0 + wave;
+  for (; s + 4 * (U - 1) < full; s += 4 * U) {
+    u32x4 tf[U][2][MT], wf[U][2][RT];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = (s + 4 * u) * 64 + h * 32;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) tf[u][h][i] = *reinterpret_cast<const u32x4*>(tp[i] + k);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) wf[u][h][j] = *reinterpret_cast<const u32x4*>(wp[j] + k);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[u][h][j], tf[u][h][i], acc[i][j]);
+  }
+  for (; s < s1; s += 4) {  // what is left, columns past the end as zeros on both sides
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = s * 64 + h * 32;
+      const bool in = k + lq * 8 < d;
+      u32x4 tf[MT], wf[RT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) tf[i] = in ? *reinterpret_cast<const u32x4*>(tp[i] + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < RT; ++j) wf[j] = in ? *reinterpret_cast<const u32x4*>(wp[j] + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[j], tf[i], acc[i][j]);
+    }
+  }
+  // a lane holds z[position lr][ranks 4 lq .. 4 lq + 3] of every 16 x 16 block
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) *reinterpret_cast<f32x4*>(&red[wave - 1][i * 16 + lr][j * 16 + lq * 4]) = acc[i][j];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  const float scale = scales[adapter];
+  float* zp = z + (int64_t)blockIdx.y * n * rp;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int p = p0 + i * 16 + lr;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      const int r = j * 16 + lq * 4;
+      f32x4 v = acc[i][j];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) v += *reinterpret_cast<const f32x4*>(&red[q][i * 16 + lr][r]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = r + q < rank ? v[q] * scale : 0.f;
+      if (p < p1 && r < rp) *reinterpret_cast<f32x4*>(zp + (int64_t)p * rp + r) = v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// expand: out[row][c] = bf16(base[row][c] + sum_r z[p][r] * w[adapter][r][c]).
+// A workgroup takes 64 positions x COLS columns.  The factor tile [r][COLS] goes to LDS once; the matrix cores' A operand is its transpose (columns as
+// rows), read with ds_read_b64_tr_b16 so that a lane ends up with 8 consecutive columns of one position: base and out move in 16-byte accesses, whole
+// 128-byte lines per four waves.  The base is asked for before anything waits.  z is split into two bf16 terms: at rank <= 16 both fit the 32-deep
+// contraction of one instruction (its two halves read the same 16 factor rows).
+// Without base the sum starts from zero; rows of no adapter get the base as it is.  MERGE: positions are the rows of a weight, z[p][r] = scale * zb[r][p] (bf16).
+template <int RT>
+struct ExpandShape {
+  static constexpr int kCols = RT == 1 ? 512 : RT == 2 ? 512 : RT == 4 ? 256 : 128;
+  static constexpr int kStride = kCols * 2 + 32;  // bytes; a row shift of 32 bytes spreads the 8 rows that a transposed read takes at once over all banks
+  static constexpr int kSteps = RT == 1 ? 1 : RT / 2;  // 32-deep contraction steps over the rank
+  static constexpr int kTerms = RT == 1 ? 1 : 2;       // bf16 terms that are operands of their own
+  static constexpr int kBlocks = kCols / 128;          // 32-column blocks of a wave
+};
+
+template <int RT, bool MERGE>
+__global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict__ z, int parts, float* __restrict__ z_out, const bf16_t* __restrict__ zb, float merge_scale,
+                                                        const bf16_t* __restrict__ w, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                        int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place) {
+  using S = ExpandShape<RT>;
+  __shared__ __attribute__((aligned(16))) unsigned char tile[RT * 16 * S::kStride];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
+  int adapter = 0, p0 = blockIdx.x * kExpandRows, p1 = min(p0 + kExpandRows, n);
+  if constexpr (!MERGE) {
+    if (!locate(offsets, n_adapters, n, kExpandRows, blockIdx.x, lane, adapter, p0, p1)) return;
+    if (adapter < 0 && in_place) return;
+  }
+  const int c0 = blockIdx.y * S::kCols;
+  // the factor tile, rows past the rank and columns past the end as zeros
+  constexpr int kPieces = RT * 16 * S::kCols / 8 / 256;
+  u32x4 stage[kPieces];
+  if (adapter >= 0) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = i * 256 + tid, r = piece / (S::kCols / 8), c = c0 + piece % (S::kCols / 8) * 8;
+      stage[i] = r < rank && c < d ? *reinterpret_cast<const u32x4*>(w + ((int64_t)adapter * rank + r) * d + c) : u32x4{0, 0, 0, 0};
+    }
+  }
+  const int tiles16 = (p1 - p0 + 15) >> 4;
+  int64_t row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = p0 + i * 16 + lr;
+    row[i] = row_of(row_ids, p < p1 ? p : p0, n);
+  }
+  u32x4 zf[4][S::kSteps][S::kTerms];
+  if (adapter >= 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * 16 + lr;
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k) {
+        f32x4 v[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          v[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const int r = (RT == 1 ? 0 : k * 32 + h * 16) + lq * 4;
+          if (RT == 1 && h == 1) break;
+          if (p >= p1 || i >= tiles16) continue;
+          if constexpr (MERGE) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (r + q < rank) v[h][q] = merge_scale * bf16_to_f32(zb[(int64_t)(r + q) * n + p]);
+          } else if (r < rp) {
+            for (int part = 0; part < parts; ++part) v[h] += *reinterpret_cast<const f32x4*>(z + ((int64_t)part * n + p) * rp + r);
+            if (z_out && blockIdx.y == 0 && wave == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = v[h];
+          }
+        }
+        const u32x2 lead0 = take_terms(v[0]), rest0 = to_bf16(v[0]);
+        if constexpr (RT == 1) {
+          zf[i][k][0] = u32x4{lead0.x, lead0.y, rest0.x, rest0.y};
+        } else {
+          const u32x2 lead1 = take_terms(v[1]), rest1 = to_bf16(v[1]);
+          zf[i][k][0] = u32x4{lead0.x, lead0.y, lead1.x, lead1.y};
+          zf[i][k][S::kTerms - 1] = u32x4{rest0.x, rest0.y, rest1.x, rest1.y};
+        }
+      }
+    }
+  }
+  u32x4 bv[S::kBlocks][4];
+#pragma unroll
+  for (int b = 0; b < S::kBlocks; ++b) {
+    const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bv[b][i] = base && c < d && i < tiles16 ? *reinterpret_cast<const u32x4*>(base + row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+  }
+  if (adapter < 0) {  // rows of no adapter
+#pragma unroll
+    for (int b = 0; b < S::kBlocks; ++b) {
+      const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + row[i] * ldo + c) = bv[b][i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int piece = i * 256 + tid;
+    *reinterpret_cast<u32x4*>(tile + piece / (S::kCols / 8) * S::kStride + piece % (S::kCols / 8) * 16) = stage[i];
+  }
+  __syncthreads();
+  // lane (lr, lq) asks for factor row 4 lq + lr / 4 (and 16 more) at columns 8 (lr % 4) + 4 h: lane lr receives column 8 (lr / 4) + 4 h + lr % 4, so the two
+  // products h = 0, 1 leave columns 8 lq .. 8 lq + 7 of position lr in one lane
+  const unsigned char* at = tile + (lq * 4 + (lr >> 2)) * S::kStride + wave * 64 + (lr & 3) * 16;
+#pragma unroll
+  for (int b = 0; b < S::kBlocks; ++b) {
+    u32x4 wf[S::kSteps][2];
+#pragma unroll
+    for (int k = 0; k < S::kSteps; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* q = at + b * 256 + k * 32 * S::kStride + h * 8;
+        const u32x2 lo = tr_read(q), hi = RT == 1 ? lo : tr_read(q + 16 * S::kStride);
+        wf[k][h] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      }
+    const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= tiles16) break;
+      f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int k = 0; k < S::kSteps; ++k)
+#pragma unroll
+        for (int term = S::kTerms - 1; term >= 0; --term)  // the small term first
+#pragma unroll
+          for (int h = 0; h < 2; ++h) acc[h] = mfma(wf[k][h], zf[i][k][term], acc[h]);
+      u32x4 o;
+      const u32x4 v = bv[b][i];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(v[q]) + acc[q >> 1][(q & 1) * 2], bf16hi(v[q]) + acc[q >> 1][(q & 1) * 2 + 1]);
+      if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + row[i] * ldo + c) = o;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// outer: part[tile][r][c] = sum over the tile's positions of z[p][r] * t[row(p)][c], one f32 partial per tile of `rows` positions of one adapter.
+// Both products of the backward (dB from z and dy, dA from dz and x) are one launch: blockIdx.y runs over the 256-column tiles of dy, then of x.
+// The positions are the contraction, so both operands are read transposed: stages of SP positions go through LDS (t as it is, z split into three bf16
+// planes), the next stage's loads are in flight while the matrix cores work on this one.  A wave takes 64 columns and all ranks.
+struct OuterSide {
+  const float* z;      // [parts][n][rp]
+  int parts;
+  const bf16_t* t;     // [*, ldt]
+  int64_t ldt;
+  int d;
+  float* part;         // [tiles][rank][d]
+};
+
+template <int RT>
+__global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                       int n_adapters, int rank, int rp, int rows) {
+  constexpr int SP = RT <= 2 ? 64 : 32;           // positions per stage
+  constexpr int kTs = kOuterCols * 2 + 32;        // row strides in LDS: 32 bytes of shift per row keep transposed reads off each other's banks
+  constexpr int kZs = RT == 1 ? 32 : RT * 32 + 32;
+  constexpr int kTp = SP * kOuterCols / 8 / 256;  // 16-byte pieces of t per thread and stage
+  constexpr int kZp = (SP * RT * 4 + 255) / 256;  // 4-rank pieces of z per thread and stage
+  __shared__ __attribute__((aligned(16))) unsigned char lt[SP * kTs];
+  __shared__ __attribute__((aligned(16))) unsigned char lz[3][SP * kZs];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
+  const bool second = (int)blockIdx.y >= tiles0;
+  const OuterSide s = second ? s1 : s0;
+  const int c0 = (second ? blockIdx.y - tiles0 : blockIdx.y) * kOuterCols;
+  int adapter, p0, p1;
+  if (!locate(offsets, n_adapters, n, rows, blockIdx.x, lane, adapter, p0, p1) || adapter < 0) return;
+  u32x4 tv[kTp];
+  f32x4 zv[kZp];
+  auto load = [&](int ps) {
+#pragma unroll
+    for (int i = 0; i < kTp; ++i) {
+      const int piece = i * 256 + tid, p = ps + (piece >> 5), c = c0 + (piece & 31) * 8;
+      tv[i] = p < p1 && c < s.d ? *reinterpret_cast<const u32x4*>(s.t + row_of(row_ids, p, n) * s.ldt + c) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kZp; ++i) {
+      const int piece = i * 256 + tid, p = ps + piece / (RT * 4), r = piece % (RT * 4) * 4;
+      zv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p < p1 && r < rp && piece < SP * RT * 4)
+        for (int part = 0; part < s.parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(s.z + ((int64_t)part * n + p) * rp + r);
+    }
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int i = 0; i < kTp; ++i) {
+      const int piece = i * 256 + tid;
+      *reinterpret_cast<u32x4*>(lt + (piece >> 5) * kTs + (piece & 31) * 16) = tv[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kZp; ++i) {
+      const int piece = i * 256 + tid;
+      if (piece >= SP * RT * 4) break;
+      const int off = piece / (RT * 4) * kZs + piece % (RT * 4) * 8;
+      f32x4 v = zv[i];
+#pragma unroll
+      for (int term = 0; term < 3; ++term) *reinterpret_cast<u32x2*>(&lz[term][off]) = take_terms(v);
+    }
+  };
+  f32x4 acc[4][RT];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  load(p0);
+  for (int ps = p0; ps < p1; ps += SP) {
+    store();
+    __syncthreads();
+    if (ps + SP < p1) load(ps + SP);
+#pragma unroll
+    for (int k = 0; k < SP / 32; ++k) {
+      const int row = k * 32 + lq * 4 + (lr >> 2);
+      u32x4 tf[4], zf[RT][3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // columns 64 wave + 32 (i / 2) + 8 (lr / 4) + 4 (i % 2) + lr % 4
+        const unsigned char* q = lt + row * kTs + wave * 128 + (i >> 1) * 64 + (lr & 3) * 16 + (i & 1) * 8;
+        const u32x2 lo = tr_read(q), hi = tr_read(q + 16 * kTs);
+        tf[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      }
+#pragma unroll
+      for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int term = 0; term < 3; ++term) {
+          const unsigned char* q = lz[term] + row * kZs + j * 32 + (lr & 3) * 8;
+          const u32x2 lo = tr_read(q), hi = tr_read(q + 16 * kZs);
+          zf[j][term] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+#pragma unroll
+      for (int term = 2; term >= 0; --term)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][j] = mfma(tf[i], zf[j][term], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  float* part = s.part + (int64_t)blockIdx.x * rank * s.d;
+#pragma unroll
+  for (int j = 0; j < RT; ++j) {
+    const int r = j * 16 + lr;
+    if (r >= rank) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + wave * 64 + (i >> 1) * 32 + lq * 8 + (i & 1) * 4;
+      if (c < s.d) *reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c) = acc[i][j];
+    }
+  }
+}
+
+// grad[adapter][r][c] (+)= the adapter's partials, added in the order of its tiles; zero for an adapter without rows.
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part0, float* __restrict__ grad0, int64_t elems0, const float* __restrict__ part1,
+                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int n_adapters, int rows, int tiles_max,
+                                                   int accumulate) {
+  const int lane = threadIdx.x & 63, adapter = blockIdx.y;
+  int first = 0, count = 0;
+  for (int e0 = 0; e0 <= adapter; e0 += 64) {
+    const int e = e0 + lane;
+    int tiles = 0;
+    if (e <= adapter) {
+      const int lo = min(max(offsets[e], 0), n), hi = min(max(offsets[e + 1], lo), n);
+      tiles = (hi - lo + rows - 1) / rows;
+    }
+    int before = e < adapter ? tiles : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+    first += before;
+    if (adapter < e0 + 64) count = __shfl(tiles, adapter - e0, 64);
+  }
+  count = max(0, min(count, tiles_max - first));
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= elems0 + elems1) return;
+  const bool second = at >= elems0;
+  const int64_t e = second ? at - elems0 : at, elems = second ? elems1 : elems0;
+  const float* part = (second ? part1 : part0) + (int64_t)first * elems + e;
+  float* grad = (second ? grad1 : grad0) + (int64_t)adapter * elems + e;
+  f32x4 v = accumulate ? *reinterpret_cast<const f32x4*>(grad) : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < count; ++i) v += *reinterpret_cast<const f32x4*>(part + (int64_t)i * elems);
+  *reinterpret_cast<f32x4*>(grad) = v;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+static inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
+static inline int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
+static inline int shrink_rows(int rank) { return rank_tiles(rank) >= 4 ? 64 : 32; }
+
+// Parts of the long axis in shrink.  Row tiles alone fill the card from about 512 workgroups up (two on each CU); below that the axis is cut, in parts of at least
+// 512 columns (one step for each wave and two to overlap), because a single workgroup reads a factor no faster than one CU's path to L2 allows.
+static inline int shrink_parts(int64_t n, int64_t n_adapters, int d, int rank) {
+  const int64_t tiles = max_tiles(n, n_adapters, shrink_rows(rank));
+  int64_t parts = 512 / (tiles > 0 ? tiles : 1);
+  if (parts > d / 512) parts = d / 512;
+  return parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
+}
+static inline int steps_of(int d, int parts) { return (int)cdiv(cdiv(d, 64), parts); }
+
+// Positions per outer tile: enough tiles to fill the card (1024 workgroups over the column tiles), but long enough that a tile's f32 partial (4 r bytes a column, written
+// and read once) stays small beside the rows it stands for (2 bytes a column each): at least 32 r positions where there are that many.
+static inline int outer_rows(int64_t n, int d_in, int d_out, int rank) {
+  const int64_t cols = cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols);
+  int64_t rows = 64;
+  while (rows * 2 <= n * cols / 1024 && rows < 32 * rank) rows *= 2;
+  return (int)rows;
+}
+
+template <int RT>
+static void launch_shrink(const void* t, int64_t ldt, const void* w, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n, int n_adapters, int d, int rank,
+                          int parts, float* z, hipStream_t stream) {
+  constexpr int MT = RT >= 4 ? 4 : 2, U = RT == 1 ? 4 : RT == 2 ? 2 : 1;
+  const dim3 grid((unsigned)max_tiles(n, n_adapters, 16 * MT), parts);
+  hipLaunchKernelGGL((shrink_kernel<RT, MT, U>), grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets, row_ids, (int)n, n_adapters, d, rank,
+                     padded_rank(rank), steps_of(d, parts), z);
+}
+template <int RT, bool MERGE>
+static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
+                          int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t stream) {
+  const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
+  const dim3 grid((unsigned)tiles, (unsigned)cdiv(d, ExpandShape<RT>::kCols));
+  hipLaunchKernelGGL((expand_kernel<RT, MERGE>), grid, dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
+                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0);
+}
+#define PM_BY_RANK(rank, CALL)          \
+  switch (::pm::lora::rank_tiles(rank)) { \
+    case 1: { constexpr int RT = 1; CALL; } break; \
+    case 2: { constexpr int RT = 2; CALL; } break; \
+    case 4: { constexpr int RT = 4; CALL; } break; \
+    default: { constexpr int RT = 8; CALL; } break; \
+  }
+
+static int check_shape(const char* who, int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank) {
+  PM_REQUIRE(n >= 0 && n <= INT32_MAX - 4096, PM_ERR_INVALID_ARG, "%s: n_rows %lld", who, (long long)n);
+  PM_REQUIRE(n_adapters >= 1 && n_adapters <= 65535, PM_ERR_INVALID_ARG, "%s: n_adapters %lld (1 .. 65535)", who, (long long)n_adapters);
+  PM_REQUIRE(rank >= 1 && rank <= kMaxRank, PM_ERR_UNSUPPORTED, "%s: rank %lld (1 .. %d)", who, (long long)rank, kMaxRank);
+  PM_REQUIRE(d_in >= 8 && d_in % 8 == 0 && d_in <= (1 << 22) && d_out >= 8 && d_out % 8 == 0 && d_out <= (1 << 22), PM_ERR_UNSUPPORTED,
+             "%s: d_in %lld, d_out %lld (multiples of 8, at most 2^22)", who, (long long)d_in, (long long)d_out);
+  return PM_OK;
+}
+static int check_rows(const char* who, const char* name, const void* p, int64_t ld, int64_t d) {
+  PM_REQUIRE(p, PM_ERR_INVALID_ARG, "%s: null pointer (%s)", who, name);
+  PM_REQUIRE(((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= d, PM_ERR_INVALID_ARG, "%s: %s rows must start 16-byte aligned, %lld elements apart or more (stride %lld)", who, name,
+             (long long)d, (long long)ld);
+  return PM_OK;
+}
+
+}  // namespace lora
+}  // namespace pm
+
+using namespace pm;
+using namespace pm::lora;
+
+#define PM_TRY(call)              \
+  do {                            \
+    const int _rc = (call);       \
+    if (_rc != PM_OK) return _rc; \
+  } while (0)
+
+extern "C" int64_t pm_lora_z_columns(int32_t rank) { return rank >= 1 && rank <= kMaxRank ? padded_rank(rank) : 0; }
+
+extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank) {
+  if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
+  const int parts = shrink_parts(n_rows, n_adapters, (int)d_in, rank);
+  return parts > 1 ? (int64_t)parts * n_rows * padded_rank(rank) * 4 : 0;
+}
+
+extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void* b, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n_rows,
+                           int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base, int64_t ldbase, void* out, int64_t ldout, float* z, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  PM_TRY(check_shape("pm_lora_fwd", n_rows, n_adapters, d_in, d_out, rank));
+  if (n_rows == 0) return PM_OK;
+  PM_REQUIRE(a && b && scales && offsets && z, PM_ERR_INVALID_ARG, "pm_lora_fwd: null pointer");
+  PM_TRY(check_rows("pm_lora_fwd", "x", x, ldx, d_in));
+  PM_TRY(check_rows("pm_lora_fwd", "out", out, ldout, d_out));
+  if (base) PM_TRY(check_rows("pm_lora_fwd", "base", base, ldbase, d_out));
+  PM_REQUIRE(base != out || ldbase == ldout, PM_ERR_INVALID_ARG, "pm_lora_fwd: base and out are the same rows with different strides");
+  PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
+  const int parts = shrink_parts(n_rows, n_adapters, (int)d_in, rank);
+  const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, rank);
+  PM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PM_ERR_WORKSPACE, "pm_lora_fwd: workspace of %lld bytes, %lld needed",
+             (long long)workspace_bytes, (long long)need);
+  hipStream_t st = as_stream(stream);
+  float* zs = parts > 1 ? (float*)workspace : z;
+  PM_BY_RANK(rank, (launch_shrink<RT>(x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, parts, zs, st)));
+  PM_CHECK_LAUNCH("pm_lora_fwd");
+  PM_BY_RANK(rank, (launch_expand<RT, false>(zs, parts, parts > 1 ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, st)));
+  PM_CHECK_LAUNCH("pm_lora_fwd");
+  return PM_OK;
+}
+
+namespace {
+struct BwdPlan {
+  int parts, rows;
+  int64_t tiles, dz_bytes, part0_bytes, part1_bytes;
+};
+BwdPlan bwd_plan(int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int rank) {
+  BwdPlan p;
+  p.parts = shrink_parts(n, n_adapters, (int)d_out, rank);
+  p.rows = outer_rows(n, (int)d_in, (int)d_out, rank);
+  p.tiles = max_tiles(n, n_adapters, p.rows);
+  p.dz_bytes = (int64_t)p.parts * n * padded_rank(rank) * 4;
+  p.part0_bytes = p.tiles * rank * d_out * 4;
+  p.part1_bytes = p.tiles * rank * d_in * 4;
+  return p;
+}
+}  // namespace
+
+extern "C" int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank) {
+  if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
+  const BwdPlan p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank);
+  return p.dz_bytes + p.part0_bytes + p.part1_bytes;
+}
+
+extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, const float* z, const void* a, const void* b, const float* scales, const int32_t* offsets,
+                           const int32_t* row_ids, int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base, int64_t ldbase, void* grad_x,
+                           int64_t ldgx, float* grad_a, float* grad_b, int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
+  PM_TRY(check_shape("pm_lora_bwd", n_rows, n_adapters, d_in, d_out, rank));
+  PM_REQUIRE((grad_a != nullptr) == (grad_b != nullptr), PM_ERR_INVALID_ARG, "pm_lora_bwd: grad_a and grad_b go together");
+  PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z | (uintptr_t)grad_a | (uintptr_t)grad_b) & 15) == 0, PM_ERR_INVALID_ARG,
+             "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
+  PM_REQUIRE(offsets, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
+  hipStream_t st = as_stream(stream);
+  BwdPlan p{1, 64, 0, 0, 0, 0};
+  unsigned char* ws = (unsigned char*)workspace;
+  if (n_rows > 0) {
+    PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
+    PM_TRY(check_rows("pm_lora_bwd", "grad_out", grad_out, ldg, d_out));
+    if (grad_x) PM_TRY(check_rows("pm_lora_bwd", "grad_x", grad_x, ldgx, d_in));
+    if (base) PM_TRY(check_rows("pm_lora_bwd", "base", base, ldbase, d_in));
+    PM_REQUIRE(!grad_x || base != grad_x || ldbase == ldgx, PM_ERR_INVALID_ARG, "pm_lora_bwd: base and grad_x are the same rows with different strides");
+    if (grad_a) {
+      PM_REQUIRE(z, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer (z)");
+      PM_TRY(check_rows("pm_lora_bwd", "x", x, ldx, d_in));
+    }
+    p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank);
+    const int64_t need = p.dz_bytes + p.part0_bytes + p.part1_bytes;
+    PM_REQUIRE(ws && workspace_bytes >= need && ((uintptr_t)ws & 15) == 0, PM_ERR_WORKSPACE, "pm_lora_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+               (long long)need);
+    float* dz = (float*)ws;
+    PM_BY_RANK(rank, (launch_shrink<RT>(grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, p.parts, dz, st)));
+    PM_CHECK_LAUNCH("pm_lora_bwd");
+    if (grad_x) {
+      PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
+      PM_CHECK_LAUNCH("pm_lora_bwd");
+    }
+  }
+  if (!grad_a) return PM_OK;
+  float *part0 = (float*)(ws + p.dz_bytes), *part1 = (float*)(ws + p.dz_bytes + p.part0_bytes);
+  if (p.tiles > 0) {
+    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
+    const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
+    PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)p.tiles, t0 + t1), dim3(256), 0, st, s0, s1, t0, offsets, row_ids, (int)n_rows, n_adapters, rank,
+                                        padded_rank(rank), p.rows));
+    PM_CHECK_LAUNCH("pm_lora_bwd");
+  }
+  const int64_t e0 = rank * d_out, e1 = rank * d_in;
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, n_adapters, p.rows,
+                     (int)p.tiles, accumulate);
+  PM_CHECK_LAUNCH("pm_lora_bwd");
+  return PM_OK;
+}
+
+extern "C" int pm_lora_merge(const void* weight, int64_t ldw, const void* a, const void* b, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out, int64_t ldo,
+                             void* stream) {
+  PM_TRY(check_shape("pm_lora_merge", d_out, 1, d_in, d_out, rank));
+  PM_REQUIRE(a && b, PM_ERR_INVALID_ARG, "pm_lora_merge: null pointer");
+  PM_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_merge: a and b must be 16-byte aligned");
+  PM_TRY(check_rows("pm_lora_merge", "weight", weight, ldw, d_in));
+  PM_TRY(check_rows("pm_lora_merge", "out", out, ldo, d_in));
+  PM_BY_RANK(rank, (launch_expand<RT, true>(nullptr, 0, nullptr, b, scale, a, nullptr, nullptr, d_out, 1, (int)d_in, rank, weight, ldw, out, ldo, as_stream(stream))));
+  PM_CHECK_LAUNCH("pm_lora_merge");
+  return PM_OK;
+}

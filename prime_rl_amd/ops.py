@@ -1078,3 +1078,253 @@ def gemm_set_variant(v: int) -> None:
             raise PrimeMI355XError(f"gemm_set_variant({v}): this schedule exists only in a `make VARIANTS=1` build")
         lib.pm_gemm_debug_set_variant(-1)
     _default_sched = GEMM_SCHED_DEFAULT if v in (7, -1) else int(v)
+
+
+# ------------------------------------------------------------------------------------------------ adapters of many runs
+def _one_device(what: str, *tensors: Tensor | None) -> torch.device:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise PrimeMI355XError(f"{what}: expected all tensors on one GPU, got {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _launch(fn, what: str, device: torch.device, *args) -> None:
+    """The call on the current stream of the tensors' device, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, _stream()), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream()), what)
+
+
+def _lora_rows(t: Tensor, rows: int, width: int, name: str) -> int:
+    """Row stride of a [rows, width] bf16 tensor whose rows lie one behind the other, with or without a gap."""
+    _req(t, torch.bfloat16, name, contiguous=False)
+    if t.dim() != 2 or t.shape != (rows, width):
+        raise PrimeMI355XError(f"{name}: expected [{rows}, {width}], got {tuple(t.shape)}")
+    if rows == 0:
+        return width
+    if t.stride(1) != 1 or (rows > 1 and (t.stride(0) < width or t.stride(0) % 8)) or t.data_ptr() % 16:
+        raise PrimeMI355XError(f"{name}: rows must be contiguous, start 16-byte aligned and not overlap, got strides {t.stride()}")
+    return t.stride(0) if rows > 1 else width
+
+
+def _share_memory(a: Tensor, b: Tensor) -> bool:
+    """Whether two 2-D bf16 row tensors have an element in common (column slices of one buffer have none)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    lo_a, lo_b = a.data_ptr() // 2, b.data_ptr() // 2
+    hi_a, hi_b = (t + (u.shape[0] - 1) * u.stride(0) + u.shape[1] for t, u in ((lo_a, a), (lo_b, b)))
+    if hi_a <= lo_b or hi_b <= lo_a:
+        return False
+    ld = a.stride(0)
+    if a.shape[0] > 1 and b.shape[0] > 1 and ld == b.stride(0):
+        at = (lo_b - lo_a) % ld
+        return at < a.shape[1] or ld - at < b.shape[1]
+    return True
+
+
+def _lora_factors(a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, row_ids: Tensor | None, rows: int) -> tuple[int, int, int, int]:
+    _req(a, torch.bfloat16, "a"); _req(b, torch.bfloat16, "b")
+    if a.dim() != 3 or b.dim() != 3 or a.shape[:2] != b.shape[:2]:
+        raise PrimeMI355XError(f"a / b: expected [n_adapters, rank, d_in] and [n_adapters, rank, d_out], got {tuple(a.shape)} and {tuple(b.shape)}")
+    n, rank, d_in = a.shape
+    _req(scales, torch.float32, "scales"); _req(offsets, torch.int32, "offsets")
+    if scales.numel() != n or offsets.numel() != n + 1:
+        raise PrimeMI355XError(f"{n} adapters: expected {n} scales and {n + 1} offsets, got {scales.numel()} and {offsets.numel()}")
+    if row_ids is not None:
+        _req(row_ids, torch.int32, "row_ids")
+        if row_ids.numel() != rows:
+            raise PrimeMI355XError(f"row_ids: expected one for each of {rows} rows, got {row_ids.numel()}")
+    return n, rank, d_in, b.shape[2]
+
+
+def lora_rows(adapter_ids: Tensor, n_adapters: int) -> tuple[Tensor, Tensor]:
+    """(offsets [n_adapters + 1], row_ids [N]) of rows in any order, `adapter_ids` [N] holding each row's adapter; an id outside [0, n_adapters) is a row of no
+    adapter.  Rows of one adapter keep their order."""
+    ids = _req(adapter_ids, None, "adapter_ids").reshape(-1).to(torch.int64)
+    ids = torch.where((ids >= 0) & (ids < n_adapters), ids, n_adapters)
+    ids, order = torch.sort(ids, stable=True)  # plumbing: index sort only
+    return torch.searchsorted(ids, torch.arange(n_adapters + 1, device=ids.device)).to(torch.int32), order.to(torch.int32)
+
+
+def lora_fwd(x: Tensor, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, base: Tensor | None = None, row_ids: Tensor | None = None,
+             out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """(out, z) of the low-rank update beside a shared projection: out[row] = base[row] + scales[g] * (x[row] @ a[g].T) @ b[g] for the rows of adapter g, the
+    base's row for rows of no adapter (pm_lora_fwd).
+
+    x [N, d_in], base [N, d_out] (None: zeros) bf16, with row strides; a [n, rank, d_in], b [n, rank, d_out] bf16; scales [n] f32.  Position p, in
+    [offsets[g], offsets[g + 1]) of adapter g, is row `row_ids[p]` (`lora_rows`), or row p without row_ids.  `out` may be `base` (in place).  z is what `lora_bwd` takes."""
+    lib = _lib.load()
+    if x.dim() != 2:
+        raise PrimeMI355XError(f"x: expected [rows, d_in], got {tuple(x.shape)}")
+    rows = x.shape[0]
+    n, rank, d_in, d_out = _lora_factors(a, b, scales, offsets, row_ids, rows)
+    ldx = _lora_rows(x, rows, d_in, "x")
+    ldb = _lora_rows(base, rows, d_out, "base") if base is not None else 0
+    if out is None:
+        out = torch.empty((rows, d_out), dtype=torch.bfloat16, device=x.device)
+    ldo = _lora_rows(out, rows, d_out, "out")
+    device = _one_device("lora_fwd", x, a, b, scales, offsets, row_ids, base, out)
+    if base is not None and not (base.data_ptr() == out.data_ptr() and ldb == ldo) and _share_memory(base, out):
+        raise PrimeMI355XError("out overlaps base: it may be base itself or memory of its own")
+    z = torch.empty((rows, lib.pm_lora_z_columns(rank)), dtype=torch.float32, device=device)
+    nbytes = lib.pm_lora_fwd_workspace_bytes(rows, n, d_in, rank)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None  # of its own for each call: a captured graph keeps it
+    _launch(lib.pm_lora_fwd, "pm_lora_fwd", device, _p(x), ldx, _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb, _p(out), ldo, _p(z),
+            _p(ws), nbytes)
+    return out, z
+
+
+def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, base: Tensor | None = None,
+             row_ids: Tensor | None = None, grad_x: Tensor | None = None, grad_a: Tensor | None = None, grad_b: Tensor | None = None, accumulate: bool = False,
+             want_x: bool = True, want_factors: bool = True) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """(grad_x, grad_a, grad_b) of `lora_fwd` (pm_lora_bwd): with dz = scales[g] * grad_out[row] @ b[g].T, grad_x[row] = base[row] + dz @ a[g] (base: the shared
+    projection's row gradient, None: zeros; `grad_x` may be `base`), grad_a[g] = dz.T @ x, grad_b[g] = z.T @ grad_out in f32 — written, or added to the given
+    buffers with `accumulate`.  What is not wanted (`want_x`, `want_factors`) comes back as None; without the factors' gradients x and z may be None."""
+    lib = _lib.load()
+    if grad_out.dim() != 2:
+        raise PrimeMI355XError(f"grad_out: expected [rows, d_out], got {tuple(grad_out.shape)}")
+    rows = grad_out.shape[0]
+    n, rank, d_in, d_out = _lora_factors(a, b, scales, offsets, row_ids, rows)
+    ldg = _lora_rows(grad_out, rows, d_out, "grad_out")
+    ldx = ldb = ldgx = 0
+    if want_factors:
+        if x is None or z is None:
+            raise PrimeMI355XError("the factors' gradients need x and the forward's z")
+        ldx = _lora_rows(x, rows, d_in, "x")
+        _req(z, torch.float32, "z")
+        if z.shape != (rows, lib.pm_lora_z_columns(rank)):
+            raise PrimeMI355XError(f"z: expected {(rows, lib.pm_lora_z_columns(rank))} as lora_fwd returns it, got {tuple(z.shape)}")
+        if (grad_a is None) != (grad_b is None) or (accumulate and grad_a is None):
+            raise PrimeMI355XError("grad_a and grad_b go together, and accumulating needs them")
+        if grad_a is None:
+            grad_a, grad_b = (torch.empty(t.shape, dtype=torch.float32, device=grad_out.device) for t in (a, b))
+        for t, of, nm in ((grad_a, a, "grad_a"), (grad_b, b, "grad_b")):
+            _req(t, torch.float32, nm)
+            if t.shape != of.shape:
+                raise PrimeMI355XError(f"{nm}: expected {tuple(of.shape)}, got {tuple(t.shape)}")
+    else:
+        x = z = grad_a = grad_b = None
+    if want_x:
+        ldb = _lora_rows(base, rows, d_in, "base") if base is not None else 0
+        if grad_x is None:
+            grad_x = torch.empty((rows, d_in), dtype=torch.bfloat16, device=grad_out.device)
+        ldgx = _lora_rows(grad_x, rows, d_in, "grad_x")
+        if base is not None and not (base.data_ptr() == grad_x.data_ptr() and ldb == ldgx) and _share_memory(base, grad_x):
+            raise PrimeMI355XError("grad_x overlaps base: it may be base itself or memory of its own")
+        if want_factors and (_share_memory(grad_x, grad_out) or _share_memory(grad_x, x)):
+            raise PrimeMI355XError("grad_x overlaps grad_out or x, which are still read after it is written")
+    else:
+        base = grad_x = None
+    device = _one_device("lora_bwd", grad_out, x, z, a, b, scales, offsets, row_ids, base, grad_x, grad_a, grad_b)
+    nbytes = lib.pm_lora_bwd_workspace_bytes(rows, n, d_in, d_out, rank)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch(lib.pm_lora_bwd, "pm_lora_bwd", device, _p(grad_out), ldg, _p(x), ldx, _p(z), _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb,
+            _p(grad_x), ldgx, _p(grad_a), _p(grad_b), 1 if accumulate else 0, _p(ws), nbytes)
+    return grad_x, grad_a, grad_b
+
+
+def lora_merge(weight: Tensor, a: Tensor, b: Tensor, scale: float, out: Tensor | None = None) -> Tensor:
+    """weight + scale * b.T @ a, rounded once: ONE adapter (a [rank, d_in], b [rank, d_out], bf16) folded into its projection's weight [d_out, d_in] bf16
+    (pm_lora_merge), as the weight push sends it.  `out` may be `weight`."""
+    lib = _lib.load()
+    _req(a, torch.bfloat16, "a"); _req(b, torch.bfloat16, "b")
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[0]:
+        raise PrimeMI355XError(f"a / b: expected [rank, d_in] and [rank, d_out], got {tuple(a.shape)} and {tuple(b.shape)}")
+    (rank, d_in), d_out = a.shape, b.shape[1]
+    ldw = _lora_rows(weight, d_out, d_in, "weight")
+    if out is None:
+        out = torch.empty((d_out, d_in), dtype=torch.bfloat16, device=weight.device)
+    ldo = _lora_rows(out, d_out, d_in, "out")
+    device = _one_device("lora_merge", weight, a, b, out)
+    if not (weight.data_ptr() == out.data_ptr() and ldw == ldo) and _share_memory(weight, out):
+        raise PrimeMI355XError("out overlaps weight: it may be weight itself or memory of its own")
+    _launch(lib.pm_lora_merge, "pm_lora_merge", device, _p(weight), ldw, _p(a), _p(b), float(scale), d_in, d_out, rank, _p(out), ldo)
+    return out
+
+
+class GradClipPlan:
+    """The gradient norm of many tensors, by group, and clipping (pm_grad_clip): what `clip_coef` is to one flat buffer.
+
+    `grads`: contiguous f32 | bf16 GPU tensors; `groups[i]` in [0, n_groups) is the group of grads[i] (None: one group).  `out[i]`, f32 | bf16 of the same size,
+    receives the clipped grads[i] — e.g. a slice of the flat f32 gradient that `adamw_step` reads; without `out` the gradients are clipped in place.  The plan
+    holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are."""
+
+    _CHUNK_MOST, _CHUNK_LEAST = 32768, 2048
+
+    def __init__(self, grads: list[Tensor], groups: list[int] | None = None, n_groups: int | None = None, out: list[Tensor] | None = None):
+        import numpy as np
+
+        groups = [0] * len(grads) if groups is None else [int(g) for g in groups]
+        self.n_groups = n_groups if n_groups is not None else max(groups, default=0) + 1
+        if len(groups) != len(grads) or self.n_groups < 1 or any(g < 0 or g >= self.n_groups for g in groups):
+            raise PrimeMI355XError(f"groups: expected one in [0, {self.n_groups}) for each of {len(grads)} gradients")
+        dst = grads if out is None else out
+        if len(dst) != len(grads):
+            raise PrimeMI355XError(f"out: expected {len(grads)} tensors, got {len(dst)}")
+        for i, (t, o) in enumerate(zip(grads, dst)):
+            for u, nm in ((t, "grads"), (o, "out")):
+                _req(u, None, f"{nm}[{i}]")
+                if u.dtype not in _DT:
+                    raise PrimeMI355XError(f"{nm}[{i}]: dtype {u.dtype} unsupported (f32 | bf16)")
+            if o.numel() != t.numel():
+                raise PrimeMI355XError(f"out[{i}]: {o.numel()} elements for a gradient of {t.numel()}")
+            if t.numel() and o.data_ptr() == t.data_ptr() and o.dtype != t.dtype:
+                raise PrimeMI355XError(f"out[{i}]: in place only in the gradient's own type")
+        if not grads:
+            raise PrimeMI355XError("grads: no tensors")
+        self.device = _one_device("GradClipPlan", *grads, *dst)
+        self._held = [t.detach() for t in (*grads, *dst)]
+        src = np.array([(t.data_ptr(), t.numel() * t.element_size(), i) for i, t in enumerate(grads) if t.numel()], dtype=np.int64).reshape(-1, 3)
+        own = np.array([(o.data_ptr(), o.numel() * o.element_size(), i) for i, o in enumerate(dst) if o.numel()], dtype=np.int64).reshape(-1, 3)
+        spans = src if out is None else np.concatenate([src, own[own[:, 0] != src[:, 0]]])
+        spans = spans[np.argsort(spans[:, 0], kind="stable")]
+        if np.any(spans[1:, 0] < spans[:-1, 0] + spans[:-1, 1]):
+            raise PrimeMI355XError("gradients (or their outputs) overlap in memory: each may be there once")
+        # chunks: of 32 Ki elements, fewer where there is less to share out among the CUs; a group's chunks stand together
+        numel = np.array([t.numel() for t in grads], dtype=np.int64)
+        self.chunk = int(min(self._CHUNK_MOST, max(self._CHUNK_LEAST, -(-int(numel.sum()) // 1024) // 1024 * 1024)))
+        order = np.argsort(np.array(groups), kind="stable")
+        count = -(-numel[order] // self.chunk)
+        of = np.repeat(order, count)
+        first = (np.arange(of.size) - np.repeat(np.cumsum(count) - count, count)) * self.chunk
+        size = [np.array([t.element_size() for t in ts], dtype=np.int64) for ts in (grads, dst)]
+        at = [np.array([t.data_ptr() for t in ts], dtype=np.int64) for ts in (grads, dst)]
+        flags = np.array(groups, dtype=np.int64) * 256 + (size[0] == 2) + 2 * (size[1] == 2)
+        table = np.stack([at[0][of] + first * size[0][of], at[1][of] + first * size[1][of], np.minimum(self.chunk, numel[of] - first), flags[of]], axis=1)
+        self.n_chunks = int(of.size)
+        self._table = torch.from_numpy(np.ascontiguousarray(table)).to(self.device)
+        self._offsets = torch.from_numpy(np.searchsorted(np.array(groups, dtype=np.int64)[of], np.arange(self.n_groups + 1)).astype(np.int32)).to(self.device)
+
+    def _run(self, max_norm, sumsq: Tensor | None, want_sumsq: bool, scale: bool) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+        lib = _lib.load()
+        limits = None
+        if isinstance(max_norm, Tensor):
+            limits = _req(max_norm, torch.float32, "max_norm")
+        if sumsq is not None:
+            _req(sumsq, torch.float64, "sumsq")
+        for t, nm in ((limits, "max_norm"), (sumsq, "sumsq")):
+            if t is not None and (t.numel() != self.n_groups or t.device != self.device):
+                raise PrimeMI355XError(f"{nm}: expected {self.n_groups} values on {self.device}, got {t.numel()} on {t.device}")
+        partials = torch.empty(max(self.n_chunks, 1), dtype=torch.float64, device=self.device) if sumsq is None else None
+        sums = torch.empty(self.n_groups, dtype=torch.float64, device=self.device) if want_sumsq else None
+        both = None if want_sumsq else torch.empty((2, self.n_groups), dtype=torch.float32, device=self.device)
+        norms, coefs = (None, None) if both is None else (both[0], both[1])
+        _launch(lib.pm_grad_clip, "pm_grad_clip", self.device, _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(sumsq), 0.0 if limits is not None else float(max_norm),
+                _p(limits), _p(partials), _p(sums), _p(norms), _p(coefs), 1 if scale else 0)
+        return sums, norms, coefs
+
+    def sumsq(self) -> Tensor:
+        """Sum of squares of each group, f64 [n_groups]: what ranks that hold parts of one gradient add up and hand to `clip`."""
+        return self._run(0.0, None, True, False)[0]
+
+    def coefs(self, max_norm: float | Tensor, sumsq: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """(coefs, norms) [n_groups] f32 and no scaling: `coefs[g:g + 1]` is the `clip` of `adamw_step`."""
+        _, norms, coefs = self._run(max_norm, sumsq, False, False)
+        return coefs, norms
+
+    def clip(self, max_norm: float | Tensor, sumsq: Tensor | None = None) -> Tensor:
+        """Scales every gradient by min(1, max_norm / (norm of its group + 1e-6)) into `out` (or in place) and returns the norms [n_groups] f32 before clipping.
+        `max_norm`: one for all groups or f32 [n_groups]; 0: no clipping.  `sumsq`: the groups' sums of squares where they are known already."""
+        return self._run(max_norm, sumsq, False, True)[1]
