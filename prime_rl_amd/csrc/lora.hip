@@ -141,6 +141,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const bf16_t* __restrict__ 
 #pragma unroll
         for (int j = 0; j < RT; ++j) wf[u][h][j] = *reinterpret_cast<const u32x4*>(wp[j] + k);
       }
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight: left alone, the compiler takes them one step at a time to save registers
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -216,12 +217,14 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
   using S = ExpandShape<RT>;
   __shared__ __attribute__((aligned(16))) unsigned char tile[RT * 16 * S::kStride];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-  int adapter = 0, p0 = blockIdx.x * kExpandRows, p1 = min(p0 + kExpandRows, n);
+  // column tiles run fastest: workgroups that run together cover whole rows (a 64 x 512 tile copy: 5.5 TB/s against 4.2 with row tiles fastest)
+  const int col_tiles = (d + S::kCols - 1) / S::kCols, row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x % col_tiles;
+  int adapter = 0, p0 = row_tile * kExpandRows, p1 = min(p0 + kExpandRows, n);
   if constexpr (!MERGE) {
-    if (!locate(offsets, n_adapters, n, kExpandRows, blockIdx.x, lane, adapter, p0, p1)) return;
+    if (!locate(offsets, n_adapters, n, kExpandRows, row_tile, lane, adapter, p0, p1)) return;
     if (adapter < 0 && in_place) return;
   }
-  const int c0 = blockIdx.y * S::kCols;
+  const int c0 = col_tile * S::kCols;
   // the factor tile, rows past the rank and columns past the end as zeros
   constexpr int kPieces = RT * 16 * S::kCols / 8 / 256;
   u32x4 stage[kPieces];
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
               if (r + q < rank) v[h][q] = merge_scale * bf16_to_f32(zb[(int64_t)(r + q) * n + p]);
           } else if (r < rp) {
             for (int part = 0; part < parts; ++part) v[h] += *reinterpret_cast<const f32x4*>(z + ((int64_t)part * n + p) * rp + r);
-            if (z_out && blockIdx.y == 0 && wave == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = v[h];
+            if (z_out && col_tile == 0 && wave == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = v[h];
           }
         }
         const u32x2 lead0 = take_terms(v[0]), rest0 = to_bf16(v[0]);
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 
 // ---------------------------------------------------------------------------------------------------------------------
 // outer: part[tile][r][c] = sum over the tile's positions of z[p][r] * t[row(p)][c], one f32 partial per tile of `rows` positions of one adapter.
-// Both products of the backward (dB from z and dy, dA from dz and x) are one launch: blockIdx.y runs over the 256-column tiles of dy, then of x.
+// Both products of the backward (dB from z and dy, dA from dz and x) are one launch: the column tiles run over the 256-column tiles of dy, then of x.
 // The positions are the contraction, so both operands are read transposed: stages of SP positions go through LDS (t as it is, z split into three bf16
 // planes), the next stage's loads are in flight while the matrix cores work on this one.  A wave takes 64 columns and all ranks.
 struct OuterSide {
@@ -345,7 +348,7 @@ struct OuterSide {
 };
 
 template <int RT>
-__global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+__global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
                                                        int n_adapters, int rank, int rp, int rows) {
   constexpr int SP = RT <= 2 ? 64 : 32;           // positions per stage
   constexpr int kTs = kOuterCols * 2 + 32;        // row strides in LDS: 32 bytes of shift per row keep transposed reads off each other's banks
@@ -355,11 +358,12 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s
   __shared__ __attribute__((aligned(16))) unsigned char lt[SP * kTs];
   __shared__ __attribute__((aligned(16))) unsigned char lz[3][SP * kZs];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-  const bool second = (int)blockIdx.y >= tiles0;
+  const int row_tile = blockIdx.x / tiles01, col_tile = blockIdx.x % tiles01;  // columns fastest, as in expand
+  const bool second = col_tile >= tiles0;
   const OuterSide s = second ? s1 : s0;
-  const int c0 = (second ? blockIdx.y - tiles0 : blockIdx.y) * kOuterCols;
+  const int c0 = (second ? col_tile - tiles0 : col_tile) * kOuterCols;
   int adapter, p0, p1;
-  if (!locate(offsets, n_adapters, n, rows, blockIdx.x, lane, adapter, p0, p1) || adapter < 0) return;
+  if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
   u32x4 tv[kTp];
   f32x4 zv[kZp];
   auto load = [&](int ps) {
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s
     }
     __syncthreads();
   }
-  float* part = s.part + (int64_t)blockIdx.x * rank * s.d;
+  float* part = s.part + (int64_t)row_tile * rank * s.d;
 #pragma unroll
   for (int j = 0; j < RT; ++j) {
     const int r = j * 16 + lr;
@@ -510,8 +514,8 @@ template <int RT, bool MERGE>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
                           int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t stream) {
   const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
-  const dim3 grid((unsigned)tiles, (unsigned)cdiv(d, ExpandShape<RT>::kCols));
-  hipLaunchKernelGGL((expand_kernel<RT, MERGE>), grid, dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
+  const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
+  hipLaunchKernelGGL((expand_kernel<RT, MERGE>), dim3(grid), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
                      d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0);
 }
 #define PM_BY_RANK(rank, CALL)          \
@@ -642,7 +646,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
   if (p.tiles > 0) {
     const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
     const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
-    PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)p.tiles, t0 + t1), dim3(256), 0, st, s0, s1, t0, offsets, row_ids, (int)n_rows, n_adapters, rank,
+    PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(p.tiles * (t0 + t1))), dim3(256), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids, (int)n_rows, n_adapters, rank,
                                         padded_rank(rank), p.rows));
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
