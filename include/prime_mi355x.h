@@ -560,7 +560,7 @@ int pm_gemm_debug_set_variant(int32_t value);
 
 /* --------------------------------------------------------------------------------------------
  * Low-rank adapters of many runs beside a shared projection, and their gradients' norm.  Stands where the reference keeps one LoRA adapter per run in its
- * linear layers (models/layers/lora/*, rows split by the micro-batch's lora_num_tokens, trainer/rl/data.py:18-52) and clips each run's gradients
+ * linear layers (models/layers/lora, rows split by the micro-batch's lora_num_tokens, trainer/rl/data.py:18-52) and clips each run's gradients
  * (trainer/utils.py:88-98).
  *
  * Rows are grouped by adapter: adapter g owns the POSITIONS [offsets[g], offsets[g+1]) (int32 [n_adapters + 1] on the device, offsets[0] = 0, not decreasing);

@@ -24,6 +24,8 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16_t* lds_v4i16_ptr;
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+typedef __attribute__((address_space(1))) void* glb_void_ptr;
 
 constexpr int kMaxRank = 128;
 constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
@@ -90,108 +92,206 @@ static inline int64_t max_tiles(int64_t n, int64_t n_adapters, int64_t rows) {
   return t < n ? t : n;
 }
 
-__device__ __forceinline__ int64_t row_of(const int32_t* __restrict__ row_ids, int p, int n) {
-  return row_ids ? min(max(row_ids[p], 0), n - 1) : p;
+// rows of the positions p[0 .. N): the ids are asked for together
+template <int N>
+__device__ __forceinline__ void rows_of(const int32_t* __restrict__ row_ids, const int (&p)[N], int n, int (&row)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) row[i] = p[i];
+  if (row_ids) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] = row_ids[p[i]];
+#pragma unroll
+    for (int i = 0; i < N; ++i) row[i] = min(max(row[i], 0), n - 1);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // shrink: z[part][p][r] = scale * sum over the part's columns of t[row(p)][k] * w[adapter][r][k].
-// A workgroup takes 16 * MT positions and one part of the long axis; its four waves take every fourth 64-column step (128 bytes of each row: whole cache
-// lines) and wave 0 adds the four results up through LDS.  The fragments of v_mfma_f32_16x16x32_bf16 come straight from global memory: rows of the factor
-// (from L2, where it stays) as the A operand, rows of t as the B operand.  Positions past the tile's end repeat its first row and are not stored.
-template <int RT, int MT, int U>
-__global__ __launch_bounds__(256) void shrink_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
-                                                     const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank, int rp,
-                                                     int steps_per_part, float* __restrict__ z) {
-  constexpr int kStride = RT * 16 + 4;
-  __shared__ __attribute__((aligned(16))) float red[3][MT * 16][kStride];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-  int adapter, p0, p1;
-  if (!locate(offsets, n_adapters, n, 16 * MT, blockIdx.x, lane, adapter, p0, p1) || adapter < 0) return;
-  const bf16_t* tp[MT];
-  const bf16_t* wp[RT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int p = p0 + i * 16 + lr;
-    tp[i] = t + row_of(row_ids, p < p1 ? p : p0, n) * ldt + lq * 8;
+// Chunks of columns of a tile's rows and of the factor come into LDS by DMA (global_load_lds: no registers, and one instruction takes whole stretches of a
+// row), a ring of three deep, so that two are in flight while the matrix cores work on one.  16-byte slots of a row are permuted by its row number: the 16 rows
+// of a fragment read lie in different banks.  The factor's chunk is read once for each tile (from L2), which bounds how small a tile may be.
+// All tiles run at once and walk the columns together.  Each begins at a chunk of its own: in step they would ask for the same columns of every row, which lie on few
+// of the memory channels (reading 32 768 x 4096 this way: 63 us in step, 46 with the turn; a linear read takes 44).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// at most n DMA instructions of this wave outstanding
+__device__ __forceinline__ void wait_dma(int n) {
+  switch (n) {
+#define PM_CASE(N) case N: asm volatile("s_waitcnt vmcnt(" #N ")" ::: "memory"); break;
+    PM_CASE(2) PM_CASE(3) PM_CASE(4) PM_CASE(5) PM_CASE(6) PM_CASE(7) PM_CASE(8) PM_CASE(9) PM_CASE(10) PM_CASE(11) PM_CASE(12) PM_CASE(13) PM_CASE(14)
+#undef PM_CASE
+    default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
   }
+}
+__device__ __forceinline__ void dma16(const bf16_t* from, unsigned char* to) { __builtin_amdgcn_global_load_lds((glb_void_ptr)from, (lds_void_ptr)to, 16, 0, 0); }
+
+// The ring: chunk i of `count` is chunk turn + i of the part's full ones (round and round), the last, shorter one stays last and comes through registers.
+// NT + NW instructions of a wave fill a chunk: instruction i of t (i < nt) takes tp[i] to to + i * 4 KiB, of w to `wofs` behind that.
+template <int KC, int NT, int NW>
+struct Ring {
+  const bf16_t* tp[NT];  // this lane's 16 bytes of chunk 0
+  const bf16_t* wp[NW];
+  int tcol[NT], wcol[NW], nt, wofs, c0, full, turn, d;
+  __device__ __forceinline__ void fetch(int c, unsigned char* to, int lane) const {
+    if (c < full) {
+      const int k = (c0 + (c + turn < full ? c + turn : c + turn - full)) * KC;
 #pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const int r = j * 16 + lr;
-    wp[j] = w + ((int64_t)adapter * rank + (r < rank ? r : 0)) * d + lq * 8;
-  }
-  f32x4 acc[MT][RT];
+      for (int i = 0; i < NT; ++i)
+        if (i < nt) dma16(tp[i] + k, to + i * 4096);
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < NW; ++i) dma16(wp[i] + k, to + wofs + i * 4096);
+    } else {  // columns past the end are zeros
+      const int k = (c0 + c) * KC;
 #pragma unroll
-    for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int s0 = blockIdx.y * steps_per_part;
-  const int s1 = min(s0 + steps_per_part, (d + 63) >> 6);
-  const int full = min(s1, d >> 6);  // steps whose 64 columns all exist
-  int s = s0 + wave;
-  for (; s + 4 * (U - 1) < full; s += 4 * U) {
-    u32x4 tf[U][2][MT], wf[U][2][RT];
+      for (int i = 0; i < NT; ++i)
+        if (i < nt) *reinterpret_cast<u32x4*>(to + i * 4096 + lane * 16) = k + tcol[i] < d ? *reinterpret_cast<const u32x4*>(tp[i] + k) : u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = (s + 4 * u) * 64 + h * 32;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) tf[u][h][i] = *reinterpret_cast<const u32x4*>(tp[i] + k);
-#pragma unroll
-        for (int j = 0; j < RT; ++j) wf[u][h][j] = *reinterpret_cast<const u32x4*>(wp[j] + k);
-      }
-    __builtin_amdgcn_sched_barrier(0);  // all of them in flight: left alone, the compiler takes them one step at a time to save registers
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[u][h][j], tf[u][h][i], acc[i][j]);
-  }
-  for (; s < s1; s += 4) {  // what is left, columns past the end as zeros on both sides
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = s * 64 + h * 32;
-      const bool in = k + lq * 8 < d;
-      u32x4 tf[MT], wf[RT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) tf[i] = in ? *reinterpret_cast<const u32x4*>(tp[i] + k) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < RT; ++j) wf[j] = in ? *reinterpret_cast<const u32x4*>(wp[j] + k) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[j], tf[i], acc[i][j]);
+      for (int i = 0; i < NW; ++i) *reinterpret_cast<u32x4*>(to + wofs + i * 4096 + lane * 16) = k + wcol[i] < d ? *reinterpret_cast<const u32x4*>(wp[i] + k) : u32x4{0, 0, 0, 0};
     }
   }
-  // a lane holds z[position lr][ranks 4 lq .. 4 lq + 3] of every 16 x 16 block
-  if (wave > 0) {
+};
+
+// One instruction fills 1 KiB: kPer rows of KC columns.  Instruction i of wave v is piece 4 i + v.
+template <int KC, int NT, int NW>
+__device__ __forceinline__ void ring_setup(Ring<KC, NT, NW>& ring, const bf16_t* t, int64_t ldt, const bf16_t* w, const int32_t* row_ids, int n, int adapter, int rank, int d, int p0,
+                                           int p1, int nt, int rows_lds, int wave, int lane) {
+  constexpr int kSlots = KC / 8, kPer = 64 / kSlots, kMask = kSlots < 16 ? kSlots - 1 : 15;
+  const int sub = lane / kSlots, slot = lane % kSlots;
+  int pos[NT], row[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < RT; ++j) *reinterpret_cast<f32x4*>(&red[wave - 1][i * 16 + lr][j * 16 + lq * 4]) = acc[i][j];
+  for (int i = 0; i < NT; ++i) {  // positions past the tile's end repeat its first row and are not stored
+    const int p = p0 + (i * 4 + wave) * kPer + sub;
+    pos[i] = p < p1 ? p : p0;
   }
-  __syncthreads();
+  rows_of(row_ids, pos, n, row);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    ring.tcol[i] = (slot ^ (((i * 4 + wave) * kPer + sub) & kMask)) * 8;
+    ring.tp[i] = t + (int64_t)row[i] * ldt + ring.tcol[i];
+  }
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {  // factor rows past the rank repeat the first; what they give is not stored
+    const int r = (i * 4 + wave) * kPer + sub;
+    ring.wcol[i] = (slot ^ (r & kMask)) * 8;
+    ring.wp[i] = w + ((int64_t)adapter * rank + (r < rank ? r : 0)) * d + ring.wcol[i];
+  }
+  ring.nt = nt;
+  ring.wofs = rows_lds * KC * 2;
+  ring.d = d;
+}
+
+// lane -> z of position lr of 16, ranks 4 lq .. 4 lq + 3
+__device__ __forceinline__ void store_z(float* zp, f32x4 v, int p, int p1, int r, int rank, int rp, float scale) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = r + q < rank ? v[q] * scale : 0.f;
+  if (p < p1 && r < rp) *reinterpret_cast<f32x4*>(zp + (int64_t)p * rp + r) = v;
+}
+
+// rank <= 16: 32 positions, chunks of 256 columns; the four waves take 64 columns of a chunk each and add their results up through LDS.
+constexpr int kNarrowRows = 32, kNarrowChunk = 256, kRing = 3;
+__global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
+                                                               const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank,
+                                                               int parts, int chunks_per_part, float* __restrict__ z) {
+  constexpr int kRowBytes = kNarrowChunk * 2, kBytes = (kNarrowRows + 16) * kRowBytes;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kRing * kBytes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+  const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
+  int adapter, p0, p1;
+  if (!locate(offsets, n_adapters, n, kNarrowRows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
+  constexpr int NT = kNarrowRows * kRowBytes / 4096, NW = 16 * kRowBytes / 4096;
+  Ring<kNarrowChunk, NT, NW> ring;
+  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, NT, kNarrowRows, wave, lane);
+  const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + kNarrowChunk - 1) / kNarrowChunk - c0);
+  ring.c0 = c0;
+  ring.full = min(count, d / kNarrowChunk - c0);
+  ring.turn = ring.full > 0 ? row_tile % ring.full : 0;
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  unsigned char* mine = lds + wave * 1024;
+  for (int c = 0; c < kRing - 1 && c < count; ++c) ring.fetch(c, mine + c * kBytes, lane);
+  for (int c = 0, buf = 0; c < count; ++c) {
+    // chunk c has landed once at most the next one's are outstanding; where that one came without DMA, or is none, wait for all
+    wait_dma(c + 1 < ring.full ? NT + NW : 0);
+    lds_barrier();  // chunk c is there for every wave, and every wave is done with chunk c - 1, whose buffer is filled next
+    if (c + kRing - 1 < count) ring.fetch(c + kRing - 1, mine + (buf + kRing - 1 < kRing ? buf + kRing - 1 : buf - 1) * kBytes, lane);
+    const unsigned char* at = lds + buf * kBytes;
+#pragma unroll
+    for (int k = 0; k < kNarrowChunk / 128; ++k) {
+      const int off = lr * kRowBytes + (((wave * (kNarrowChunk / 128) + k) * 4 + lq) ^ lr) * 16;
+      const u32x4 wf = *reinterpret_cast<const u32x4*>(at + kNarrowRows * kRowBytes + off);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i] = mfma(wf, *reinterpret_cast<const u32x4*>(at + i * 16 * kRowBytes + off), acc[i]);
+    }
+    buf = buf + 1 < kRing ? buf + 1 : 0;
+  }
+  lds_barrier();
+  f32x4* red = reinterpret_cast<f32x4*>(lds);
+  if (wave > 0)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) red[((wave - 1) * 2 + i) * 64 + lane] = acc[i];
+  lds_barrier();
   if (wave > 0) return;
   const float scale = scales[adapter];
-  float* zp = z + (int64_t)blockIdx.y * n * rp;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int p = p0 + i * 16 + lr;
+  for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int j = 0; j < RT; ++j) {
-      const int r = j * 16 + lq * 4;
-      f32x4 v = acc[i][j];
-#pragma unroll
-      for (int q = 0; q < 3; ++q) v += *reinterpret_cast<const f32x4*>(&red[q][i * 16 + lr][r]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = r + q < rank ? v[q] * scale : 0.f;
-      if (p < p1 && r < rp) *reinterpret_cast<f32x4*>(zp + (int64_t)p * rp + r) = v;
-    }
+    for (int q = 0; q < 3; ++q) acc[i] += red[(q * 2 + i) * 64 + lane];
+    store_z(z + (int64_t)part * n * 16, acc[i], p0 + i * 16 + lr, p1, lq * 4, rank, 16, scale);
   }
+}
+
+// rank > 16: `rows` positions (a multiple of 16, chosen on the host) up to wide_rows, chunks of KC columns: 64, or 128 for tiles low enough that three such chunks fit the
+// LDS (low tiles need them to keep enough bytes in flight); the waves take every fourth 16 positions and all columns.
+constexpr int wide_rows(int rt, int kc) { return kc == 64 ? 192 : rt <= 4 ? 96 : 64; }
+template <int RT, int KC>
+__global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
+                                                          const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank, int rp,
+                                                          int rows, int parts, int chunks_per_part, float* __restrict__ z) {
+  constexpr int kMost = wide_rows(RT, KC), kRowBytes = KC * 2, kBytes = (kMost + RT * 16) * kRowBytes, kPass = 4 * (512 / KC), NW = RT * 16 / kPass;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kRing * kBytes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+  const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
+  int adapter, p0, p1;
+  if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
+  const int nt = (p1 - p0 + kPass - 1) / kPass;  // instructions of a wave that bring the rows, kPass of them by the four waves
+  Ring<KC, 6, NW> ring;
+  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, nt, kMost, wave, lane);
+  const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + KC - 1) / KC - c0);
+  ring.c0 = c0;
+  ring.full = min(count, d / KC - c0);
+  ring.turn = ring.full > 0 ? row_tile % ring.full : 0;
+  f32x4 acc[3][RT];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  unsigned char* mine = lds + wave * 1024;
+  for (int c = 0; c < kRing - 1 && c < count; ++c) ring.fetch(c, mine + c * kBytes, lane);
+  for (int c = 0, buf = 0; c < count; ++c) {
+    wait_dma(c + 1 < ring.full ? nt + NW : 0);
+    lds_barrier();
+    if (c + kRing - 1 < count) ring.fetch(c + kRing - 1, mine + (buf + kRing - 1 < kRing ? buf + kRing - 1 : buf - 1) * kBytes, lane);
+    const unsigned char* at = lds + buf * kBytes;
+#pragma unroll
+    for (int k = 0; k < KC / 32; ++k) {
+      const int off = lr * kRowBytes + (((k * 4 + lq) ^ (lr & (KC / 8 - 1))) << 4);
+      u32x4 wf[RT];
+#pragma unroll
+      for (int j = 0; j < RT; ++j) wf[j] = *reinterpret_cast<const u32x4*>(at + (kMost + j * 16) * kRowBytes + off);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int group = i * 4 + wave;
+        if (group * 16 >= p1 - p0) break;
+        const u32x4 tf = *reinterpret_cast<const u32x4*>(at + group * 16 * kRowBytes + off);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[j], tf, acc[i][j]);
+      }
+    }
+    buf = buf + 1 < kRing ? buf + 1 : 0;
+  }
+  const float scale = scales[adapter];
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) store_z(z + (int64_t)part * n * rp, acc[i][j], p0 + (i * 4 + wave) * 16 + lr, p1, j * 16 + lq * 4, rank, rp, scale);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -204,6 +304,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(const bf16_t* __restrict__ 
 template <int RT>
 struct ExpandShape {
   static constexpr int kCols = RT == 1 ? 512 : RT == 2 ? 512 : RT == 4 ? 256 : 128;
+  static constexpr int kZStride = RT * 32 + (RT == 4 ? 16 : 32);  // bytes of a row of z's bf16 terms (rank 64: three workgroups still fit a CU's LDS)
   static constexpr int kStride = kCols * 2 + 32;  // bytes; a row shift of 32 bytes spreads the 8 rows that a transposed read takes at once over all banks
   static constexpr int kSteps = RT == 1 ? 1 : RT / 2;  // 32-deep contraction steps over the rank
   static constexpr int kTerms = RT == 1 ? 1 : 2;       // bf16 terms that are operands of their own
@@ -216,6 +317,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
                                                         int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place) {
   using S = ExpandShape<RT>;
   __shared__ __attribute__((aligned(16))) unsigned char tile[RT * 16 * S::kStride];
+  __shared__ __attribute__((aligned(16))) unsigned char lz[2][kExpandRows * S::kZStride];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
   // column tiles run fastest: workgroups that run together cover whole rows (a 64 x 512 tile copy: 5.5 TB/s against 4.2 with row tiles fastest)
   const int col_tiles = (d + S::kCols - 1) / S::kCols, row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x % col_tiles;
@@ -236,43 +338,31 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
     }
   }
   const int tiles16 = (p1 - p0 + 15) >> 4;
-  int64_t row[4];
+  int pos[4], row[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int p = p0 + i * 16 + lr;
-    row[i] = row_of(row_ids, p < p1 ? p : p0, n);
+    pos[i] = p < p1 ? p : p0;
   }
-  u32x4 zf[4][S::kSteps][S::kTerms];
-  if (adapter >= 0) {
+  rows_of(row_ids, pos, n, row);
+  // z, split into its two bf16 terms on the way to LDS
+  constexpr int kZb = (RT * 2 + 3) / 4;
+  f32x4 zv[MERGE ? 1 : RT];  // thread -> 4 ranks of one position, RT times
+  u32x4 zbv[kZb];            // merge: 8 positions of one rank
+  if constexpr (MERGE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = p0 + i * 16 + lr;
+    for (int i = 0; i < kZb; ++i) {
+      const int piece = i * 256 + tid, r = piece >> 3, p = p0 + (piece & 7) * 8;
+      zbv[i] = r < rank && p < p1 ? *reinterpret_cast<const u32x4*>(zb + (int64_t)r * n + p) : u32x4{0, 0, 0, 0};
+    }
+  } else if (adapter >= 0) {
 #pragma unroll
-      for (int k = 0; k < S::kSteps; ++k) {
-        f32x4 v[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          v[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-          const int r = (RT == 1 ? 0 : k * 32 + h * 16) + lq * 4;
-          if (RT == 1 && h == 1) break;
-          if (p >= p1 || i >= tiles16) continue;
-          if constexpr (MERGE) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (r + q < rank) v[h][q] = merge_scale * bf16_to_f32(zb[(int64_t)(r + q) * n + p]);
-          } else if (r < rp) {
-            for (int part = 0; part < parts; ++part) v[h] += *reinterpret_cast<const f32x4*>(z + ((int64_t)part * n + p) * rp + r);
-            if (z_out && col_tile == 0 && wave == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = v[h];
-          }
-        }
-        const u32x2 lead0 = take_terms(v[0]), rest0 = to_bf16(v[0]);
-        if constexpr (RT == 1) {
-          zf[i][k][0] = u32x4{lead0.x, lead0.y, rest0.x, rest0.y};
-        } else {
-          const u32x2 lead1 = take_terms(v[1]), rest1 = to_bf16(v[1]);
-          zf[i][k][0] = u32x4{lead0.x, lead0.y, lead1.x, lead1.y};
-          zf[i][k][S::kTerms - 1] = u32x4{rest0.x, rest0.y, rest1.x, rest1.y};
-        }
+    for (int i = 0; i < RT; ++i) {
+      const int piece = i * 256 + tid, p = p0 + piece / (RT * 4), r = piece % (RT * 4) * 4;
+      zv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p < p1 && r < rp) {
+        for (int part = 0; part < parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(z + ((int64_t)part * n + p) * rp + r);
+        if (z_out && col_tile == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = zv[i];
       }
     }
   }
@@ -281,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
   for (int b = 0; b < S::kBlocks; ++b) {
     const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bv[b][i] = base && c < d && i < tiles16 ? *reinterpret_cast<const u32x4*>(base + row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+    for (int i = 0; i < 4; ++i) bv[b][i] = base && c < d && i < tiles16 ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
   }
   if (adapter < 0) {  // rows of no adapter
 #pragma unroll
@@ -289,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
       const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + row[i] * ldo + c) = bv[b][i];
+        if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = bv[b][i];
     }
     return;
   }
@@ -298,7 +388,47 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
     const int piece = i * 256 + tid;
     *reinterpret_cast<u32x4*>(tile + piece / (S::kCols / 8) * S::kStride + piece % (S::kCols / 8) * 16) = stage[i];
   }
+  if constexpr (MERGE) {
+#pragma unroll
+    for (int i = 0; i < kZb; ++i) {
+      const int piece = i * 256 + tid, r = piece >> 3;
+      if (r >= RT * 16) break;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float v = merge_scale * (q & 1 ? bf16hi(zbv[i][q >> 1]) : bf16lo(zbv[i][q >> 1]));
+        f32x4 one = {v, 0.f, 0.f, 0.f};
+        const int off = ((piece & 7) * 8 + q) * S::kZStride + r * 2;
+        *reinterpret_cast<bf16_t*>(&lz[0][off]) = (bf16_t)take_terms(one).x;
+        *reinterpret_cast<bf16_t*>(&lz[1][off]) = f32_to_bf16(one[0]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int piece = i * 256 + tid, off = piece / (RT * 4) * S::kZStride + piece % (RT * 4) * 8;
+      *reinterpret_cast<u32x2*>(&lz[0][off]) = take_terms(zv[i]);
+      *reinterpret_cast<u32x2*>(&lz[1][off]) = to_bf16(zv[i]);
+    }
+  }
   __syncthreads();
+  u32x4 zf[4][S::kSteps][S::kTerms];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < S::kSteps; ++k) {
+      const int off = (i * 16 + lr) * S::kZStride + k * 64 + lq * 8;
+      u32x2 v[2][2];
+#pragma unroll
+      for (int term = 0; term < 2; ++term)
+#pragma unroll
+        for (int h = 0; h < (RT == 1 ? 1 : 2); ++h) v[term][h] = *reinterpret_cast<const u32x2*>(&lz[term][off + h * 32]);
+      if constexpr (RT == 1) {
+        zf[i][k][0] = u32x4{v[0][0].x, v[0][0].y, v[1][0].x, v[1][0].y};
+      } else {
+#pragma unroll
+        for (int term = 0; term < 2; ++term) zf[i][k][term < S::kTerms ? term : 0] = u32x4{v[term][0].x, v[term][0].y, v[term][1].x, v[term][1].y};
+      }
+    }
   // lane (lr, lq) asks for factor row 4 lq + lr / 4 (and 16 more) at columns 8 (lr % 4) + 4 h: lane lr receives column 8 (lr / 4) + 4 h + lr % 4, so the two
   // products h = 0, 1 leave columns 8 lq .. 8 lq + 7 of position lr in one lane
   const unsigned char* at = tile + (lq * 4 + (lr >> 2)) * S::kStride + wave * 64 + (lr & 3) * 16;
@@ -328,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
       const u32x4 v = bv[b][i];
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(v[q]) + acc[q >> 1][(q & 1) * 2], bf16hi(v[q]) + acc[q >> 1][(q & 1) * 2 + 1]);
-      if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + row[i] * ldo + c) = o;
+      if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = o;
     }
   }
 }
@@ -367,11 +497,14 @@ __global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s
   u32x4 tv[kTp];
   f32x4 zv[kZp];
   auto load = [&](int ps) {
+    int pos[kTp], row[kTp];
 #pragma unroll
-    for (int i = 0; i < kTp; ++i) {
-      const int piece = i * 256 + tid, p = ps + (piece >> 5), c = c0 + (piece & 31) * 8;
-      tv[i] = p < p1 && c < s.d ? *reinterpret_cast<const u32x4*>(s.t + row_of(row_ids, p, n) * s.ldt + c) : u32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < kTp; ++i) pos[i] = min(ps + i * 8 + (tid >> 5), p1 - 1);
+    rows_of(row_ids, pos, n, row);
+    const int c = c0 + (tid & 31) * 8;
+#pragma unroll
+    for (int i = 0; i < kTp; ++i)
+      tv[i] = ps + i * 8 + (tid >> 5) < p1 && c < s.d ? *reinterpret_cast<const u32x4*>(s.t + (int64_t)row[i] * s.ldt + c) : u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < kZp; ++i) {
       const int piece = i * 256 + tid, p = ps + piece / (RT * 4), r = piece % (RT * 4) * 4;
@@ -481,17 +614,33 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // host side
 static inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 static inline int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
-static inline int shrink_rows(int rank) { return rank_tiles(rank) >= 4 ? 64 : 32; }
-
-// Parts of the long axis in shrink.  Row tiles alone fill the card from about 512 workgroups up (two on each CU); below that the axis is cut, in parts of at least
-// 512 columns (one step for each wave and two to overlap), because a single workgroup reads a factor no faster than one CU's path to L2 allows.
-static inline int shrink_parts(int64_t n, int64_t n_adapters, int d, int rank) {
-  const int64_t tiles = max_tiles(n, n_adapters, shrink_rows(rank));
-  int64_t parts = 512 / (tiles > 0 ? tiles : 1);
-  if (parts > d / 512) parts = d / 512;
-  return parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
+struct ShrinkPlan {
+  int rows, chunk, parts, chunks_per_part;
+  int64_t tiles;
+};
+// Narrow: 32 positions a tile, two workgroups fit a CU.  Wide: one workgroup fits a CU, so what a launch takes goes with the rounds of 256 tiles times a tile's
+// bytes (its rows and the factor); 257 tiles of 128 rows take 1.5 times as long as 256.  The tile's rows are chosen to make that least.
+// Where the tiles are too few to fill the card, the long axis is cut into parts of at least two chunks.
+static inline ShrinkPlan shrink_plan(int64_t n, int64_t n_adapters, int d, int rank) {
+  ShrinkPlan p;
+  const bool narrow = rank <= 16;
+  p.rows = kNarrowRows;
+  if (!narrow) {
+    int64_t least = INT64_MAX;
+    for (int rows = 16; rows <= 192; rows += 16) {
+      const int64_t cost = cdiv(max_tiles(n, n_adapters, rows), 256) * (rows + rank_tiles(rank) * 16);
+      if (cost <= least) least = cost, p.rows = rows;
+    }
+  }
+  p.tiles = max_tiles(n, n_adapters, p.rows);
+  p.chunk = narrow ? kNarrowChunk : p.rows <= wide_rows(rank_tiles(rank), 128) ? 128 : 64;
+  const int64_t chunks = cdiv(d, p.chunk);
+  int64_t parts = (narrow ? 512 : 256) / (p.tiles > 0 ? p.tiles : 1);
+  if (parts > chunks / 2) parts = chunks / 2;
+  p.parts = parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
+  p.chunks_per_part = (int)cdiv(chunks, p.parts);
+  return p;
 }
-static inline int steps_of(int d, int parts) { return (int)cdiv(cdiv(d, 64), parts); }
 
 // Positions per outer tile: enough tiles to fill the card (1024 workgroups over the column tiles), but long enough that a tile's f32 partial (4 r bytes a column, written
 // and read once) stays small beside the rows it stands for (2 bytes a column each): at least 32 r positions where there are that many.
@@ -503,12 +652,15 @@ static inline int outer_rows(int64_t n, int d_in, int d_out, int rank) {
 }
 
 template <int RT>
-static void launch_shrink(const void* t, int64_t ldt, const void* w, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n, int n_adapters, int d, int rank,
-                          int parts, float* z, hipStream_t stream) {
-  constexpr int MT = RT >= 4 ? 4 : 2, U = RT == 1 ? 4 : RT == 2 ? 2 : 1;
-  const dim3 grid((unsigned)max_tiles(n, n_adapters, 16 * MT), parts);
-  hipLaunchKernelGGL((shrink_kernel<RT, MT, U>), grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets, row_ids, (int)n, n_adapters, d, rank,
-                     padded_rank(rank), steps_of(d, parts), z);
+static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, const void* w, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n,
+                          int n_adapters, int d, int rank, float* z, hipStream_t stream) {
+  const dim3 grid((unsigned)(plan.tiles * plan.parts));
+  if constexpr (RT == 1)
+    hipLaunchKernelGGL(shrink_narrow_kernel, grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets, row_ids, (int)n, n_adapters, d, rank, plan.parts,
+                       plan.chunks_per_part, z);
+  else
+    hipLaunchKernelGGL((plan.chunk == 128 ? shrink_wide_kernel<RT, 128> : shrink_wide_kernel<RT, 64>), grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales,
+                       offsets, row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.parts, plan.chunks_per_part, z);
 }
 template <int RT, bool MERGE>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
@@ -557,7 +709,7 @@ extern "C" int64_t pm_lora_z_columns(int32_t rank) { return rank >= 1 && rank <=
 
 extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank) {
   if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
-  const int parts = shrink_parts(n_rows, n_adapters, (int)d_in, rank);
+  const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank).parts;
   return parts > 1 ? (int64_t)parts * n_rows * padded_rank(rank) * 4 : 0;
 }
 
@@ -572,13 +724,14 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   if (base) PM_TRY(check_rows("pm_lora_fwd", "base", base, ldbase, d_out));
   PM_REQUIRE(base != out || ldbase == ldout, PM_ERR_INVALID_ARG, "pm_lora_fwd: base and out are the same rows with different strides");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
-  const int parts = shrink_parts(n_rows, n_adapters, (int)d_in, rank);
+  const ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank);
+  const int parts = plan.parts;
   const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, rank);
   PM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PM_ERR_WORKSPACE, "pm_lora_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)need);
   hipStream_t st = as_stream(stream);
   float* zs = parts > 1 ? (float*)workspace : z;
-  PM_BY_RANK(rank, (launch_shrink<RT>(x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, parts, zs, st)));
+  PM_BY_RANK(rank, (launch_shrink<RT>(plan, x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, zs, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
   PM_BY_RANK(rank, (launch_expand<RT, false>(zs, parts, parts > 1 ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
@@ -587,15 +740,16 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
 
 namespace {
 struct BwdPlan {
-  int parts, rows;
+  ShrinkPlan shrink;
+  int rows;
   int64_t tiles, dz_bytes, part0_bytes, part1_bytes;
 };
 BwdPlan bwd_plan(int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int rank) {
   BwdPlan p;
-  p.parts = shrink_parts(n, n_adapters, (int)d_out, rank);
+  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
   p.rows = outer_rows(n, (int)d_in, (int)d_out, rank);
   p.tiles = max_tiles(n, n_adapters, p.rows);
-  p.dz_bytes = (int64_t)p.parts * n * padded_rank(rank) * 4;
+  p.dz_bytes = (int64_t)p.shrink.parts * n * padded_rank(rank) * 4;
   p.part0_bytes = p.tiles * rank * d_out * 4;
   p.part1_bytes = p.tiles * rank * d_in * 4;
   return p;
@@ -617,7 +771,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
              "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
   PM_REQUIRE(offsets, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
   hipStream_t st = as_stream(stream);
-  BwdPlan p{1, 64, 0, 0, 0, 0};
+  BwdPlan p{{}, 64, 0, 0, 0, 0};
   unsigned char* ws = (unsigned char*)workspace;
   if (n_rows > 0) {
     PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
@@ -634,26 +788,28 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     PM_REQUIRE(ws && workspace_bytes >= need && ((uintptr_t)ws & 15) == 0, PM_ERR_WORKSPACE, "pm_lora_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                (long long)need);
     float* dz = (float*)ws;
-    PM_BY_RANK(rank, (launch_shrink<RT>(grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, p.parts, dz, st)));
+    PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
     PM_CHECK_LAUNCH("pm_lora_bwd");
-    if (grad_x) {
-      PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
+  }
+  if (grad_a) {
+    float *part0 = (float*)(ws + p.dz_bytes), *part1 = (float*)(ws + p.dz_bytes + p.part0_bytes);
+    if (p.tiles > 0) {
+      const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
+      const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
+      PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(p.tiles * (t0 + t1))), dim3(256), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids, (int)n_rows, n_adapters, rank,
+                                          padded_rank(rank), p.rows));
       PM_CHECK_LAUNCH("pm_lora_bwd");
     }
-  }
-  if (!grad_a) return PM_OK;
-  float *part0 = (float*)(ws + p.dz_bytes), *part1 = (float*)(ws + p.dz_bytes + p.part0_bytes);
-  if (p.tiles > 0) {
-    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
-    const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
-    PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(p.tiles * (t0 + t1))), dim3(256), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids, (int)n_rows, n_adapters, rank,
-                                        padded_rank(rank), p.rows));
+    const int64_t e0 = rank * d_out, e1 = rank * d_in;
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, n_adapters, p.rows,
+                       (int)p.tiles, accumulate);
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
-  const int64_t e0 = rank * d_out, e1 = rank * d_in;
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, n_adapters, p.rows,
-                     (int)p.tiles, accumulate);
-  PM_CHECK_LAUNCH("pm_lora_bwd");
+  if (n_rows > 0 && grad_x) {
+    float* dz = (float*)ws;
+    PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
+    PM_CHECK_LAUNCH("pm_lora_bwd");
+  }
   return PM_OK;
 }
 
