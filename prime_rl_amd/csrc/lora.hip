@@ -16,6 +16,7 @@
 // in expand, whose result is rounded to bf16 (8 bits) anyway, three terms (24 bits: all of it) in outer, whose results are f32 gradients.  Everything else in
 // the products is bf16 by type and every sum is f32, in a fixed order (no atomics: the same inputs give the same bits).
 #include "common.hip.h"
+#include <type_traits>
 
 namespace pm {
 namespace lora {
@@ -29,7 +30,7 @@ typedef __attribute__((address_space(1))) void* glb_void_ptr;
 
 constexpr int kMaxRank = 128;
 constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
-constexpr int kOuterCols = 256;  // columns per outer tile
+constexpr int kOuterCols = 512;  // columns of an outer workgroup
 
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -464,149 +465,202 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// outer: part[tile][r][c] = sum over the tile's positions of z[p][r] * t[row(p)][c], one f32 partial per tile of `rows` positions of one adapter.
-// Both products of the backward (dB from z and dy, dA from dz and x) are one launch: the column tiles run over the 256-column tiles of dy, then of x.
-// The positions are the contraction, so both operands are read transposed: stages of SP positions go through LDS (t as it is, z split into three bf16
-// planes), the next stage's loads are in flight while the matrix cores work on this one.  A wave takes 64 columns and all ranks.
+// outer: dW[adapter][r][c] = sum over the adapter's positions of z[p][r] * t[row(p)][c].
+// Both products of the backward (dB from z and dy, dA from dz and x) are one launch.  A workgroup takes 512 columns and one of equal ranges of positions, whatever
+// adapters these belong to: the ranges are cut so that all workgroups run in one round, one on each CU, with the same work each.  At the end of an adapter's positions
+// (or of the range) the sum goes to a partial: range s and adapter g meet at most once, and s + g is a number of their own for every pair that meets.
+// The positions are the contraction, so both operands are read transposed (ds_read_b64_tr_b16).  Stages of 32 positions go through LDS: t by DMA, a ring of three deep
+// (16-byte slot pairs permuted by the row's number, so that the 8 rows of half a transposed read lie in different banks), z through registers, where it is split into
+// three bf16 planes.  A wave takes 64 columns and all ranks.
 struct OuterSide {
   const float* z;      // [parts][n][rp]
   int parts;
   const bf16_t* t;     // [*, ldt]
   int64_t ldt;
   int d;
-  float* part;         // [tiles][rank][d]
+  float* part;         // [ranges + adapters][rank][d]
 };
+constexpr int kOuterStage = 32, kOuterRing = 3, kOuterIds = 1024;  // kOuterIds: row ids held in LDS at a time
+
+// the transposed fragments of four 16-column blocks (addresses a[0 .. 3]) of a [32][512] tile: rows 4 lq + .., then 16 more.  One block with its own wait: the compiler would
+// wait for every DMA in flight before a transposed read through its builtin.
+__device__ __forceinline__ void tr_read_tile(const uint32_t (&a)[4], u32x2 (&v)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:16384\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:16384\n\t"
+      "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:16384\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:16384\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3])
+      : "memory");
+}
 
 template <int RT>
-__global__ __launch_bounds__(256, 2) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
-                                                       int n_adapters, int rank, int rp, int rows) {
-  constexpr int SP = RT <= 2 ? 64 : 32;           // positions per stage
-  constexpr int kTs = kOuterCols * 2 + 32;        // row strides in LDS: 32 bytes of shift per row keep transposed reads off each other's banks
-  constexpr int kZs = RT == 1 ? 32 : RT * 32 + 32;
-  constexpr int kTp = SP * kOuterCols / 8 / 256;  // 16-byte pieces of t per thread and stage
-  constexpr int kZp = (SP * RT * 4 + 255) / 256;  // 4-rank pieces of z per thread and stage
-  __shared__ __attribute__((aligned(16))) unsigned char lt[SP * kTs];
-  __shared__ __attribute__((aligned(16))) unsigned char lz[3][SP * kZs];
+__global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                    int n_adapters, int rank, int rp, int range) {
+  constexpr int SP = kOuterStage, kRowBytes = kOuterCols * 2, kBuf = SP * kRowBytes;
+  constexpr int kZs = RT == 1 ? 32 : RT * 32 + 32;  // 32 bytes of shift per row keep transposed reads off each other's banks
+  constexpr int kZp = (SP * RT * 4 + 511) / 512;    // 4-rank pieces of z per thread and stage
+  constexpr int kDma = SP / 8;                      // instructions of a wave and stage: one row each
+  __shared__ __attribute__((aligned(1024))) unsigned char lt[kOuterRing * kBuf];
+  __shared__ __attribute__((aligned(16))) unsigned char lz[2][3][SP * kZs];
+  __shared__ int li[kOuterIds];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-  const int row_tile = blockIdx.x / tiles01, col_tile = blockIdx.x % tiles01;  // columns fastest, as in expand
+  const int split = blockIdx.x / tiles01, col_tile = blockIdx.x % tiles01;
   const bool second = col_tile >= tiles0;
   const OuterSide s = second ? s1 : s0;
   const int c0 = (second ? col_tile - tiles0 : col_tile) * kOuterCols;
-  int adapter, p0, p1;
-  if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
-  u32x4 tv[kTp];
-  f32x4 zv[kZp];
-  auto load = [&](int ps) {
-    int pos[kTp], row[kTp];
-#pragma unroll
-    for (int i = 0; i < kTp; ++i) pos[i] = min(ps + i * 8 + (tid >> 5), p1 - 1);
-    rows_of(row_ids, pos, n, row);
-    const int c = c0 + (tid & 31) * 8;
-#pragma unroll
-    for (int i = 0; i < kTp; ++i)
-      tv[i] = ps + i * 8 + (tid >> 5) < p1 && c < s.d ? *reinterpret_cast<const u32x4*>(s.t + (int64_t)row[i] * s.ldt + c) : u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < kZp; ++i) {
-      const int piece = i * 256 + tid, p = ps + piece / (RT * 4), r = piece % (RT * 4) * 4;
-      zv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (p < p1 && r < rp && piece < SP * RT * 4)
-        for (int part = 0; part < s.parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(s.z + ((int64_t)part * n + p) * rp + r);
+  const int begin = split * range, end = min(begin + range, n);
+  // the first adapter whose positions reach past `begin`
+  int g = n_adapters;
+  for (int e0 = 0; e0 < n_adapters; e0 += 64) {
+    const unsigned long long hit = __ballot(e0 + lane < n_adapters && offsets[min(e0 + lane, n_adapters - 1) + 1] > begin);
+    if (hit) {
+      g = e0 + __ffsll((long long)hit) - 1;
+      break;
     }
-  };
-  auto store = [&]() {
+  }
+  uint32_t ta[4];
 #pragma unroll
-    for (int i = 0; i < kTp; ++i) {
-      const int piece = i * 256 + tid;
-      *reinterpret_cast<u32x4*>(lt + (piece >> 5) * kTs + (piece & 31) * 16) = tv[i];
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int row = lq * 4 + (lr >> 2);
+    ta[i] = (uint32_t)(uintptr_t)(lds_void_ptr)lt + row * kRowBytes + (((wave * 4 + i) ^ (row & 7)) << 5) + (lr & 3) * 8;
+  }
+  int lo = g < n_adapters ? min(max(offsets[g], begin), end) : end;
+  for (; g < n_adapters && lo < end; ++g) {
+    const int hi = min(max(offsets[g + 1], lo), end);
+    if (hi == lo) continue;
+    f32x4 acc[4][RT];
 #pragma unroll
-    for (int i = 0; i < kZp; ++i) {
-      const int piece = i * 256 + tid;
-      if (piece >= SP * RT * 4) break;
-      const int off = piece / (RT * 4) * kZs + piece % (RT * 4) * 8;
-      f32x4 v = zv[i];
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int term = 0; term < 3; ++term) *reinterpret_cast<u32x2*>(&lz[term][off]) = take_terms(v);
-    }
-  };
-  f32x4 acc[4][RT];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load(p0);
-  for (int ps = p0; ps < p1; ps += SP) {
-    store();
-    __syncthreads();
-    if (ps + SP < p1) load(ps + SP);
-#pragma unroll
-    for (int k = 0; k < SP / 32; ++k) {
-      const int row = k * 32 + lq * 4 + (lr >> 2);
-      u32x4 tf[4], zf[RT][3];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // columns 64 wave + 32 (i / 2) + 8 (lr / 4) + 4 (i % 2) + lr % 4
-        const unsigned char* q = lt + row * kTs + wave * 128 + (i >> 1) * 64 + (lr & 3) * 16 + (i & 1) * 8;
-        const u32x2 lo = tr_read(q), hi = tr_read(q + 16 * kTs);
-        tf[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int first = lo, last; first < hi; first = last) {
+      last = row_ids ? min(first + kOuterIds, hi) : hi;
+      const int stages = (last - first + SP - 1) / SP, full = (last - first) / SP;
+      lds_barrier();  // the buffers are free
+      if (row_ids) {
+        for (int i = tid; i < last - first; i += 512) li[i] = min(max(row_ids[first + i], 0), n - 1);
+        lds_barrier();
       }
+      // wave w brings rows w, w + 8, ..; slot pairs of row r are permuted by r % 8 = w; columns past the end repeat column 0 and are not stored
+      const int src = (lane ^ (wave << 1)) * 8, col = c0 + src < s.d ? c0 + src : 0;
+      auto fetch = [&](int st, bool whole) {
+        unsigned char* to = lt + st % kOuterRing * kBuf + wave * kRowBytes;
 #pragma unroll
-      for (int j = 0; j < RT; ++j)
-#pragma unroll
-        for (int term = 0; term < 3; ++term) {
-          const unsigned char* q = lz[term] + row * kZs + j * 32 + (lr & 3) * 8;
-          const u32x2 lo = tr_read(q), hi = tr_read(q + 16 * kZs);
-          zf[j][term] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        for (int i = 0; i < kDma; ++i) {
+          const int p = st * SP + i * 8 + wave;
+          if (whole || first + p < last) {
+            const int row = row_ids ? li[p] : first + p;
+            dma16(s.t + (int64_t)row * s.ldt + col, to + i * 8 * kRowBytes);
+          } else {  // positions behind the last are zeros on both sides
+            *reinterpret_cast<u32x4*>(to + i * 8 * kRowBytes + lane * 16) = u32x4{0, 0, 0, 0};
+          }
         }
+      };
+      auto load_z = [&](int st, f32x4 (&zv)[kZp], int parts) {
 #pragma unroll
-      for (int term = 2; term >= 0; --term)
+        for (int i = 0; i < kZp; ++i) {
+          const int piece = (i * 512 + tid) % (SP * RT * 4), p = min(first + st * SP + piece / (RT * 4), last - 1), r = min(piece % (RT * 4) * 4, rp - 4);
+          const float* at = s.z + (int64_t)p * rp + r;
+          zv[i] = *reinterpret_cast<const f32x4*>(at);
+          for (int part = 1; part < parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(at + (int64_t)part * n * rp);
+        }
+      };
+      auto split_z = [&](int st, f32x4 (&zv)[kZp]) {
+#pragma unroll
+        for (int i = 0; i < kZp; ++i) {
+          const int piece = i * 512 + tid, q = piece / (RT * 4), r = piece % (RT * 4) * 4;
+          f32x4 v = first + st * SP + q < last && r < rp ? zv[i] : f32x4{0.f, 0.f, 0.f, 0.f};
+          if (piece >= SP * RT * 4) break;
+#pragma unroll
+          for (int term = 0; term < 3; ++term) *reinterpret_cast<u32x2*>(&lz[st & 1][term][q * kZs + r * 2]) = take_terms(v);
+        }
+      };
+      auto multiply = [&](int st) {
+        uint32_t a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = ta[i] + st % kOuterRing * kBuf;
+        u32x2 tv[8];
+        tr_read_tile(a, tv);
+        const int zrow = (lq * 4 + (lr >> 2)) * kZs + (lr & 3) * 8;
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][j] = mfma(tf[i], zf[j][term], acc[i][j]);
-    }
-    __syncthreads();
-  }
-  float* part = s.part + (int64_t)row_tile * rank * s.d;
+          for (int term = 2; term >= 0; --term) {
+            const unsigned char* q = &lz[st & 1][term][zrow + j * 32];
+            const u32x2 l = tr_read(q), h = tr_read(q + 16 * kZs);
+            const u32x4 zf = {l.x, l.y, h.x, h.y};
 #pragma unroll
-  for (int j = 0; j < RT; ++j) {
-    const int r = j * 16 + lr;
-    if (r >= rank) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = c0 + wave * 64 + (i >> 1) * 32 + lq * 8 + (i & 1) * 4;
-      if (c < s.d) *reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c) = acc[i][j];
+            for (int i = 0; i < 4; ++i) acc[i][j] = mfma(u32x4{tv[2 * i].x, tv[2 * i].y, tv[2 * i + 1].x, tv[2 * i + 1].y}, zf, acc[i][j]);
+          }
+      };
+      // stage st: t comes two stages ahead, z three (it is split one stage ahead)
+      f32x4 za[kZp], zb[kZp];
+      fetch(0, full > 0);
+      load_z(0, za, s.parts);
+      if (stages > 1) fetch(1, full > 1);
+      split_z(0, za);
+      load_z(min(1, stages - 1), zb, s.parts);
+      load_z(min(2, stages - 1), za, s.parts);
+      int st = 0;
+      auto stage = [&](auto steady, f32x4 (&next)[kZp]) {  // `next` holds z of stage st + 1, and gets that of st + 3
+        if constexpr (decltype(steady)::value) {
+          wait_dma(kDma + kZp);  // younger than t of this stage: t of the next, and z of the one after it
+          lds_barrier();
+          split_z(st + 1, next);
+          fetch(st + 2, true);
+          load_z(st + 3, next, 1);
+        } else {
+          wait_dma(0);
+          lds_barrier();
+          if (st + 1 < stages) split_z(st + 1, next);
+          if (st + 2 < stages) fetch(st + 2, st + 2 < full);
+          if (st + 3 < stages) load_z(st + 3, next, s.parts);
+        }
+        multiply(st);
+        ++st;
+      };
+      if (s.parts == 1)
+        while (st + 4 < full) {
+          stage(std::true_type{}, zb);
+          stage(std::true_type{}, za);
+        }
+      while (st < stages) {
+        stage(std::false_type{}, zb);
+        if (st < stages) stage(std::false_type{}, za);
+      }
     }
+    float* part = s.part + (int64_t)(split + g) * rank * s.d;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+      const int r = j * 16 + lr;
+      if (r >= rank) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + wave * 64 + i * 16 + lq * 4;
+        if (c < s.d) *reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c) = acc[i][j];
+      }
+    }
+    lo = hi;
   }
 }
 
-// grad[adapter][r][c] (+)= the adapter's partials, added in the order of its tiles; zero for an adapter without rows.
+// grad[adapter][r][c] (+)= the adapter's partials, added in the order of its positions; zero for an adapter without rows.
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part0, float* __restrict__ grad0, int64_t elems0, const float* __restrict__ part1,
-                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int n_adapters, int rows, int tiles_max,
-                                                   int accumulate) {
-  const int lane = threadIdx.x & 63, adapter = blockIdx.y;
-  int first = 0, count = 0;
-  for (int e0 = 0; e0 <= adapter; e0 += 64) {
-    const int e = e0 + lane;
-    int tiles = 0;
-    if (e <= adapter) {
-      const int lo = min(max(offsets[e], 0), n), hi = min(max(offsets[e + 1], lo), n);
-      tiles = (hi - lo + rows - 1) / rows;
-    }
-    int before = e < adapter ? tiles : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
-    first += before;
-    if (adapter < e0 + 64) count = __shfl(tiles, adapter - e0, 64);
-  }
-  count = max(0, min(count, tiles_max - first));
+                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int range, int accumulate) {
+  const int g = blockIdx.y;
+  const int lo = min(max(offsets[g], 0), n), hi = min(max(offsets[g + 1], lo), n);
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= elems0 + elems1) return;
   const bool second = at >= elems0;
   const int64_t e = second ? at - elems0 : at, elems = second ? elems1 : elems0;
-  const float* part = (second ? part1 : part0) + (int64_t)first * elems + e;
-  float* grad = (second ? grad1 : grad0) + (int64_t)adapter * elems + e;
+  const float* part = (second ? part1 : part0) + e;
+  float* grad = (second ? grad1 : grad0) + (int64_t)g * elems + e;
   f32x4 v = accumulate ? *reinterpret_cast<const f32x4*>(grad) : f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < count; ++i) v += *reinterpret_cast<const f32x4*>(part + (int64_t)i * elems);
+  if (lo < hi)
+    for (int split = lo / range; split <= (hi - 1) / range; ++split) v += *reinterpret_cast<const f32x4*>(part + (int64_t)(split + g) * elems);
   *reinterpret_cast<f32x4*>(grad) = v;
 }
 
@@ -642,13 +696,17 @@ static inline ShrinkPlan shrink_plan(int64_t n, int64_t n_adapters, int d, int r
   return p;
 }
 
-// Positions per outer tile: enough tiles to fill the card (1024 workgroups over the column tiles), but long enough that a tile's f32 partial (4 r bytes a column, written
-// and read once) stays small beside the rows it stands for (2 bytes a column each): at least 32 r positions where there are that many.
-static inline int outer_rows(int64_t n, int d_in, int d_out, int rank) {
-  const int64_t cols = cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols);
-  int64_t rows = 64;
-  while (rows * 2 <= n * cols / 1024 && rows < 32 * rank) rows *= 2;
-  return (int)rows;
+// Ranges of positions in outer.  One workgroup fits a CU: what a launch takes goes with its rounds of 256, times what a workgroup moves, in rows of 512 columns
+// (1 KiB): its positions, and for each adapter among them a partial (written, and read by the join: 4 rank) and the wait for the first stage (as long as about 96 rows).
+static inline int outer_range(int64_t n, int64_t n_adapters, int64_t col_tiles, int rank) {
+  double least = 0.0;
+  int64_t best = n > 0 ? n : 1;
+  for (int64_t splits = 1; splits <= n && splits <= 1024; ++splits) {
+    const int64_t range = cdiv(n, splits), used = cdiv(n, range);
+    const double cost = (double)cdiv(used * col_tiles, 256) * ((double)(range < 32 ? 32 : range) + (4.0 * rank + 96.0) * (1.0 + (double)n_adapters / (double)used));
+    if (splits == 1 || cost < least) least = cost, best = range;
+  }
+  return (int)best;
 }
 
 template <int RT>
@@ -741,17 +799,17 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
 namespace {
 struct BwdPlan {
   ShrinkPlan shrink;
-  int rows;
-  int64_t tiles, dz_bytes, part0_bytes, part1_bytes;
+  int range;
+  int64_t slots, dz_bytes, part0_bytes, part1_bytes;
 };
 BwdPlan bwd_plan(int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int rank) {
   BwdPlan p;
   p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
-  p.rows = outer_rows(n, (int)d_in, (int)d_out, rank);
-  p.tiles = max_tiles(n, n_adapters, p.rows);
+  p.range = outer_range(n, n_adapters, cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols), rank);
+  p.slots = cdiv(n, p.range) + n_adapters;
   p.dz_bytes = (int64_t)p.shrink.parts * n * padded_rank(rank) * 4;
-  p.part0_bytes = p.tiles * rank * d_out * 4;
-  p.part1_bytes = p.tiles * rank * d_in * 4;
+  p.part0_bytes = p.slots * rank * d_out * 4;
+  p.part1_bytes = p.slots * rank * d_in * 4;
   return p;
 }
 }  // namespace
@@ -771,7 +829,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
              "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
   PM_REQUIRE(offsets, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
   hipStream_t st = as_stream(stream);
-  BwdPlan p{{}, 64, 0, 0, 0, 0};
+  BwdPlan p{{}, 1, 0, 0, 0, 0};
   unsigned char* ws = (unsigned char*)workspace;
   if (n_rows > 0) {
     PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
@@ -793,16 +851,16 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
   }
   if (grad_a) {
     float *part0 = (float*)(ws + p.dz_bytes), *part1 = (float*)(ws + p.dz_bytes + p.part0_bytes);
-    if (p.tiles > 0) {
+    if (n_rows > 0) {
       const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
       const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
-      PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(p.tiles * (t0 + t1))), dim3(256), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids, (int)n_rows, n_adapters, rank,
-                                          padded_rank(rank), p.rows));
+      PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(cdiv(n_rows, p.range) * (t0 + t1))), dim3(512), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids,
+                                          (int)n_rows, n_adapters, rank, padded_rank(rank), p.range));
       PM_CHECK_LAUNCH("pm_lora_bwd");
     }
     const int64_t e0 = rank * d_out, e1 = rank * d_in;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, n_adapters, p.rows,
-                       (int)p.tiles, accumulate);
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, p.range,
+                       accumulate);
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
   if (n_rows > 0 && grad_x) {
