@@ -297,19 +297,26 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restri
 
 // ---------------------------------------------------------------------------------------------------------------------
 // expand: out[row][c] = bf16(base[row][c] + sum_r z[p][r] * w[adapter][r][c]).
-// A workgroup takes 64 positions x COLS columns.  The factor tile [r][COLS] goes to LDS once; the matrix cores' A operand is its transpose (columns as
-// rows), read with ds_read_b64_tr_b16 so that a lane ends up with 8 consecutive columns of one position: base and out move in 16-byte accesses, whole
-// 128-byte lines per four waves.  The base is asked for before anything waits.  z is split into two bf16 terms: at rank <= 16 both fit the 32-deep
-// contraction of one instruction (its two halves read the same 16 factor rows).
+// A workgroup takes 64 positions x COLS columns.  The factor tile [r][COLS] and z's two bf16 terms go through LDS into fragments; the factor is read transposed
+// (ds_read_b64_tr_b16), as the matrix cores' A operand, so that a lane ends up with 8 consecutive columns of one position.  At rank <= 16 both terms of z fit the
+// 32-deep contraction of one instruction (its two halves read the same 16 factor rows).
+// base is asked for before anything waits.  It and out move row by row (512 bytes of a row and more in one instruction), and the products, 32 positions at a time, come through
+// LDS into that order, over the factor tile's place: accesses in the fragments' own order (16 rows x 64 bytes) reach 4.5 TB/s where these reach 5.5 (copies of 16 384 x 6144).
+// Column tiles run fastest, so that workgroups that run together cover whole rows (5.5 TB/s against 4.2 with row tiles fastest).
 // Without base the sum starts from zero; rows of no adapter get the base as it is.  MERGE: positions are the rows of a weight, z[p][r] = scale * zb[r][p] (bf16).
 template <int RT>
 struct ExpandShape {
-  static constexpr int kCols = RT == 1 ? 512 : RT == 2 ? 512 : RT == 4 ? 256 : 128;
-  static constexpr int kZStride = RT * 32 + (RT == 4 ? 16 : 32);  // bytes of a row of z's bf16 terms (rank 64: three workgroups still fit a CU's LDS)
+  static constexpr int kCols = RT <= 4 ? 256 : 128;
+  static constexpr int kZStride = RT * 32 + (RT == 4 ? 16 : 32);  // bytes of a row of z's terms (rank 64: three workgroups still fit a CU's LDS)
   static constexpr int kStride = kCols * 2 + 32;  // bytes; a row shift of 32 bytes spreads the 8 rows that a transposed read takes at once over all banks
+  static constexpr int kSumStride = kCols * 4 + 32;
   static constexpr int kSteps = RT == 1 ? 1 : RT / 2;  // 32-deep contraction steps over the rank
   static constexpr int kTerms = RT == 1 ? 1 : 2;       // bf16 terms that are operands of their own
   static constexpr int kBlocks = kCols / 128;          // 32-column blocks of a wave
+  static constexpr int kLanes = kCols / 8;             // lanes that move one row
+  static constexpr int kMoves = kCols / 64;            // accesses of a lane for 32 positions
+  static constexpr int kZAt = RT * 16 * kStride, kIn = kZAt + 2 * kExpandRows * kZStride, kSums = 32 * kSumStride;
+  static constexpr int kLds = kIn > kSums ? kIn : kSums;
 };
 
 template <int RT, bool MERGE>
@@ -317,10 +324,8 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
                                                         const bf16_t* __restrict__ w, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
                                                         int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place) {
   using S = ExpandShape<RT>;
-  __shared__ __attribute__((aligned(16))) unsigned char tile[RT * 16 * S::kStride];
-  __shared__ __attribute__((aligned(16))) unsigned char lz[2][kExpandRows * S::kZStride];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-  // column tiles run fastest: workgroups that run together cover whole rows (a 64 x 512 tile copy: 5.5 TB/s against 4.2 with row tiles fastest)
   const int col_tiles = (d + S::kCols - 1) / S::kCols, row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x % col_tiles;
   int adapter = 0, p0 = row_tile * kExpandRows, p1 = min(p0 + kExpandRows, n);
   if constexpr (!MERGE) {
@@ -329,23 +334,15 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
   }
   const int c0 = col_tile * S::kCols;
   // the factor tile, rows past the rank and columns past the end as zeros
-  constexpr int kPieces = RT * 16 * S::kCols / 8 / 256;
+  constexpr int kPieces = RT * 16 * S::kLanes / 256;
   u32x4 stage[kPieces];
   if (adapter >= 0) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * 256 + tid, r = piece / (S::kCols / 8), c = c0 + piece % (S::kCols / 8) * 8;
+      const int piece = i * 256 + tid, r = piece / S::kLanes, c = c0 + piece % S::kLanes * 8;
       stage[i] = r < rank && c < d ? *reinterpret_cast<const u32x4*>(w + ((int64_t)adapter * rank + r) * d + c) : u32x4{0, 0, 0, 0};
     }
   }
-  const int tiles16 = (p1 - p0 + 15) >> 4;
-  int pos[4], row[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int p = p0 + i * 16 + lr;
-    pos[i] = p < p1 ? p : p0;
-  }
-  rows_of(row_ids, pos, n, row);
   // z, split into its two bf16 terms on the way to LDS
   constexpr int kZb = (RT * 2 + 3) / 4;
   f32x4 zv[MERGE ? 1 : RT];  // thread -> 4 ranks of one position, RT times
@@ -367,28 +364,34 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
       }
     }
   }
-  u32x4 bv[S::kBlocks][4];
+  // base: move m of half h covers positions 32 h + (m * 4 + wave) * 64 / kLanes + lane / kLanes
+  const int mrow = lane / S::kLanes, mcol = lane % S::kLanes * 8, c = c0 + mcol;
+  int pos[2 * S::kMoves], row[2 * S::kMoves];
 #pragma unroll
-  for (int b = 0; b < S::kBlocks; ++b) {
-    const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bv[b][i] = base && c < d && i < tiles16 ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+  for (int i = 0; i < 2 * S::kMoves; ++i) {
+    const int p = p0 + i / S::kMoves * 32 + (i % S::kMoves * 4 + wave) * (64 / S::kLanes) + mrow;
+    pos[i] = p < p1 ? p : p0;
   }
+  rows_of(row_ids, pos, n, row);
+  u32x4 bv[2 * S::kMoves];
+#pragma unroll
+  for (int i = 0; i < 2 * S::kMoves; ++i) bv[i] = base && c < d && (i < S::kMoves || p1 - p0 > 32) ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+  auto store = [&](int i, const u32x4& v) {
+    const int p = p0 + i / S::kMoves * 32 + (i % S::kMoves * 4 + wave) * (64 / S::kLanes) + mrow;
+    if (c < d && p < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = v;
+  };
   if (adapter < 0) {  // rows of no adapter
 #pragma unroll
-    for (int b = 0; b < S::kBlocks; ++b) {
-      const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = bv[b][i];
-    }
+    for (int i = 0; i < 2 * S::kMoves; ++i) store(i, bv[i]);
     return;
   }
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const int piece = i * 256 + tid;
-    *reinterpret_cast<u32x4*>(tile + piece / (S::kCols / 8) * S::kStride + piece % (S::kCols / 8) * 16) = stage[i];
+    *reinterpret_cast<u32x4*>(lds + piece / S::kLanes * S::kStride + piece % S::kLanes * 16) = stage[i];
   }
+  unsigned char* const lz = lds + S::kZAt;
+  constexpr int kTerm = kExpandRows * S::kZStride;
   if constexpr (MERGE) {
 #pragma unroll
     for (int i = 0; i < kZb; ++i) {
@@ -399,19 +402,19 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
         const float v = merge_scale * (q & 1 ? bf16hi(zbv[i][q >> 1]) : bf16lo(zbv[i][q >> 1]));
         f32x4 one = {v, 0.f, 0.f, 0.f};
         const int off = ((piece & 7) * 8 + q) * S::kZStride + r * 2;
-        *reinterpret_cast<bf16_t*>(&lz[0][off]) = (bf16_t)take_terms(one).x;
-        *reinterpret_cast<bf16_t*>(&lz[1][off]) = f32_to_bf16(one[0]);
+        *reinterpret_cast<bf16_t*>(lz + off) = (bf16_t)take_terms(one).x;
+        *reinterpret_cast<bf16_t*>(lz + kTerm + off) = f32_to_bf16(one[0]);
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int piece = i * 256 + tid, off = piece / (RT * 4) * S::kZStride + piece % (RT * 4) * 8;
-      *reinterpret_cast<u32x2*>(&lz[0][off]) = take_terms(zv[i]);
-      *reinterpret_cast<u32x2*>(&lz[1][off]) = to_bf16(zv[i]);
+      *reinterpret_cast<u32x2*>(lz + off) = take_terms(zv[i]);
+      *reinterpret_cast<u32x2*>(lz + kTerm + off) = to_bf16(zv[i]);
     }
   }
-  __syncthreads();
+  lds_barrier();
   u32x4 zf[4][S::kSteps][S::kTerms];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -422,7 +425,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 #pragma unroll
       for (int term = 0; term < 2; ++term)
 #pragma unroll
-        for (int h = 0; h < (RT == 1 ? 1 : 2); ++h) v[term][h] = *reinterpret_cast<const u32x2*>(&lz[term][off + h * 32]);
+        for (int h = 0; h < (RT == 1 ? 1 : 2); ++h) v[term][h] = *reinterpret_cast<const u32x2*>(lz + term * kTerm + off + h * 32);
       if constexpr (RT == 1) {
         zf[i][k][0] = u32x4{v[0][0].x, v[0][0].y, v[1][0].x, v[1][0].y};
       } else {
@@ -432,34 +435,46 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
     }
   // lane (lr, lq) asks for factor row 4 lq + lr / 4 (and 16 more) at columns 8 (lr % 4) + 4 h: lane lr receives column 8 (lr / 4) + 4 h + lr % 4, so the two
   // products h = 0, 1 leave columns 8 lq .. 8 lq + 7 of position lr in one lane
-  const unsigned char* at = tile + (lq * 4 + (lr >> 2)) * S::kStride + wave * 64 + (lr & 3) * 16;
+  u32x4 wf[S::kBlocks][S::kSteps][2];
 #pragma unroll
-  for (int b = 0; b < S::kBlocks; ++b) {
-    u32x4 wf[S::kSteps][2];
+  for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
     for (int k = 0; k < S::kSteps; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const unsigned char* q = at + b * 256 + k * 32 * S::kStride + h * 8;
+        const unsigned char* q = lds + (k * 32 + lq * 4 + (lr >> 2)) * S::kStride + (wave * S::kBlocks + b) * 64 + (lr & 3) * 16 + h * 8;
         const u32x2 lo = tr_read(q), hi = RT == 1 ? lo : tr_read(q + 16 * S::kStride);
-        wf[k][h] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        wf[b][k][h] = u32x4{lo.x, lo.y, hi.x, hi.y};
       }
-    const int c = c0 + (b * 4 + wave) * 32 + lq * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= tiles16) break;
-      f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int half = 0; half < 2; ++half) {
+    if (half && p1 - p0 <= 32) break;
+    lds_barrier();  // the fragments, or the last half's sums, have been read
 #pragma unroll
-      for (int k = 0; k < S::kSteps; ++k)
+    for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
-        for (int term = S::kTerms - 1; term >= 0; --term)  // the small term first
+      for (int i = 0; i < 2; ++i) {
+        f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) acc[h] = mfma(wf[k][h], zf[i][k][term], acc[h]);
+        for (int k = 0; k < S::kSteps; ++k)
+#pragma unroll
+          for (int term = S::kTerms - 1; term >= 0; --term)  // the small term first
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[h] = mfma(wf[b][k][h], zf[half * 2 + i][k][term], acc[h]);
+        f32x4* to = reinterpret_cast<f32x4*>(lds + (i * 16 + lr) * S::kSumStride + ((wave * S::kBlocks + b) * 32 + lq * 8) * 4);
+        to[0] = acc[0];
+        to[1] = acc[1];
+      }
+    lds_barrier();
+#pragma unroll
+    for (int m = 0; m < S::kMoves; ++m) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(lds + ((m * 4 + wave) * (64 / S::kLanes) + mrow) * S::kSumStride + mcol * 4);
+      const f32x4 sum[2] = {from[0], from[1]};
+      const u32x4 v = bv[half * S::kMoves + m];
       u32x4 o;
-      const u32x4 v = bv[b][i];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(v[q]) + acc[q >> 1][(q & 1) * 2], bf16hi(v[q]) + acc[q >> 1][(q & 1) * 2 + 1]);
-      if (c < d && p0 + i * 16 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = o;
+      for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(v[q]) + sum[q >> 1][(q & 1) * 2], bf16hi(v[q]) + sum[q >> 1][(q & 1) * 2 + 1]);
+      store(half * S::kMoves + m, o);
     }
   }
 }
