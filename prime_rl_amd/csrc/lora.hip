@@ -109,7 +109,7 @@ __device__ __forceinline__ void rows_of(const int32_t* __restrict__ row_ids, con
 // ---------------------------------------------------------------------------------------------------------------------
 // shrink: z[part][p][r] = scale * sum over the part's columns of t[row(p)][k] * w[adapter][r][k].
 // Chunks of columns of a tile's rows and of the factor come into LDS by DMA (global_load_lds: no registers, and one instruction takes whole stretches of a
-// row), a ring of three deep, so that two are in flight while the matrix cores work on one.  16-byte slots of a row are permuted by its row number: the 16 rows
+// row), a ring of mostly three deep, so that two are in flight while the matrix cores work on one.  16-byte slots of a row are permuted by its row number: the 16 rows
 // of a fragment read lie in different banks.  The factor's chunk is read once for each tile (from L2), which bounds how small a tile may be.
 // All tiles run at once and walk the columns together.  Each begins at a chunk of its own: in step they would ask for the same columns of every row, which lie on few
 // of the memory channels (reading 32 768 x 4096 this way: 63 us in step, 46 with the turn; a linear read takes 44).
@@ -118,7 +118,10 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 __device__ __forceinline__ void wait_dma(int n) {
   switch (n) {
 #define PM_CASE(N) case N: asm volatile("s_waitcnt vmcnt(" #N ")" ::: "memory"); break;
-    PM_CASE(2) PM_CASE(3) PM_CASE(4) PM_CASE(5) PM_CASE(6) PM_CASE(7) PM_CASE(8) PM_CASE(9) PM_CASE(10) PM_CASE(11) PM_CASE(12) PM_CASE(13) PM_CASE(14)
+    PM_CASE(1) PM_CASE(2) PM_CASE(3) PM_CASE(4) PM_CASE(5) PM_CASE(6) PM_CASE(7) PM_CASE(8) PM_CASE(9) PM_CASE(10)
+    PM_CASE(11) PM_CASE(12) PM_CASE(13) PM_CASE(14) PM_CASE(15) PM_CASE(16) PM_CASE(17) PM_CASE(18) PM_CASE(19) PM_CASE(20)
+    PM_CASE(21) PM_CASE(22) PM_CASE(23) PM_CASE(24) PM_CASE(25) PM_CASE(26) PM_CASE(27) PM_CASE(28) PM_CASE(29) PM_CASE(30)
+    PM_CASE(31) PM_CASE(32) PM_CASE(33) PM_CASE(34) PM_CASE(35) PM_CASE(36) PM_CASE(37) PM_CASE(38) PM_CASE(39) PM_CASE(40)
 #undef PM_CASE
     default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
   }
@@ -239,44 +242,46 @@ __global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __r
   }
 }
 
-// rank > 16: `rows` positions (a multiple of 16, chosen on the host) up to wide_rows, chunks of KC columns: 64, or 128 for tiles low enough that three such chunks fit the
-// LDS (low tiles need them to keep enough bytes in flight); the waves take every fourth 16 positions and all columns.
-constexpr int wide_rows(int rt, int kc) { return kc == 64 ? 192 : rt <= 4 ? 96 : 64; }
-template <int RT, int KC>
+// rank > 16: `rows` positions (a multiple of 4 up to 192, chosen on the host), chunks of 128 columns, a ring as deep as the LDS takes (2 to 4); the waves take every
+// fourth 16 positions and all columns.
+constexpr int kWideRows = 192, kWideChunk = 128;
+template <int RT>
 __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
                                                           const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank, int rp,
-                                                          int rows, int parts, int chunks_per_part, float* __restrict__ z) {
-  constexpr int kMost = wide_rows(RT, KC), kRowBytes = KC * 2, kBytes = (kMost + RT * 16) * kRowBytes, kPass = 4 * (512 / KC), NW = RT * 16 / kPass;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[kRing * kBytes];
+                                                          int rows, int depth, int parts, int chunks_per_part, float* __restrict__ z) {
+  constexpr int kRowBytes = kWideChunk * 2;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
   const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
   int adapter, p0, p1;
   if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
-  const int nt = (p1 - p0 + kPass - 1) / kPass;  // instructions of a wave that bring the rows, kPass of them by the four waves
-  Ring<KC, 6, NW> ring;
-  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, nt, kMost, wave, lane);
-  const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + KC - 1) / KC - c0);
+  const int nt = (p1 - p0 + 15 - 4 * wave) >> 4;  // instructions of this wave that bring rows, four each; every fourth is its own
+  const int held = (rows + 15) & ~15;
+  Ring<kWideChunk, kWideRows / 16, RT> ring;
+  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, nt, held, wave, lane);
+  const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + kWideChunk - 1) / kWideChunk - c0);
   ring.c0 = c0;
-  ring.full = min(count, d / KC - c0);
+  ring.full = min(count, d / kWideChunk - c0);
   ring.turn = ring.full > 0 ? row_tile % ring.full : 0;
   f32x4 acc[3][RT];
 #pragma unroll
   for (int i = 0; i < 3; ++i)
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int bytes = (held + RT * 16) * kRowBytes, newer = (depth - 2) * (nt + RT);
   unsigned char* mine = lds + wave * 1024;
-  for (int c = 0; c < kRing - 1 && c < count; ++c) ring.fetch(c, mine + c * kBytes, lane);
+  for (int c = 0; c < depth - 1 && c < count; ++c) ring.fetch(c, mine + c * bytes, lane);
   for (int c = 0, buf = 0; c < count; ++c) {
-    wait_dma(c + 1 < ring.full ? nt + NW : 0);
+    wait_dma(c + depth - 2 < ring.full ? newer : 0);
     lds_barrier();
-    if (c + kRing - 1 < count) ring.fetch(c + kRing - 1, mine + (buf + kRing - 1 < kRing ? buf + kRing - 1 : buf - 1) * kBytes, lane);
-    const unsigned char* at = lds + buf * kBytes;
+    if (c + depth - 1 < count) ring.fetch(c + depth - 1, mine + (buf > 0 ? buf - 1 : depth - 1) * bytes, lane);
+    const unsigned char* at = lds + buf * bytes;
 #pragma unroll
-    for (int k = 0; k < KC / 32; ++k) {
-      const int off = lr * kRowBytes + (((k * 4 + lq) ^ (lr & (KC / 8 - 1))) << 4);
+    for (int k = 0; k < kWideChunk / 32; ++k) {
+      const int off = lr * kRowBytes + (((k * 4 + lq) ^ lr) << 4);
       u32x4 wf[RT];
 #pragma unroll
-      for (int j = 0; j < RT; ++j) wf[j] = *reinterpret_cast<const u32x4*>(at + (kMost + j * 16) * kRowBytes + off);
+      for (int j = 0; j < RT; ++j) wf[j] = *reinterpret_cast<const u32x4*>(at + (held + j * 16) * kRowBytes + off);
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
         const int group = i * 4 + wave;
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restri
         for (int j = 0; j < RT; ++j) acc[i][j] = mfma(wf[j], tf, acc[i][j]);
       }
     }
-    buf = buf + 1 < kRing ? buf + 1 : 0;
+    buf = buf + 1 < depth ? buf + 1 : 0;
   }
   const float scale = scales[adapter];
 #pragma unroll
@@ -683,45 +688,53 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // host side
 static inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 static inline int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
+constexpr int kLdsBytes = 160 * 1024;  // of a CU
 struct ShrinkPlan {
-  int rows, chunk, parts, chunks_per_part;
+  int rows, depth, parts, chunks_per_part;
   int64_t tiles;
 };
-// Narrow: 32 positions a tile, two workgroups fit a CU.  Wide: one workgroup fits a CU, so what a launch takes goes with the rounds of 256 tiles times a tile's
-// bytes (its rows and the factor); 257 tiles of 128 rows take 1.5 times as long as 256.  The tile's rows are chosen to make that least.
-// Where the tiles are too few to fill the card, the long axis is cut into parts of at least two chunks.
-static inline ShrinkPlan shrink_plan(int64_t n, int64_t n_adapters, int d, int rank) {
+// Narrow: 32 positions a tile; where the tiles are fewer than the 512 workgroups that run at once, the long axis is cut into parts of at least two chunks.
+// Wide: a tile's rows and the parts are chosen together to make the busiest CU's work least: rounds of 256 workgroups (257 tiles of 128 rows take 1.5 times as long as 256) times
+// what one moves (its rows and the factor, 256 bytes each in a chunk, and a start as long as 160 of these), and the parts of z, which are written and read again.
+static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank) {
   ShrinkPlan p;
   const bool narrow = rank <= 16;
-  p.rows = kNarrowRows;
-  if (!narrow) {
-    int64_t least = INT64_MAX;
-    for (int rows = 16; rows <= 192; rows += 16) {
-      const int64_t cost = cdiv(max_tiles(n, n_adapters, rows), 256) * (rows + rank_tiles(rank) * 16);
-      if (cost <= least) least = cost, p.rows = rows;
+  const int factor = rank_tiles(rank) * 16, chunks = (int)cdiv(d, narrow ? kNarrowChunk : kWideChunk), most = chunks / 2 < 8 ? (chunks / 2 > 1 ? chunks / 2 : 1) : 8;
+  auto parts_of = [&](int64_t tiles, int at_once) { return tiles * most <= at_once ? most : tiles < at_once ? (int)(at_once / tiles) : 1; };
+  if (narrow) {
+    p.rows = kNarrowRows, p.depth = kRing, p.tiles = max_tiles(n, n_adapters, p.rows);
+    p.parts = parts_of(p.tiles > 0 ? p.tiles : 1, 512);
+  } else {
+    double least = 0.0;
+    p.rows = 0;
+    for (int rows = 16; rows <= kWideRows; rows += rows < 64 ? 16 : 4) {
+      const uint32_t worst = ((uint32_t)n + (uint32_t)n_adapters * (uint32_t)(rows - 1)) / (uint32_t)rows, tiles = worst < n ? worst : (uint32_t)n;  // with rows, at most
+      const int parts = parts_of(tiles > 0 ? tiles : 1, 256);
+      const double cost = (double)((tiles * parts + 255) / 256) * ((rows + factor) * ((chunks + parts - 1) / parts) + 160.0) + (parts > 1 ? tiles * parts * rows * factor / (256.0 * 32.0) : 0.0);
+      if (p.rows == 0 || cost <= least) least = cost, p.rows = rows, p.parts = parts;
     }
+    const int fit = kLdsBytes / (((p.rows + 15) / 16 * 16 + factor) * kWideChunk * 2);
+    p.depth = fit >= 6 ? 3 : fit > 4 ? 4 : fit;
+    p.tiles = max_tiles(n, n_adapters, p.rows);
   }
-  p.tiles = max_tiles(n, n_adapters, p.rows);
-  p.chunk = narrow ? kNarrowChunk : p.rows <= wide_rows(rank_tiles(rank), 128) ? 128 : 64;
-  const int64_t chunks = cdiv(d, p.chunk);
-  int64_t parts = (narrow ? 512 : 256) / (p.tiles > 0 ? p.tiles : 1);
-  if (parts > chunks / 2) parts = chunks / 2;
-  p.parts = parts < 1 ? 1 : parts > 8 ? 8 : (int)parts;
-  p.chunks_per_part = (int)cdiv(chunks, p.parts);
+  p.chunks_per_part = (chunks + p.parts - 1) / p.parts;
   return p;
 }
 
 // Ranges of positions in outer.  One workgroup fits a CU: what a launch takes goes with its rounds of 256, times what a workgroup moves, in rows of 512 columns
 // (1 KiB): its positions, and for each adapter among them a partial (written, and read by the join: 4 rank) and the wait for the first stage (as long as about 96 rows).
-static inline int outer_range(int64_t n, int64_t n_adapters, int64_t col_tiles, int rank) {
+static inline int outer_range(int64_t n, int n_adapters, int col_tiles, int rank) {
   double least = 0.0;
-  int64_t best = n > 0 ? n : 1;
-  for (int64_t splits = 1; splits <= n && splits <= 1024; ++splits) {
-    const int64_t range = cdiv(n, splits), used = cdiv(n, range);
-    const double cost = (double)cdiv(used * col_tiles, 256) * ((double)(range < 32 ? 32 : range) + (4.0 * rank + 96.0) * (1.0 + (double)n_adapters / (double)used));
-    if (splits == 1 || cost < least) least = cost, best = range;
+  int best = n > 0 ? (int)n : 1;
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    int splits = 256 * rounds / col_tiles;  // as many as fill the rounds
+    if (splits < 1 && rounds > 1) continue;
+    splits = splits < 1 ? 1 : splits > n ? (int)n : splits;
+    const int range = splits > 0 ? (int)cdiv(n, splits) : 1, used = range > 0 ? (int)cdiv(n, range) : 1;
+    const double cost = (double)((used * col_tiles + 255) / 256) * ((range < 32 ? 32 : range) + (4.0 * rank + 96.0) * (1.0 + (double)n_adapters / (used > 0 ? used : 1)));
+    if (rounds == 1 || cost < least) least = cost, best = range > 0 ? range : 1;
   }
-  return (int)best;
+  return best;
 }
 
 template <int RT>
@@ -731,9 +744,17 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
   if constexpr (RT == 1)
     hipLaunchKernelGGL(shrink_narrow_kernel, grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets, row_ids, (int)n, n_adapters, d, rank, plan.parts,
                        plan.chunks_per_part, z);
-  else
-    hipLaunchKernelGGL((plan.chunk == 128 ? shrink_wide_kernel<RT, 128> : shrink_wide_kernel<RT, 64>), grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales,
-                       offsets, row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.parts, plan.chunks_per_part, z);
+  else {
+    static bool attr_done[64] = {};  // per device: more than 64 KiB of LDS has to be asked for
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    if (!attr_done[dev & 63]) {
+      (void)hipFuncSetAttribute((const void*)shrink_wide_kernel<RT>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+      attr_done[dev & 63] = true;
+    }
+    hipLaunchKernelGGL((shrink_wide_kernel<RT>), grid, dim3(256), plan.depth * ((plan.rows + 15) / 16 * 16 + RT * 16) * kWideChunk * 2, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets,
+                       row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.depth, plan.parts, plan.chunks_per_part, z);
+  }
 }
 template <int RT, bool MERGE>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
@@ -819,8 +840,8 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int rank) {
   BwdPlan p;
-  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
-  p.range = outer_range(n, n_adapters, cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols), rank);
+  p.shrink = shrink_plan(n, (int)n_adapters, (int)d_out, rank);
+  p.range = outer_range(n, (int)n_adapters, (int)(cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols)), rank);
   p.slots = cdiv(n, p.range) + n_adapters;
   p.dz_bytes = (int64_t)p.shrink.parts * n * padded_rank(rank) * 4;
   p.part0_bytes = p.slots * rank * d_out * 4;
