@@ -83,22 +83,30 @@ __global__ __launch_bounds__(256) void squares_kernel(const Chunk* __restrict__ 
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-// group g's partials are [offsets[g], offsets[g + 1]) (offsets null: one each).  coef as torch's clip_grad_norm_ has it: a norm that is not a number leaves none.
+__device__ __forceinline__ float limit_of(int g, float max_norm, const float* max_norms) { return max_norms ? max_norms[g] : max_norm; }
+// as torch's clip_grad_norm_ has it: a norm that is not a number leaves none
+__device__ __forceinline__ float coef_of(float norm, float limit) {
+  const float c = limit > 0.f ? limit / (norm + 1e-6f) : 1.0f;
+  return c > 1.0f ? 1.0f : c;
+}
+// the sum of group g's partials, [lo, hi), in one order wherever it is taken
+__device__ __forceinline__ double group_sum(const double* __restrict__ partials, int lo, int hi, double* smem) {
+  double s = 0.0;
+  for (int i = lo + threadIdx.x; i < hi; i += 256) s += partials[i];
+  return block_sum_f64(s, smem);
+}
+
+// group g's partials are [offsets[g], offsets[g + 1]) (offsets null: one each)
 __global__ __launch_bounds__(256) void coef_kernel(const double* __restrict__ partials, const int32_t* __restrict__ offsets, float max_norm, const float* __restrict__ max_norms,
                                                    double* __restrict__ sumsq, float* __restrict__ norms, float* __restrict__ coefs) {
   __shared__ double smem[4];
   const int g = blockIdx.x;
-  const int lo = offsets ? offsets[g] : g, hi = offsets ? offsets[g + 1] : g + 1;
-  double s = 0.0;
-  for (int i = lo + threadIdx.x; i < hi; i += 256) s += partials[i];
-  s = block_sum_f64(s, smem);
+  const double s = group_sum(partials, offsets ? offsets[g] : g, offsets ? offsets[g + 1] : g + 1, smem);
   if (threadIdx.x) return;
   if (sumsq) sumsq[g] = s;
   if (!norms) return;
-  const float norm = (float)sqrt(s), limit = max_norms ? max_norms[g] : max_norm;
-  norms[g] = norm;
-  const float c = limit > 0.f ? limit / (norm + 1e-6f) : 1.0f;
-  coefs[g] = c > 1.0f ? 1.0f : c;
+  norms[g] = (float)sqrt(s);
+  coefs[g] = coef_of(norms[g], limit_of(g, max_norm, max_norms));
 }
 
 template <bool SRC_BF16, bool DST_BF16>
@@ -147,9 +155,7 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float coef) {
   if (tail + threadIdx.x < c.n) put(tail + threadIdx.x, one<SRC_BF16>(c.src, tail + threadIdx.x) * coef);
 }
 
-__global__ __launch_bounds__(256) void scale_kernel(const Chunk* __restrict__ chunks, const float* __restrict__ coefs) {
-  const Chunk c = chunks[blockIdx.x];
-  const float coef = coefs[c.flags >> 8];
+__device__ __forceinline__ void scale_any(const Chunk& c, float coef) {
   if (!c.dst || (coef == 1.0f && c.dst == c.src)) return;  // in place, nothing to clip: every value times one is itself
   switch (c.flags & 3) {
     case 0: scale_chunk<false, false>(c, coef); break;
@@ -157,6 +163,31 @@ __global__ __launch_bounds__(256) void scale_kernel(const Chunk* __restrict__ ch
     case 2: scale_chunk<false, true>(c, coef); break;
     default: scale_chunk<true, true>(c, coef); break;
   }
+}
+// the last chunks first: they were read last and are still in the caches
+__global__ __launch_bounds__(256) void scale_kernel(const Chunk* __restrict__ chunks, const float* __restrict__ coefs) {
+  const Chunk c = chunks[gridDim.x - 1 - blockIdx.x];
+  scale_any(c, coefs[c.flags >> 8]);
+}
+// The same where groups are of few chunks: every workgroup adds up its group's partials itself, which takes less than a launch for it would.  The first workgroups write the
+// groups' norms and factors.
+__global__ __launch_bounds__(256) void coef_scale_kernel(const Chunk* __restrict__ chunks, int n_groups, const double* __restrict__ partials, const int32_t* __restrict__ offsets,
+                                                         float max_norm, const float* __restrict__ max_norms, double* __restrict__ sumsq, float* __restrict__ norms,
+                                                         float* __restrict__ coefs) {
+  __shared__ double smem[2][4];
+  const Chunk c = chunks[blockIdx.x];
+  const int own = (int)(c.flags >> 8);
+  const float coef = coef_of((float)sqrt(group_sum(partials, offsets[own], offsets[own + 1], smem[0])), limit_of(own, max_norm, max_norms));
+  for (int g = blockIdx.x; g < n_groups; g += gridDim.x) {
+    __syncthreads();
+    const double s = group_sum(partials, offsets[g], offsets[g + 1], smem[1]);
+    if (threadIdx.x == 0) {
+      if (sumsq) sumsq[g] = s;
+      norms[g] = (float)sqrt(s);
+      coefs[g] = coef_of(norms[g], limit_of(g, max_norm, max_norms));
+    }
+  }
+  scale_any(c, coef);
 }
 
 }  // namespace gclip
@@ -174,6 +205,11 @@ extern "C" int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32
   if (n_chunks > 0 && !sumsq_in) {
     hipLaunchKernelGGL(gclip::squares_kernel, dim3((unsigned)n_chunks), dim3(256), 0, st, table, partials);
     PM_CHECK_LAUNCH("pm_grad_clip");
+  }
+  if (scale && !sumsq_in && n_chunks > 0 && n_chunks <= 1024) {
+    hipLaunchKernelGGL(gclip::coef_scale_kernel, dim3((unsigned)n_chunks), dim3(256), 0, st, table, n_groups, partials, group_offsets, max_norm, max_norms, sumsq_out, norms, coefs);
+    PM_CHECK_LAUNCH("pm_grad_clip");
+    return PM_OK;
   }
   hipLaunchKernelGGL(gclip::coef_kernel, dim3(n_groups), dim3(256), 0, st, sumsq_in ? sumsq_in : partials, sumsq_in ? nullptr : group_offsets, max_norm, max_norms, sumsq_out, norms, coefs);
   PM_CHECK_LAUNCH("pm_grad_clip");

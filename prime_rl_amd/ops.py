@@ -1081,62 +1081,60 @@ def gemm_set_variant(v: int) -> None:
 
 
 # ------------------------------------------------------------------------------------------------ adapters of many runs
-def _one_device(what: str, *tensors: Tensor | None) -> torch.device:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise PrimeMI355XError(f"{what}: expected all tensors on one GPU, got {sorted(map(str, devices))}")
-    return devices.pop()
-
-
-def _launch(fn, what: str, device: torch.device, *args) -> None:
+def _launch(fn, what: str, tensors: tuple, *args) -> None:
     """The call on the current stream of the tensors' device, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, _stream()), what)
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise PrimeMI355XError(f"{what}: expected all tensors on one GPU, got {[str(u.device) for u in tensors if u is not None]}")
+    if index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _stream()), what)
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
 def _lora_rows(t: Tensor, rows: int, width: int, name: str) -> int:
     """Row stride of a [rows, width] bf16 tensor whose rows lie one behind the other, with or without a gap."""
-    _req(t, torch.bfloat16, name, contiguous=False)
-    if t.dim() != 2 or t.shape != (rows, width):
+    if t.dtype != torch.bfloat16 or not t.is_cuda:
+        _req(t, torch.bfloat16, name, contiguous=False)
+    if t.shape != (rows, width):
         raise PrimeMI355XError(f"{name}: expected [{rows}, {width}], got {tuple(t.shape)}")
     if rows == 0:
         return width
-    if t.stride(1) != 1 or (rows > 1 and (t.stride(0) < width or t.stride(0) % 8)) or t.data_ptr() % 16:
+    ld, step = t.stride()
+    if step != 1 or (rows > 1 and (ld < width or ld % 8)) or t.data_ptr() % 16:
         raise PrimeMI355XError(f"{name}: rows must be contiguous, start 16-byte aligned and not overlap, got strides {t.stride()}")
-    return t.stride(0) if rows > 1 else width
+    return ld if rows > 1 else width
 
 
-def _share_memory(a: Tensor, b: Tensor) -> bool:
-    """Whether two 2-D bf16 row tensors have an element in common (column slices of one buffer have none)."""
-    if a.numel() == 0 or b.numel() == 0:
+def _share_memory(a: Tensor, ld_a: int, b: Tensor, ld_b: int) -> bool:
+    """Whether two bf16 row tensors have an element in common (column slices of one buffer have none)."""
+    (rows_a, width_a), (rows_b, width_b) = a.shape, b.shape
+    at_a, at_b = a.data_ptr() // 2, b.data_ptr() // 2
+    if at_a + (rows_a - 1) * ld_a + width_a <= at_b or at_b + (rows_b - 1) * ld_b + width_b <= at_a or not rows_a or not rows_b:
         return False
-    lo_a, lo_b = a.data_ptr() // 2, b.data_ptr() // 2
-    hi_a, hi_b = (t + (u.shape[0] - 1) * u.stride(0) + u.shape[1] for t, u in ((lo_a, a), (lo_b, b)))
-    if hi_a <= lo_b or hi_b <= lo_a:
-        return False
-    ld = a.stride(0)
-    if a.shape[0] > 1 and b.shape[0] > 1 and ld == b.stride(0):
-        at = (lo_b - lo_a) % ld
-        return at < a.shape[1] or ld - at < b.shape[1]
+    if rows_a > 1 and rows_b > 1 and ld_a == ld_b:
+        at = (at_b - at_a) % ld_a
+        return at < width_a or ld_a - at < width_b
     return True
 
 
 def _lora_factors(a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, row_ids: Tensor | None, rows: int) -> tuple[int, int, int, int]:
-    _req(a, torch.bfloat16, "a"); _req(b, torch.bfloat16, "b")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[:2] != b.shape[:2]:
-        raise PrimeMI355XError(f"a / b: expected [n_adapters, rank, d_in] and [n_adapters, rank, d_out], got {tuple(a.shape)} and {tuple(b.shape)}")
-    n, rank, d_in = a.shape
-    _req(scales, torch.float32, "scales"); _req(offsets, torch.int32, "offsets")
+    for t, dtype, nm in ((a, torch.bfloat16, "a"), (b, torch.bfloat16, "b"), (scales, torch.float32, "scales"), (offsets, torch.int32, "offsets")):
+        if t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+            _req(t, dtype, nm)
+    sa, sb = a.shape, b.shape
+    if len(sa) != 3 or len(sb) != 3 or sa[:2] != sb[:2]:
+        raise PrimeMI355XError(f"a / b: expected [n_adapters, rank, d_in] and [n_adapters, rank, d_out], got {tuple(sa)} and {tuple(sb)}")
+    n, rank, d_in = sa
     if scales.numel() != n or offsets.numel() != n + 1:
         raise PrimeMI355XError(f"{n} adapters: expected {n} scales and {n + 1} offsets, got {scales.numel()} and {offsets.numel()}")
     if row_ids is not None:
         _req(row_ids, torch.int32, "row_ids")
         if row_ids.numel() != rows:
             raise PrimeMI355XError(f"row_ids: expected one for each of {rows} rows, got {row_ids.numel()}")
-    return n, rank, d_in, b.shape[2]
+    return n, rank, d_in, sb[2]
 
 
 def lora_rows(adapter_ids: Tensor, n_adapters: int) -> tuple[Tensor, Tensor]:
@@ -1156,23 +1154,22 @@ def lora_fwd(x: Tensor, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, b
     x [N, d_in], base [N, d_out] (None: zeros) bf16, with row strides; a [n, rank, d_in], b [n, rank, d_out] bf16; scales [n] f32.  Position p, in
     [offsets[g], offsets[g + 1]) of adapter g, is row `row_ids[p]` (`lora_rows`), or row p without row_ids.  `out` may be `base` (in place).  z is what `lora_bwd` takes."""
     lib = _lib.load()
-    if x.dim() != 2:
-        raise PrimeMI355XError(f"x: expected [rows, d_in], got {tuple(x.shape)}")
     rows = x.shape[0]
     n, rank, d_in, d_out = _lora_factors(a, b, scales, offsets, row_ids, rows)
     ldx = _lora_rows(x, rows, d_in, "x")
     ldb = _lora_rows(base, rows, d_out, "base") if base is not None else 0
     if out is None:
         out = torch.empty((rows, d_out), dtype=torch.bfloat16, device=x.device)
-    ldo = _lora_rows(out, rows, d_out, "out")
-    device = _one_device("lora_fwd", x, a, b, scales, offsets, row_ids, base, out)
-    if base is not None and not (base.data_ptr() == out.data_ptr() and ldb == ldo) and _share_memory(base, out):
-        raise PrimeMI355XError("out overlaps base: it may be base itself or memory of its own")
-    z = torch.empty((rows, lib.pm_lora_z_columns(rank)), dtype=torch.float32, device=device)
+        ldo = d_out
+    else:
+        ldo = _lora_rows(out, rows, d_out, "out")
+        if base is not None and not (base.data_ptr() == out.data_ptr() and ldb == ldo) and _share_memory(base, ldb, out, ldo):
+            raise PrimeMI355XError("out overlaps base: it may be base itself or memory of its own")
+    z = torch.empty((rows, (rank + 15) // 16 * 16), dtype=torch.float32, device=x.device)
     nbytes = lib.pm_lora_fwd_workspace_bytes(rows, n, d_in, rank)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None  # of its own for each call: a captured graph keeps it
-    _launch(lib.pm_lora_fwd, "pm_lora_fwd", device, _p(x), ldx, _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb, _p(out), ldo, _p(z),
-            _p(ws), nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None  # of its own for each call: a captured graph keeps it
+    _launch(lib.pm_lora_fwd, "pm_lora_fwd", (x, a, b, scales, offsets, row_ids, base, out), x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), offsets.data_ptr(),
+            _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb, out.data_ptr(), ldo, z.data_ptr(), _p(ws), nbytes)
     return out, z
 
 
@@ -1183,8 +1180,6 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
     projection's row gradient, None: zeros; `grad_x` may be `base`), grad_a[g] = dz.T @ x, grad_b[g] = z.T @ grad_out in f32 — written, or added to the given
     buffers with `accumulate`.  What is not wanted (`want_x`, `want_factors`) comes back as None; without the factors' gradients x and z may be None."""
     lib = _lib.load()
-    if grad_out.dim() != 2:
-        raise PrimeMI355XError(f"grad_out: expected [rows, d_out], got {tuple(grad_out.shape)}")
     rows = grad_out.shape[0]
     n, rank, d_in, d_out = _lora_factors(a, b, scales, offsets, row_ids, rows)
     ldg = _lora_rows(grad_out, rows, d_out, "grad_out")
@@ -1194,8 +1189,8 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
             raise PrimeMI355XError("the factors' gradients need x and the forward's z")
         ldx = _lora_rows(x, rows, d_in, "x")
         _req(z, torch.float32, "z")
-        if z.shape != (rows, lib.pm_lora_z_columns(rank)):
-            raise PrimeMI355XError(f"z: expected {(rows, lib.pm_lora_z_columns(rank))} as lora_fwd returns it, got {tuple(z.shape)}")
+        if z.shape != (rows, (rank + 15) // 16 * 16):
+            raise PrimeMI355XError(f"z: expected {(rows, (rank + 15) // 16 * 16)} as lora_fwd returns it, got {tuple(z.shape)}")
         if (grad_a is None) != (grad_b is None) or (accumulate and grad_a is None):
             raise PrimeMI355XError("grad_a and grad_b go together, and accumulating needs them")
         if grad_a is None:
@@ -1210,17 +1205,16 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
         ldb = _lora_rows(base, rows, d_in, "base") if base is not None else 0
         if grad_x is None:
             grad_x = torch.empty((rows, d_in), dtype=torch.bfloat16, device=grad_out.device)
-        ldgx = _lora_rows(grad_x, rows, d_in, "grad_x")
-        if base is not None and not (base.data_ptr() == grad_x.data_ptr() and ldb == ldgx) and _share_memory(base, grad_x):
-            raise PrimeMI355XError("grad_x overlaps base: it may be base itself or memory of its own")
-        if want_factors and (_share_memory(grad_x, grad_out) or _share_memory(grad_x, x)):
-            raise PrimeMI355XError("grad_x overlaps grad_out or x, which are still read after it is written")
+            ldgx = d_in
+        else:
+            ldgx = _lora_rows(grad_x, rows, d_in, "grad_x")
+            if base is not None and not (base.data_ptr() == grad_x.data_ptr() and ldb == ldgx) and _share_memory(base, ldb, grad_x, ldgx):
+                raise PrimeMI355XError("grad_x overlaps base: it may be base itself or memory of its own")
     else:
         base = grad_x = None
-    device = _one_device("lora_bwd", grad_out, x, z, a, b, scales, offsets, row_ids, base, grad_x, grad_a, grad_b)
     nbytes = lib.pm_lora_bwd_workspace_bytes(rows, n, d_in, d_out, rank)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _launch(lib.pm_lora_bwd, "pm_lora_bwd", device, _p(grad_out), ldg, _p(x), ldx, _p(z), _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb,
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad_out.device) if nbytes else None
+    _launch(lib.pm_lora_bwd, "pm_lora_bwd", (grad_out, x, z, a, b, scales, offsets, row_ids, base, grad_x, grad_a, grad_b), _p(grad_out), ldg, _p(x), ldx, _p(z), _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb,
             _p(grad_x), ldgx, _p(grad_a), _p(grad_b), 1 if accumulate else 0, _p(ws), nbytes)
     return grad_x, grad_a, grad_b
 
@@ -1236,11 +1230,12 @@ def lora_merge(weight: Tensor, a: Tensor, b: Tensor, scale: float, out: Tensor |
     ldw = _lora_rows(weight, d_out, d_in, "weight")
     if out is None:
         out = torch.empty((d_out, d_in), dtype=torch.bfloat16, device=weight.device)
-    ldo = _lora_rows(out, d_out, d_in, "out")
-    device = _one_device("lora_merge", weight, a, b, out)
-    if not (weight.data_ptr() == out.data_ptr() and ldw == ldo) and _share_memory(weight, out):
-        raise PrimeMI355XError("out overlaps weight: it may be weight itself or memory of its own")
-    _launch(lib.pm_lora_merge, "pm_lora_merge", device, _p(weight), ldw, _p(a), _p(b), float(scale), d_in, d_out, rank, _p(out), ldo)
+        ldo = d_in
+    else:
+        ldo = _lora_rows(out, d_out, d_in, "out")
+        if not (weight.data_ptr() == out.data_ptr() and ldw == ldo) and _share_memory(weight, ldw, out, ldo):
+            raise PrimeMI355XError("out overlaps weight: it may be weight itself or memory of its own")
+    _launch(lib.pm_lora_merge, "pm_lora_merge", (weight, a, b, out), _p(weight), ldw, _p(a), _p(b), float(scale), d_in, d_out, rank, _p(out), ldo)
     return out
 
 
@@ -1274,7 +1269,9 @@ class GradClipPlan:
                 raise PrimeMI355XError(f"out[{i}]: in place only in the gradient's own type")
         if not grads:
             raise PrimeMI355XError("grads: no tensors")
-        self.device = _one_device("GradClipPlan", *grads, *dst)
+        self.device = grads[0].device
+        if any(t.device != self.device for t in (*grads, *dst)):
+            raise PrimeMI355XError(f"GradClipPlan: expected all tensors on {self.device}")
         self._held = [t.detach() for t in (*grads, *dst)]
         src = np.array([(t.data_ptr(), t.numel() * t.element_size(), i) for i, t in enumerate(grads) if t.numel()], dtype=np.int64).reshape(-1, 3)
         own = np.array([(o.data_ptr(), o.numel() * o.element_size(), i) for i, o in enumerate(dst) if o.numel()], dtype=np.int64).reshape(-1, 3)
@@ -1301,18 +1298,21 @@ class GradClipPlan:
         lib = _lib.load()
         limits = None
         if isinstance(max_norm, Tensor):
-            limits = _req(max_norm, torch.float32, "max_norm")
+            limits, max_norm = _req(max_norm, torch.float32, "max_norm"), 0.0
         if sumsq is not None:
             _req(sumsq, torch.float64, "sumsq")
         for t, nm in ((limits, "max_norm"), (sumsq, "sumsq")):
             if t is not None and (t.numel() != self.n_groups or t.device != self.device):
                 raise PrimeMI355XError(f"{nm}: expected {self.n_groups} values on {self.device}, got {t.numel()} on {t.device}")
-        partials = torch.empty(max(self.n_chunks, 1), dtype=torch.float64, device=self.device) if sumsq is None else None
-        sums = torch.empty(self.n_groups, dtype=torch.float64, device=self.device) if want_sumsq else None
-        both = None if want_sumsq else torch.empty((2, self.n_groups), dtype=torch.float32, device=self.device)
-        norms, coefs = (None, None) if both is None else (both[0], both[1])
-        _launch(lib.pm_grad_clip, "pm_grad_clip", self.device, _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(sumsq), 0.0 if limits is not None else float(max_norm),
-                _p(limits), _p(partials), _p(sums), _p(norms), _p(coefs), 1 if scale else 0)
+        partials = torch.empty(self.n_chunks + 1, dtype=torch.float64, device=self.device) if sumsq is None else None
+        sums = both = norms = coefs = None
+        if want_sumsq:
+            sums = torch.empty(self.n_groups, dtype=torch.float64, device=self.device)
+        else:
+            both = torch.empty((2, self.n_groups), dtype=torch.float32, device=self.device)
+            norms, coefs = both.unbind()
+        _launch(lib.pm_grad_clip, "pm_grad_clip", (self._table,), _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(sumsq), max_norm, _p(limits), _p(partials), _p(sums),
+                _p(norms), _p(coefs), 1 if scale else 0)
         return sums, norms, coefs
 
     def sumsq(self) -> Tensor:
