@@ -587,14 +587,15 @@ int pm_lora_bwd(const void* grad_out_bf16, int64_t ldg, const void* x_bf16, int6
                 int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream);
 int pm_lora_merge(const void* weight_bf16, int64_t ldw, const void* a_bf16, const void* b_bf16, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out_bf16, int64_t ldo,
                   void* stream);
-/* Gradient norms of many tensors by group, and clipping (torch clip_grad_norm_ over each group; trainer/utils.py:88-98).  `chunks`: int64 [n_chunks][4] on the device, rows
- * {source address, destination address (0: none), elements, (group << 8) | source is bf16 (bit 0) | destination is bf16 (bit 1)}, f32 where a bit is clear; the chunks of one group
- * stand together, group g's at [group_offsets[g], group_offsets[g+1]) (int32 [n_groups + 1]).  Destinations are their source (same type) or memory of their own.
+/* Gradient norms of many tensors by group, and clipping (torch clip_grad_norm_ over each group; trainer/utils.py:88-98).  `chunks` and `pieces`: int64 [n][4] on the device, rows
+ * {source address, destination address (0: none), elements, (group << 8) | source is bf16 (bit 0) | destination is bf16 (bit 1)}, f32 where a bit is clear.  The chunks (what is
+ * added up) of one group stand together, group g's at [group_offsets[g], group_offsets[g+1]) (int32 [n_groups + 1]); the pieces (what is scaled; n_pieces 0: nothing) are any cut of the
+ * same memory, about 2048 elements each.  Destinations are their source (same type) or memory of their own.
  *   sumsq_out[g] = sum of squares in 64 bits (nullable); norms[g] = sqrt of it; coefs[g] = min(1, max_norm / (norms[g] + 1e-6)), 1 for max_norm <= 0 (max_norms [n_groups], where it
- *   is not NULL, in the place of max_norm); with scale != 0, destination = source * coefs[group].  sumsq_in (nullable) stands in for the sums: what an all-reduce over ranks made of
- *   them.  norms and coefs may both be NULL where only sumsq_out is wanted.  partials: f64 [n_chunks] of the caller's. */
-int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32_t* group_offsets, int32_t n_groups, const double* sumsq_in /* nullable */, float max_norm,
-                 const float* max_norms /* nullable */, double* partials, double* sumsq_out /* nullable */, float* norms /* nullable */, float* coefs /* nullable */, int32_t scale,
+ *   is not NULL, in the place of max_norm); destination = source * coefs[group].  sumsq_in (nullable) stands in for the sums: what an all-reduce over ranks made of them.  norms and
+ *   coefs may both be NULL where only sumsq_out is wanted.  partials: f64 [n_chunks] of the caller's. */
+int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32_t* group_offsets, int32_t n_groups, const int64_t* pieces, int64_t n_pieces, const double* sumsq_in /* nullable */,
+                 float max_norm, const float* max_norms /* nullable */, double* partials, double* sumsq_out /* nullable */, float* norms /* nullable */, float* coefs /* nullable */,
                  void* stream);
 
 /* --------------------------------------------------------------------------------------------

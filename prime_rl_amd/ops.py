@@ -1246,7 +1246,7 @@ class GradClipPlan:
     receives the clipped grads[i] — e.g. a slice of the flat f32 gradient that `adamw_step` reads; without `out` the gradients are clipped in place.  The plan
     holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are."""
 
-    _CHUNK_MOST, _CHUNK_LEAST = 32768, 2048
+    _CHUNK_MOST, _PIECE = 65536, 2048
 
     def __init__(self, grads: list[Tensor], groups: list[int] | None = None, n_groups: int | None = None, out: list[Tensor] | None = None):
         import numpy as np
@@ -1279,19 +1279,23 @@ class GradClipPlan:
         spans = spans[np.argsort(spans[:, 0], kind="stable")]
         if np.any(spans[1:, 0] < spans[:-1, 0] + spans[:-1, 1]):
             raise PrimeMI355XError("gradients (or their outputs) overlap in memory: each may be there once")
-        # chunks: of 32 Ki elements, fewer where there is less to share out among the CUs; a group's chunks stand together
+        # chunks are added up: of 64 Ki elements, fewer where there is less to share out among the CUs; pieces are scaled.  A group's stand together.
         numel = np.array([t.numel() for t in grads], dtype=np.int64)
-        self.chunk = int(min(self._CHUNK_MOST, max(self._CHUNK_LEAST, -(-int(numel.sum()) // 1024) // 1024 * 1024)))
         order = np.argsort(np.array(groups), kind="stable")
-        count = -(-numel[order] // self.chunk)
-        of = np.repeat(order, count)
-        first = (np.arange(of.size) - np.repeat(np.cumsum(count) - count, count)) * self.chunk
         size = [np.array([t.element_size() for t in ts], dtype=np.int64) for ts in (grads, dst)]
         at = [np.array([t.data_ptr() for t in ts], dtype=np.int64) for ts in (grads, dst)]
         flags = np.array(groups, dtype=np.int64) * 256 + (size[0] == 2) + 2 * (size[1] == 2)
-        table = np.stack([at[0][of] + first * size[0][of], at[1][of] + first * size[1][of], np.minimum(self.chunk, numel[of] - first), flags[of]], axis=1)
-        self.n_chunks = int(of.size)
-        self._table = torch.from_numpy(np.ascontiguousarray(table)).to(self.device)
+
+        def cut(length: int):
+            count = -(-numel[order] // length)
+            of = np.repeat(order, count)
+            first = (np.arange(of.size) - np.repeat(np.cumsum(count) - count, count)) * length
+            return of, np.stack([at[0][of] + first * size[0][of], at[1][of] + first * size[1][of], np.minimum(length, numel[of] - first), flags[of]], axis=1)
+
+        of, chunks = cut(int(min(self._CHUNK_MOST, max(self._PIECE, int(numel.sum()) // 1024 // 1024 * 1024))))
+        _, pieces = cut(self._PIECE)
+        self.n_chunks, self.n_pieces = len(chunks), len(pieces)
+        self._table, self._pieces = (torch.from_numpy(np.ascontiguousarray(t)).to(self.device) for t in (chunks, pieces))
         self._offsets = torch.from_numpy(np.searchsorted(np.array(groups, dtype=np.int64)[of], np.arange(self.n_groups + 1)).astype(np.int32)).to(self.device)
 
     def _run(self, max_norm, sumsq: Tensor | None, want_sumsq: bool, scale: bool) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
@@ -1311,8 +1315,8 @@ class GradClipPlan:
         else:
             both = torch.empty((2, self.n_groups), dtype=torch.float32, device=self.device)
             norms, coefs = both.unbind()
-        _launch(lib.pm_grad_clip, "pm_grad_clip", (self._table,), _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(sumsq), max_norm, _p(limits), _p(partials), _p(sums),
-                _p(norms), _p(coefs), 1 if scale else 0)
+        _launch(lib.pm_grad_clip, "pm_grad_clip", (self._table,), _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(self._pieces), self.n_pieces if scale else 0,
+                _p(sumsq), max_norm, _p(limits), _p(partials), _p(sums), _p(norms), _p(coefs))
         return sums, norms, coefs
 
     def sumsq(self) -> Tensor:
