@@ -18,6 +18,7 @@ from torch import nn
 
 from .... import ops
 from .linear import fused_linear, linear
+from .lora import adapters_of, lora_linear
 from .norms import RMSNorm, RMSNormConfig
 
 
@@ -159,7 +160,12 @@ class HipVarlenAttention(nn.Module):
         assert b == 1, "packed batches are [1, N, H] (trainer/batch.py)"
         x = hidden_states[0]
         # one q|k|v product on the hand-written core when the three weights lie back to back (a trainer engine's flat buffer); else three + a concatenation
-        qkv = fused_linear(x, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], [self.q_proj.bias, self.k_proj.bias, self.v_proj.bias])
+        projections = [self.q_proj, self.k_proj, self.v_proj]
+        adapters = adapters_of(projections)
+        if adapters is not None:
+            qkv = lora_linear(x, projections, adapters)
+        else:
+            qkv = fused_linear(x, [p.weight for p in projections], [p.bias for p in projections])
         cos, sin = position_embeddings
         half = self.head_dim // 2
         # accept the reference's cat(f,f) tables too; the kernels read bf16 (the reference casts cos/sin to x.dtype, rotary_emb.py:72-73)
@@ -170,7 +176,9 @@ class HipVarlenAttention(nn.Module):
             seq_start = ops.seq_start_with_window(seq_start, sliding_window)
         qw, kw = (self.q_norm.weight, self.k_norm.weight) if self.use_qk_norm else (None, None)
         out = _QKVAttnFn.apply(qkv.contiguous(), qw, kw, cos, sin, seq_start, self.hq, self.hkv, self.head_dim, self.eps if self.use_qk_norm else 0.0, self.scaling)
-        return linear(out.view(n, self.hq * self.head_dim), self.o_proj.weight).unsqueeze(0), None
+        out = out.view(n, self.hq * self.head_dim)
+        adapters = adapters_of([self.o_proj])
+        return (linear(out, self.o_proj.weight) if adapters is None else lora_linear(out, [self.o_proj], adapters)).unsqueeze(0), None
 
 
 ATTN_IMPL2CLASS = {"hip_varlen": HipVarlenAttention}

@@ -1,0 +1,197 @@
+"""Low-rank adapters of many runs on the dense projections — the LoRA linears of the reference's multi-run trainer (src/prime_rl/trainer/models/layers/lora) on the
+adapter kernels (csrc/lora.hip).
+
+One frozen model serves every run: run g's rows of a pass (the micro-batch's `lora_num_tokens`, trainer/rl/data.py) get `scale[g] * (x A_g^T) B_g` added to the
+shared projection's output.  `attach_lora(model, ...)` hangs a `LoRAAdapters` on the chosen `nn.Linear`s as their submodule `lora` (the linear keeps its name and
+weight) and freezes everything else; the layer seams (layers/attn.py, layers/mlp.py) then run `lora_linear` in the place of `linear` / `fused_linear`: the products of
+layers/linear.py with every adapter's update added in place to its columns, and one autograd node for all of it.
+
+Factors are rank-major, `a [n, rank, in]` and `b [n, rank, out]` (a checkpoint's `lora_B [out, rank]` is `b[g].T`).  Parameters are f32 (the products take them as
+bf16): adapters are small, and their gradients arrive in f32 without a rounding."""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Iterable, Sequence
+
+import torch
+import torch.nn.functional as F
+from torch import Tensor, nn
+
+from .... import ops
+from .linear import _adjacent_view
+
+
+class LoRARows:
+    """Which rows of a pass belong to which adapter: `offsets` i32 [n + 1], adapter g owns positions [offsets[g], offsets[g + 1]); `row_ids` i32 [rows] or None
+    (position p is row p)."""
+
+    def __init__(self, offsets: Tensor, row_ids: Tensor | None = None):
+        self.offsets, self.row_ids = offsets, row_ids
+
+    @classmethod
+    def packed(cls, num_tokens: Sequence[int] | Tensor, device) -> LoRARows:
+        """Runs packed one behind the other, `num_tokens[g]` rows of run g (`lora_num_tokens`); rows behind the last run belong to none."""
+        counts = torch.as_tensor(num_tokens, dtype=torch.int32).reshape(-1)
+        if not counts.is_cuda and counts.numel() and int(counts.min()) < 0:
+            raise ValueError(f"num_tokens: expected no negative counts, got {counts.tolist()}")
+        offsets = torch.zeros(counts.numel() + 1, dtype=torch.int32, device=counts.device)
+        offsets[1:] = counts.cumsum(0)
+        return cls(offsets.to(device))
+
+    @classmethod
+    def of(cls, adapter_ids: Tensor, n_adapters: int) -> LoRARows:
+        """Rows in any order, `adapter_ids[row]` their adapter (outside [0, n_adapters): none)."""
+        return cls(*ops.lora_rows(adapter_ids, n_adapters))
+
+
+class LoRAState:
+    """What all adapters of a model share: their number, rank and scales, and the rows of the pass that is to run."""
+
+    def __init__(self, n_adapters: int, rank: int, alpha: float | Sequence[float], device):
+        alphas = list(alpha) if isinstance(alpha, Iterable) else [alpha] * n_adapters
+        if n_adapters < 1 or rank < 1 or len(alphas) != n_adapters:
+            raise ValueError(f"expected one alpha for each of {n_adapters} adapters of rank {rank}, got {len(alphas)}")
+        self.n_adapters, self.rank = n_adapters, rank
+        self.scales = torch.tensor([x / rank for x in alphas], dtype=torch.float32, device=device)
+        self.rows: LoRARows | None = None
+
+    def set_rows(self, rows: LoRARows) -> None:
+        if rows.offsets.numel() != self.n_adapters + 1:
+            raise ValueError(f"rows of {rows.offsets.numel() - 1} adapters for a model of {self.n_adapters}")
+        self.rows = rows
+
+
+class LoRAAdapters(nn.Module):
+    """The adapters of one projection; `a` starts uniform (as nn.Linear's weight does), `b` at zero: the update starts at zero."""
+
+    def __init__(self, linear: nn.Linear, state: LoRAState):
+        super().__init__()
+        self.state = state
+        device = linear.weight.device
+        self.a = nn.Parameter(torch.empty(state.n_adapters, state.rank, linear.in_features, dtype=torch.float32, device=device))
+        self.b = nn.Parameter(torch.zeros(state.n_adapters, state.rank, linear.out_features, dtype=torch.float32, device=device))
+        nn.init.uniform_(self.a, -1.0 / math.sqrt(linear.in_features), 1.0 / math.sqrt(linear.in_features))
+
+
+def adapters_of(linears: Sequence[nn.Linear]) -> list[LoRAAdapters | None] | None:
+    """The adapters of each projection, None where none of them has any."""
+    found = [getattr(lin, "lora", None) for lin in linears]
+    return found if any(f is not None for f in found) else None
+
+
+def _product(x: Tensor, w: Tensor, bias: Tensor | None, out: Tensor) -> None:
+    """out = x @ w.T (+ bias) on the core where it takes the shapes."""
+    if ops.gemm_supported(x, w, out=out):
+        ops.gemm(x, w, out=out, bias=bias)
+    else:
+        out.copy_(F.linear(x, w, bias))
+
+
+class _LoRALinearFn(torch.autograd.Function):
+    """cat([x @ w_i.T + bias_i + update_i]) over several projections of the same rows; the updates go into the output's columns in place."""
+
+    @staticmethod
+    def forward(ctx, x, rows, scales, has_adapter, weights, biases, *factors):
+        n, widths = x.shape[0], [w.shape[0] for w in weights]
+        y = torch.empty((n, sum(widths)), dtype=x.dtype, device=x.device)
+        joined = _adjacent_view(weights)
+        if joined is not None and all(b is None for b in biases):
+            _product(x, joined, None, y)
+        else:
+            for w, b, part in zip(weights, biases, y.split(widths, dim=1)):
+                _product(x, w, b, part)
+        halves = [f.detach().to(torch.bfloat16) for f in factors]
+        zs, at = [], 0
+        for i, part in enumerate(y.split(widths, dim=1)):
+            if has_adapter[i]:
+                zs.append(ops.lora_fwd(x, halves[at], halves[at + 1], scales, rows.offsets, base=part, row_ids=rows.row_ids, out=part)[1])
+                at += 2
+        ctx.save_for_backward(x, scales, *halves, *zs)
+        ctx.rows, ctx.has_adapter, ctx.weights, ctx.joined, ctx.widths = rows, has_adapter, weights, joined, widths
+        ctx.dtypes = [f.dtype for f in factors]
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, scales, *rest = ctx.saved_tensors
+        n_factors = len(ctx.dtypes)
+        halves, zs = rest[:n_factors], rest[n_factors:]
+        dy = dy if dy.stride(1) == 1 and dy.stride(0) % 8 == 0 and dy.data_ptr() % 16 == 0 else dy.contiguous()
+        want_x, want_factors = ctx.needs_input_grad[0], any(ctx.needs_input_grad[6:])
+        dx, parts = None, dy.split(ctx.widths, dim=1)
+        if want_x:
+            pairs = [(dy, ctx.joined)] if ctx.joined is not None else list(zip(parts, ctx.weights))
+            for d, w in pairs:
+                step = ops.gemm(d, w.t()) if ops.gemm_supported(d, w.t()) else d @ w
+                dx = step if dx is None else dx.add_(step)
+        grads: list[Tensor] = []
+        for i, d in enumerate(parts):
+            if not ctx.has_adapter[i]:
+                continue
+            k = len(grads)
+            _, da, db = ops.lora_bwd(d, x, zs[k // 2], halves[k], halves[k + 1], scales, ctx.rows.offsets, base=dx, row_ids=ctx.rows.row_ids, grad_x=dx, want_x=want_x,
+                                     want_factors=want_factors)
+            grads += [da, db]
+        if not want_factors:
+            return dx, None, None, None, None, None, *([None] * n_factors)
+        return dx, None, None, None, None, None, *(g.to(t) for g, t in zip(grads, ctx.dtypes))
+
+
+def lora_linear(x: Tensor, linears: Sequence[nn.Linear], adapters: Sequence[LoRAAdapters | None] | None = None) -> Tensor:
+    """cat([linear_i(x)], dim=-1) with the projections' adapters for x [N, in] bf16 rows of the pass that `LoRAState.set_rows` described.  The shared weights are
+    frozen: gradients go to x and the adapters."""
+    adapters = adapters if adapters is not None else adapters_of(linears)
+    if adapters is None:
+        raise ValueError("none of the projections has adapters")
+    if any(p is not None and p.requires_grad for lin in linears for p in (lin.weight, lin.bias)):
+        raise ValueError("the projections beside adapters are frozen: requires_grad_(False) their weight and bias (attach_lora does)")
+    state = next(a.state for a in adapters if a is not None)
+    if state.rows is None:
+        raise ValueError("LoRAState.set_rows says which rows of the pass belong to which adapter: call it before the model")
+    x = x if x.is_contiguous() else x.contiguous()
+    factors = [f for a in adapters if a is not None for f in (a.a, a.b)]
+    return _LoRALinearFn.apply(x, state.rows, state.scales, [a is not None for a in adapters], [lin.weight.detach() for lin in linears],
+                               [None if lin.bias is None else lin.bias.detach() for lin in linears], *factors)
+
+
+TARGETS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+
+def attach_lora(model: nn.Module, n_adapters: int, rank: int, alpha: float | Sequence[float], targets: Sequence[str] = TARGETS) -> LoRAState:
+    """Hangs adapters on every projection of the attention and dense MLP seams that `targets` names, freezes all other parameters, and returns the state whose
+    `set_rows` describes each pass."""
+    from .attn import HipVarlenAttention
+    from .mlp import MLP
+
+    unknown = set(targets) - set(TARGETS)
+    if unknown:
+        raise ValueError(f"targets: expected names among {TARGETS}, got {sorted(unknown)}")
+    device = next(model.parameters()).device
+    state = LoRAState(n_adapters, rank, alpha, device)
+    linears = [lin for m in model.modules() if isinstance(m, (HipVarlenAttention, MLP)) for name, lin in m.named_children() if name in targets]
+    if not linears:
+        raise ValueError(f"the model has none of the projections {tuple(targets)}")
+    for p in model.parameters():
+        p.requires_grad_(False)
+    for lin in linears:
+        lin.lora = LoRAAdapters(lin, state)
+    return state
+
+
+def adapter_parameters(model: nn.Module) -> list[nn.Parameter]:
+    """All adapters' factors, in the model's order; run g's share of a factor p (and of its gradient) is p[g]."""
+    return [p for m in model.modules() if isinstance(m, LoRAAdapters) for p in (m.a, m.b)]
+
+
+@torch.no_grad()
+def merged_state_dict(model: nn.Module, adapter: int) -> dict[str, Tensor]:
+    """The model's state dict as a model without adapters has it, with one run's adapter folded into the projections (`ops.lora_merge`): what the weight push
+    sends to that run's inference engine."""
+    sd = {k: v.detach() for k, v in model.state_dict().items() if ".lora." not in k}
+    for name, m in model.named_modules():
+        lora = getattr(m, "lora", None)
+        if isinstance(lora, LoRAAdapters):
+            scale = float(lora.state.scales[adapter])
+            sd[f"{name}.weight"] = ops.lora_merge(m.weight.detach(), lora.a[adapter].to(torch.bfloat16), lora.b[adapter].to(torch.bfloat16), scale)
+    return sd

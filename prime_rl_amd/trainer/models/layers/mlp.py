@@ -12,6 +12,7 @@ from torch import nn
 
 from .... import ops
 from .linear import fused_linear, linear, swiglu_mlp
+from .lora import adapters_of, lora_linear
 
 
 @dataclass
@@ -53,6 +54,12 @@ class MLP(nn.Module):
     def forward(self, x, routed_experts: torch.Tensor | None = None):
         shape = x.shape
         x2 = x.reshape(-1, shape[-1])
+        inner, outer = adapters_of([self.gate_proj, self.up_proj]), adapters_of([self.down_proj])
+        if inner is not None or outer is not None:
+            gate_up = lora_linear(x2, [self.gate_proj, self.up_proj], inner) if inner is not None else fused_linear(x2, [self.gate_proj.weight, self.up_proj.weight])
+            act = swiglu(gate_up)
+            y = lora_linear(act, [self.down_proj], outer) if outer is not None else linear(act, self.down_proj.weight)
+            return y.view(*shape[:-1], self.hidden_size)
         # one node on the hand-written core (gate|up product + SwiGLU epilogue, down product; SwiGLU backward in the down row gradient's epilogue) when
         # gate_proj / up_proj lie back to back (a trainer engine's flat buffer); else the three projections on the core and the SwiGLU kernel
         y = swiglu_mlp(x2.contiguous(), self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight) if x2.is_cuda else None
