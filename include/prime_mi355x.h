@@ -580,7 +580,7 @@ int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t 
 int pm_lora_fwd(const void* x_bf16, int64_t ldx, const void* a_bf16, const void* b_bf16, const float* scales, const int32_t* offsets, const int32_t* row_ids /* nullable */,
                 int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base_bf16 /* nullable */, int64_t ldbase, void* out_bf16, int64_t ldout,
                 float* z, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank);
+int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, int32_t factors /* 1: grad_a and grad_b are wanted */);
 int pm_lora_bwd(const void* grad_out_bf16, int64_t ldg, const void* x_bf16, int64_t ldx, const float* z, const void* a_bf16, const void* b_bf16, const float* scales,
                 const int32_t* offsets, const int32_t* row_ids /* nullable */, int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank,
                 const void* base_bf16 /* nullable */, int64_t ldbase, void* grad_x_bf16 /* nullable */, int64_t ldgx, float* grad_a /* nullable */, float* grad_b /* nullable */,

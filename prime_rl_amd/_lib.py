@@ -162,7 +162,7 @@ SIGNATURES: dict[str, tuple] = {
     "pm_lora_z_columns": (I64, [I32]),
     "pm_lora_fwd_workspace_bytes": (I64, [I64, I32, I64, I32]),
     "pm_lora_fwd": (I, [P, I64, P, P, P, P, P, I64, I32, I64, I64, I32, P, I64, P, I64, P, P, I64, P]),
-    "pm_lora_bwd_workspace_bytes": (I64, [I64, I32, I64, I64, I32]),
+    "pm_lora_bwd_workspace_bytes": (I64, [I64, I32, I64, I64, I32, I32]),
     "pm_lora_bwd": (I, [P, I64, P, I64, P, P, P, P, P, P, I64, I32, I64, I64, I32, P, I64, P, I64, P, P, I32, P, I64, P]),
     "pm_lora_merge": (I, [P, I64, P, P, F, I64, I64, I32, P, I64, P]),
     "pm_grad_clip": (I, [P, I64, P, I32, P, I64, P, F, P, P, P, P, P, P]),

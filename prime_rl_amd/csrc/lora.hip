@@ -106,6 +106,21 @@ __device__ __forceinline__ void rows_of(const int32_t* __restrict__ row_ids, con
   }
 }
 
+constexpr int kMostParts = 8;
+// z of 4 ranks: the sum of the long axis' parts, four of them in flight
+__device__ __forceinline__ f32x4 sum_parts(const float* __restrict__ at, int64_t stride, int parts) {
+  f32x4 sum = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll 1
+  for (int q = 1; q < parts; q += 4) {
+    f32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4*>(at + min(q + i, parts - 1) * stride);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += q + i < parts ? v[i] : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  return sum;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // shrink: z[part][p][r] = scale * sum over the part's columns of t[row(p)][k] * w[adapter][r][k].
 // Chunks of columns of a tile's rows and of the factor come into LDS by DMA (global_load_lds: no registers, and one instruction takes whole stretches of a
@@ -348,6 +363,22 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
       stage[i] = r < rank && c < d ? *reinterpret_cast<const u32x4*>(w + ((int64_t)adapter * rank + r) * d + c) : u32x4{0, 0, 0, 0};
     }
   }
+  // base: move m of half h covers positions 32 h + (m * 4 + wave) * 64 / kLanes + lane / kLanes
+  const int mrow = lane / S::kLanes, mcol = lane % S::kLanes * 8, c = c0 + mcol;
+  int pos[2 * S::kMoves], row[2 * S::kMoves];
+#pragma unroll
+  for (int i = 0; i < 2 * S::kMoves; ++i) {
+    const int p = p0 + i / S::kMoves * 32 + (i % S::kMoves * 4 + wave) * (64 / S::kLanes) + mrow;
+    pos[i] = p < p1 ? p : p0;
+  }
+  u32x4 bv[2 * S::kMoves];
+  auto load_base = [&]() {
+    rows_of(row_ids, pos, n, row);
+#pragma unroll
+    for (int i = 0; i < 2 * S::kMoves; ++i)
+      bv[i] = base && c < d && (i < S::kMoves || p1 - p0 > 32) ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+  };
+  if (parts > 1) load_base();  // adding z's parts up waits for them: the base is asked for first
   // z, split into its two bf16 terms on the way to LDS
   constexpr int kZb = (RT * 2 + 3) / 4;
   f32x4 zv[MERGE ? 1 : RT];  // thread -> 4 ranks of one position, RT times
@@ -364,23 +395,12 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
       const int piece = i * 256 + tid, p = p0 + piece / (RT * 4), r = piece % (RT * 4) * 4;
       zv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (p < p1 && r < rp) {
-        for (int part = 0; part < parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(z + ((int64_t)part * n + p) * rp + r);
+        zv[i] = sum_parts(z + (int64_t)p * rp + r, (int64_t)n * rp, parts);
         if (z_out && col_tile == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)p * rp + r) = zv[i];
       }
     }
   }
-  // base: move m of half h covers positions 32 h + (m * 4 + wave) * 64 / kLanes + lane / kLanes
-  const int mrow = lane / S::kLanes, mcol = lane % S::kLanes * 8, c = c0 + mcol;
-  int pos[2 * S::kMoves], row[2 * S::kMoves];
-#pragma unroll
-  for (int i = 0; i < 2 * S::kMoves; ++i) {
-    const int p = p0 + i / S::kMoves * 32 + (i % S::kMoves * 4 + wave) * (64 / S::kLanes) + mrow;
-    pos[i] = p < p1 ? p : p0;
-  }
-  rows_of(row_ids, pos, n, row);
-  u32x4 bv[2 * S::kMoves];
-#pragma unroll
-  for (int i = 0; i < 2 * S::kMoves; ++i) bv[i] = base && c < d && (i < S::kMoves || p1 - p0 > 32) ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+  if (parts <= 1) load_base();
   auto store = [&](int i, const u32x4& v) {
     const int p = p0 + i / S::kMoves * 32 + (i % S::kMoves * 4 + wave) * (64 / S::kLanes) + mrow;
     if (c < d && p < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[i] * ldo + c) = v;
@@ -492,6 +512,8 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 // The positions are the contraction, so both operands are read transposed (ds_read_b64_tr_b16).  Stages of 32 positions go through LDS: t by DMA, a ring of three deep
 // (16-byte slot pairs permuted by the row's number, so that the 8 rows of half a transposed read lie in different banks), z through registers, where it is split into
 // three bf16 planes.  A wave takes 64 columns and all ranks.
+// DZ (rank <= 16, many rows): the same pass over dy also gives dz, so that dy is read once: the tile's 512 columns are contracted with the factor's (from registers), the
+// waves' results are added up through LDS while the next stage runs, and dz comes in one part for each column tile (6 % of the bytes of dy, written and read once).
 struct OuterSide {
   const float* z;      // [parts][n][rp]
   int parts;
@@ -499,6 +521,10 @@ struct OuterSide {
   int64_t ldt;
   int d;
   float* part;         // [ranges + adapters][rank][d]
+  int range;           // positions of a workgroup
+  const bf16_t* w;     // DZ: the factor and scales of dz
+  const float* scales;
+  float* dz;           // DZ: [column tiles][n][16]
 };
 constexpr int kOuterStage = 32, kOuterRing = 3, kOuterIds = 1024;  // kOuterIds: row ids held in LDS at a time
 
@@ -516,9 +542,10 @@ __device__ __forceinline__ void tr_read_tile(const uint32_t (&a)[4], u32x2 (&v)[
       : "memory");
 }
 
-template <int RT>
+template <int RT, bool DZ>
 __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
-                                                    int n_adapters, int rank, int rp, int range) {
+                                                    int n_adapters, int rank, int rp) {
+  static_assert(!DZ || RT == 1, "dz beside dB: one 16-row block of ranks");
   constexpr int SP = kOuterStage, kRowBytes = kOuterCols * 2, kBuf = SP * kRowBytes;
   constexpr int kZs = RT == 1 ? 32 : RT * 32 + 32;  // 32 bytes of shift per row keep transposed reads off each other's banks
   constexpr int kZp = (SP * RT * 4 + 511) / 512;    // 4-rank pieces of z per thread and stage
@@ -526,12 +553,13 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
   __shared__ __attribute__((aligned(1024))) unsigned char lt[kOuterRing * kBuf];
   __shared__ __attribute__((aligned(16))) unsigned char lz[2][3][SP * kZs];
   __shared__ int li[kOuterIds];
+  __shared__ __attribute__((aligned(16))) float lp[DZ ? 2 : 1][DZ ? 8 * SP * 16 : 4];  // dz of a stage, from each wave
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
   const int split = blockIdx.x / tiles01, col_tile = blockIdx.x % tiles01;
   const bool second = col_tile >= tiles0;
   const OuterSide s = second ? s1 : s0;
   const int c0 = (second ? col_tile - tiles0 : col_tile) * kOuterCols;
-  const int begin = split * range, end = min(begin + range, n);
+  const int begin = split * s.range, end = min(begin + s.range, n);
   // the first adapter whose positions reach past `begin`
   int g = n_adapters;
   for (int e0 = 0; e0 < n_adapters; e0 += 64) {
@@ -556,6 +584,15 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 wf[2];
+    float scale = 0.f;
+    const int wcol = c0 + wave * 64 + lq * 8;
+    if constexpr (DZ) {
+      scale = s.scales[g];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        wf[k] = lr < rank && wcol + k * 32 < s.d ? *reinterpret_cast<const u32x4*>(s.w + ((int64_t)g * rank + lr) * s.d + wcol + k * 32) : u32x4{0, 0, 0, 0};
+    }
     for (int first = lo, last; first < hi; first = last) {
       last = row_ids ? min(first + kOuterIds, hi) : hi;
       const int stages = (last - first + SP - 1) / SP, full = (last - first) / SP;
@@ -584,8 +621,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         for (int i = 0; i < kZp; ++i) {
           const int piece = (i * 512 + tid) % (SP * RT * 4), p = min(first + st * SP + piece / (RT * 4), last - 1), r = min(piece % (RT * 4) * 4, rp - 4);
           const float* at = s.z + (int64_t)p * rp + r;
-          zv[i] = *reinterpret_cast<const f32x4*>(at);
-          for (int part = 1; part < parts; ++part) zv[i] += *reinterpret_cast<const f32x4*>(at + (int64_t)part * n * rp);
+          zv[i] = sum_parts(at, (int64_t)n * rp, parts);
         }
       };
       auto split_z = [&](int st, f32x4 (&zv)[kZp]) {
@@ -616,6 +652,27 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
             for (int i = 0; i < 4; ++i) acc[i][j] = mfma(u32x4{tv[2 * i].x, tv[2 * i].y, tv[2 * i + 1].x, tv[2 * i + 1].y}, zf, acc[i][j]);
           }
       };
+      // this wave's 64 columns of dz, 32 positions x 16 ranks; and a value of the last stage's dz from all waves for each thread
+      auto contract = [&](int st) {
+        const unsigned char* at = lt + st % kOuterRing * kBuf;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(at + (i * 16 + lr) * kRowBytes + (((wave * 8 + k * 4 + lq) ^ ((lr & 7) << 1)) << 4));
+            sum = mfma(wf[k], wcol + k * 32 < s.d ? v : u32x4{0, 0, 0, 0}, sum);
+          }
+          *reinterpret_cast<f32x4*>(&lp[st & 1][(wave * SP + i * 16 + lr) * 16 + lq * 4]) = sum;
+        }
+      };
+      auto store_dz = [&](int st, bool whole) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += lp[st & 1][w * SP * 16 + tid];
+        const int p = first + st * SP + (tid >> 4);
+        if (whole || p < last) s.dz[((int64_t)col_tile * n + p) * 16 + (tid & 15)] = (tid & 15) < rank ? sum * scale : 0.f;
+      };
       // stage st: t comes two stages ahead, z three (it is split one stage ahead)
       f32x4 za[kZp], zb[kZp];
       fetch(0, full > 0);
@@ -627,19 +684,24 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
       int st = 0;
       auto stage = [&](auto steady, f32x4 (&next)[kZp]) {  // `next` holds z of stage st + 1, and gets that of st + 3
         if constexpr (decltype(steady)::value) {
-          wait_dma(kDma + kZp);  // younger than t of this stage: t of the next, and z of the one after it
+          wait_dma(kDma + kZp + (DZ ? 1 : 0));  // younger than t of this stage: t of the next, z of the one after it, a store of dz
           lds_barrier();
+          if constexpr (DZ)
+            if (st > 0) store_dz(st - 1, true);
           split_z(st + 1, next);
           fetch(st + 2, true);
           load_z(st + 3, next, 1);
         } else {
           wait_dma(0);
           lds_barrier();
+          if constexpr (DZ)
+            if (st > 0) store_dz(st - 1, false);
           if (st + 1 < stages) split_z(st + 1, next);
           if (st + 2 < stages) fetch(st + 2, st + 2 < full);
           if (st + 3 < stages) load_z(st + 3, next, s.parts);
         }
         multiply(st);
+        if constexpr (DZ) contract(st);
         ++st;
       };
       if (s.parts == 1)
@@ -650,6 +712,10 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
       while (st < stages) {
         stage(std::false_type{}, zb);
         if (st < stages) stage(std::false_type{}, za);
+      }
+      if constexpr (DZ) {
+        lds_barrier();
+        store_dz(stages - 1, false);
       }
     }
     float* part = s.part + (int64_t)(split + g) * rank * s.d;
@@ -667,20 +733,44 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
   }
 }
 
+// dz of 4 ranks: the column tiles' parts, added in their order
+__global__ __launch_bounds__(256) void sum_dz_kernel(const float* __restrict__ parts, int count, int64_t elems, float* __restrict__ dz) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= elems) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < count; c += 8) {
+    f32x4 p[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) p[q] = c + q < count ? *reinterpret_cast<const f32x4*>(parts + (c + q) * elems + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += p[q];
+  }
+  *reinterpret_cast<f32x4*>(dz + at) = v;
+}
+
 // grad[adapter][r][c] (+)= the adapter's partials, added in the order of its positions; zero for an adapter without rows.
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part0, float* __restrict__ grad0, int64_t elems0, const float* __restrict__ part1,
-                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int range, int accumulate) {
+                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int range0, int range1, int accumulate) {
   const int g = blockIdx.y;
   const int lo = min(max(offsets[g], 0), n), hi = min(max(offsets[g + 1], lo), n);
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= elems0 + elems1) return;
   const bool second = at >= elems0;
   const int64_t e = second ? at - elems0 : at, elems = second ? elems1 : elems0;
+  const int range = second ? range1 : range0;
   const float* part = (second ? part1 : part0) + e;
   float* grad = (second ? grad1 : grad0) + (int64_t)g * elems + e;
   f32x4 v = accumulate ? *reinterpret_cast<const f32x4*>(grad) : f32x4{0.f, 0.f, 0.f, 0.f};
-  if (lo < hi)
-    for (int split = lo / range; split <= (hi - 1) / range; ++split) v += *reinterpret_cast<const f32x4*>(part + (int64_t)(split + g) * elems);
+  if (lo < hi) {
+    const int last = (hi - 1) / range;
+    for (int split = lo / range; split <= last; split += 8) {  // eight at a time in flight
+      f32x4 p[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) p[q] = split + q <= last ? *reinterpret_cast<const f32x4*>(part + (int64_t)(split + q + g) * elems) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += p[q];
+    }
+  }
   *reinterpret_cast<f32x4*>(grad) = v;
 }
 
@@ -699,7 +789,7 @@ struct ShrinkPlan {
 static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank) {
   ShrinkPlan p;
   const bool narrow = rank <= 16;
-  const int factor = rank_tiles(rank) * 16, chunks = (int)cdiv(d, narrow ? kNarrowChunk : kWideChunk), most = chunks / 2 < 8 ? (chunks / 2 > 1 ? chunks / 2 : 1) : 8;
+  const int factor = rank_tiles(rank) * 16, chunks = (int)cdiv(d, narrow ? kNarrowChunk : kWideChunk), most = chunks / 2 < kMostParts ? (chunks / 2 > 1 ? chunks / 2 : 1) : kMostParts;
   auto parts_of = [&](int64_t tiles, int at_once) { return tiles * most <= at_once ? most : tiles < at_once ? (int)(at_once / tiles) : 1; };
   if (narrow) {
     p.rows = kNarrowRows, p.depth = kRing, p.tiles = max_tiles(n, n_adapters, p.rows);
@@ -833,27 +923,36 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
 }
 
 namespace {
+// dz beside dB in one pass over grad_out pays from about 64 Mi elements of it, where the caches no longer hold it for the second pass (rank 16, all of the backward, two passes
+// against one: 16 384 rows 4096 -> 4096 155 and 149 us, -> 12288 259 and 215, 32 768 rows 449 and 371; 8192 rows 4096 -> 4096 92 and 97).
+constexpr int64_t kFusedElements = (int64_t)64 << 20;
 struct BwdPlan {
+  bool fused;
   ShrinkPlan shrink;
-  int range;
-  int64_t slots, dz_bytes, part0_bytes, part1_bytes;
+  int tiles0, tiles1, range0, range1;
+  int64_t dz_bytes, dz_parts_bytes, part0_bytes, part1_bytes;
 };
-BwdPlan bwd_plan(int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int rank) {
+BwdPlan bwd_plan(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int rank, bool factors) {
   BwdPlan p;
-  p.shrink = shrink_plan(n, (int)n_adapters, (int)d_out, rank);
-  p.range = outer_range(n, (int)n_adapters, (int)(cdiv(d_in, kOuterCols) + cdiv(d_out, kOuterCols)), rank);
-  p.slots = cdiv(n, p.range) + n_adapters;
-  p.dz_bytes = (int64_t)p.shrink.parts * n * padded_rank(rank) * 4;
-  p.part0_bytes = p.slots * rank * d_out * 4;
-  p.part1_bytes = p.slots * rank * d_in * 4;
+  const int rp = padded_rank(rank);
+  p.tiles0 = (int)cdiv(d_out, kOuterCols), p.tiles1 = (int)cdiv(d_in, kOuterCols);
+  p.fused = factors && rank <= 16 && n * d_out >= kFusedElements;
+  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
+  if (p.fused) p.shrink.parts = 1;
+  p.range0 = outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
+  p.range1 = p.fused ? outer_range(n, n_adapters, p.tiles1, rank) : p.range0;
+  p.dz_bytes = (int64_t)p.shrink.parts * n * rp * 4;
+  p.dz_parts_bytes = p.fused ? (int64_t)p.tiles0 * n * rp * 4 : 0;
+  p.part0_bytes = factors ? (cdiv(n, p.range0) + n_adapters) * rank * d_out * 4 : 0;
+  p.part1_bytes = factors ? (cdiv(n, p.range1) + n_adapters) * rank * d_in * 4 : 0;
   return p;
 }
 }  // namespace
 
-extern "C" int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank) {
+extern "C" int64_t pm_lora_bwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, int32_t factors) {
   if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
-  const BwdPlan p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank);
-  return p.dz_bytes + p.part0_bytes + p.part1_bytes;
+  const BwdPlan p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank, factors != 0);
+  return p.dz_bytes + p.dz_parts_bytes + p.part0_bytes + p.part1_bytes;
 }
 
 extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, const float* z, const void* a, const void* b, const float* scales, const int32_t* offsets,
@@ -865,8 +964,10 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
              "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
   PM_REQUIRE(offsets, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
   hipStream_t st = as_stream(stream);
-  BwdPlan p{{}, 1, 0, 0, 0, 0};
   unsigned char* ws = (unsigned char*)workspace;
+  BwdPlan p{};
+  p.range0 = p.range1 = 1;
+  float *dz = (float*)ws, *dz_parts = nullptr, *part0 = nullptr, *part1 = nullptr;
   if (n_rows > 0) {
     PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
     PM_TRY(check_rows("pm_lora_bwd", "grad_out", grad_out, ldg, d_out));
@@ -877,30 +978,40 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
       PM_REQUIRE(z, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer (z)");
       PM_TRY(check_rows("pm_lora_bwd", "x", x, ldx, d_in));
     }
-    p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank);
-    const int64_t need = p.dz_bytes + p.part0_bytes + p.part1_bytes;
+    p = bwd_plan(n_rows, n_adapters, d_in, d_out, rank, grad_a != nullptr);
+    const int64_t need = p.dz_bytes + p.dz_parts_bytes + p.part0_bytes + p.part1_bytes;
     PM_REQUIRE(ws && workspace_bytes >= need && ((uintptr_t)ws & 15) == 0, PM_ERR_WORKSPACE, "pm_lora_bwd: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                (long long)need);
-    float* dz = (float*)ws;
-    PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
-    PM_CHECK_LAUNCH("pm_lora_bwd");
+    dz_parts = (float*)(ws + p.dz_bytes);
+    part0 = (float*)(ws + p.dz_bytes + p.dz_parts_bytes);
+    part1 = (float*)(ws + p.dz_bytes + p.dz_parts_bytes + p.part0_bytes);
+    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
+    const OuterSide s1{dz, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
+    const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
+    if (p.fused) {
+      hipLaunchKernelGGL((outer_kernel<1, true>), dim3(splits0 * p.tiles0), dim3(512), 0, st, s0, s0, p.tiles0, p.tiles0, offsets, row_ids, (int)n_rows, n_adapters, rank, 16);
+      PM_CHECK_LAUNCH("pm_lora_bwd");
+      hipLaunchKernelGGL(sum_dz_kernel, dim3((unsigned)cdiv(n_rows * 4, 256)), dim3(256), 0, st, dz_parts, p.tiles0, n_rows * 16, dz);
+      PM_CHECK_LAUNCH("pm_lora_bwd");
+      hipLaunchKernelGGL((outer_kernel<1, false>), dim3(splits1 * p.tiles1), dim3(512), 0, st, s1, s1, p.tiles1, p.tiles1, offsets, row_ids, (int)n_rows, n_adapters, rank, 16);
+      PM_CHECK_LAUNCH("pm_lora_bwd");
+    } else {
+      PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
+      PM_CHECK_LAUNCH("pm_lora_bwd");
+      if (grad_a) {
+        PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT, false>), dim3(splits0 * (p.tiles0 + p.tiles1)), dim3(512), 0, st, s0, s1, p.tiles0, p.tiles0 + p.tiles1, offsets, row_ids,
+                                            (int)n_rows, n_adapters, rank, padded_rank(rank)));
+        PM_CHECK_LAUNCH("pm_lora_bwd");
+      }
+    }
   }
   if (grad_a) {
-    float *part0 = (float*)(ws + p.dz_bytes), *part1 = (float*)(ws + p.dz_bytes + p.part0_bytes);
-    if (n_rows > 0) {
-      const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0}, s1{(const float*)ws, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1};
-      const int t0 = (int)cdiv(d_out, kOuterCols), t1 = (int)cdiv(d_in, kOuterCols);
-      PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT>), dim3((unsigned)(cdiv(n_rows, p.range) * (t0 + t1))), dim3(512), 0, st, s0, s1, t0, t0 + t1, offsets, row_ids,
-                                          (int)n_rows, n_adapters, rank, padded_rank(rank), p.range));
-      PM_CHECK_LAUNCH("pm_lora_bwd");
-    }
     const int64_t e0 = rank * d_out, e1 = rank * d_in;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, p.range,
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, p.range0, p.range1,
                        accumulate);
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
   if (n_rows > 0 && grad_x) {
-    float* dz = (float*)ws;
     PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }

@@ -1212,7 +1212,7 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
                 raise PrimeMI355XError("grad_x overlaps base: it may be base itself or memory of its own")
     else:
         base = grad_x = None
-    nbytes = lib.pm_lora_bwd_workspace_bytes(rows, n, d_in, d_out, rank)
+    nbytes = lib.pm_lora_bwd_workspace_bytes(rows, n, d_in, d_out, rank, 1 if want_factors else 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=grad_out.device) if nbytes else None
     _launch(lib.pm_lora_bwd, "pm_lora_bwd", (grad_out, x, z, a, b, scales, offsets, row_ids, base, grad_x, grad_a, grad_b), _p(grad_out), ldg, _p(x), ldx, _p(z), _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb,
             _p(grad_x), ldgx, _p(grad_a), _p(grad_b), 1 if accumulate else 0, _p(ws), nbytes)

@@ -99,6 +99,10 @@ CASES = [  # rows of each adapter, d_in, d_out, rank, rows of none, in any order
     ([3, 0, 1, 2] * 20, 128, 64, 12, 4, True),  # more adapters than lanes of a wave
     ([9000, 7421, 0, 600], 192, 128, 16, 11, False),
     ([4100, 4097], 256, 512, 64, 1, True),
+    # enough of grad_out that dz comes with dB in one pass
+    ([9000, 0, 7421, 600], 264, 4104, 16, 11, False),
+    ([8000, 33, 9000], 128, 4096, 12, 40, True),
+    ([17000], 520, 4008, 1, 0, False),
 ]
 
 
@@ -204,6 +208,29 @@ def test_lora_other_rows_and_adapters_do_not_leak(ops):
     one["x"][2, 5] = float("inf")
     out, z = ops.lora_fwd(one["x"], one["a"], one["b"], one["scales"], one["offsets"])
     assert torch.isinf(z[2, 0]) and torch.isinf(out[2]).all() and torch.isfinite(out[[0, 1, 3]]).all()
+
+
+def test_lora_bwd_in_one_pass_keeps_infinities_in_their_rows(ops):
+    c = _case([9000, 7000, 500], 128, 4104, 11, without=50, mixed=True)
+    args = (c["a"], c["b"], c["scales"], c["offsets"])
+    _, z = ops.lora_fwd(c["x"], *args, base=c["base"], row_ids=c["row_ids"])
+    clean = ops.lora_bwd(c["dy"], c["x"], z, *args, base=c["bx"], row_ids=c["row_ids"])
+    rows = c["row_ids"].long()
+    dy = c["dy"].clone()
+    dy[rows[9000:9040]] = float("inf")
+    dy[rows[9050:9060], 0] = float("nan")
+    dy[rows[16500:]] = float("nan")
+    got = ops.lora_bwd(dy, c["x"], z, *args, base=c["bx"], row_ids=c["row_ids"])
+    keep = torch.cat([rows[:9000], rows[9040:9050], rows[9060:]])
+    assert torch.equal(got[0][keep], clean[0][keep])
+    for k in (1, 2):
+        assert torch.equal(got[k][0], clean[k][0]) and torch.equal(got[k][2], clean[k][2]) and not torch.isfinite(got[k][1]).all()
+    dy = c["dy"].clone()
+    dy[rows[20], 5] = float("inf")  # an infinite gradient of one column: every column of grad_x that the adapter reaches is infinite, not NaN, where the rank is one
+    r1 = (c["a"][:, :1].contiguous(), c["b"][:, :1].contiguous(), c["scales"], c["offsets"])
+    _, z1 = ops.lora_fwd(c["x"], *r1, base=c["base"], row_ids=c["row_ids"])
+    one = ops.lora_bwd(dy, c["x"], z1, *r1, row_ids=c["row_ids"])[0]
+    assert torch.isinf(one[rows[20]]).all() and torch.isfinite(one[rows[21]]).all()
 
 
 def test_lora_padding_ranks_with_zero_rows_changes_nothing(ops):
