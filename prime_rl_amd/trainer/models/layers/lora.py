@@ -57,6 +57,7 @@ class LoRAState:
         self.rows: LoRARows | None = None
 
     def set_rows(self, rows: LoRARows) -> None:
+        """The rows of the passes that follow, until the next call; where layers are recomputed in the backward, the next call comes after it."""
         if rows.offsets.numel() != self.n_adapters + 1:
             raise ValueError(f"rows of {rows.offsets.numel() - 1} adapters for a model of {self.n_adapters}")
         self.rows = rows
@@ -107,21 +108,24 @@ class _LoRALinearFn(torch.autograd.Function):
             if has_adapter[i]:
                 zs.append(ops.lora_fwd(x, halves[at], halves[at + 1], scales, rows.offsets, base=part, row_ids=rows.row_ids, out=part)[1])
                 at += 2
-        ctx.save_for_backward(x, scales, *halves, *zs)
-        ctx.rows, ctx.has_adapter, ctx.weights, ctx.joined, ctx.widths = rows, has_adapter, weights, joined, widths
+        # the rows' tables and the weights too: changed in place before the backward, they raise there
+        ctx.save_for_backward(x, scales, rows.offsets, rows.row_ids, *weights, *halves, *zs)
+        ctx.has_adapter, ctx.widths = has_adapter, widths
         ctx.dtypes = [f.dtype for f in factors]
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, scales, *rest = ctx.saved_tensors
-        n_factors = len(ctx.dtypes)
-        halves, zs = rest[:n_factors], rest[n_factors:]
-        dy = dy if dy.stride(1) == 1 and dy.stride(0) % 8 == 0 and dy.data_ptr() % 16 == 0 else dy.contiguous()
+        x, scales, offsets, row_ids, *rest = ctx.saved_tensors
+        n_factors, n_weights = len(ctx.dtypes), len(ctx.widths)
+        weights, halves, zs = rest[:n_weights], rest[n_weights:n_weights + n_factors], rest[n_weights + n_factors:]
+        joined = _adjacent_view(weights)
+        # rows that overlap (a gradient that is one row for all, say) are written out
+        dy = dy if dy.stride(1) == 1 and dy.stride(0) >= dy.shape[1] and dy.stride(0) % 8 == 0 and dy.data_ptr() % 16 == 0 else dy.contiguous()
         want_x, want_factors = ctx.needs_input_grad[0], any(ctx.needs_input_grad[6:])
         dx, parts = None, dy.split(ctx.widths, dim=1)
         if want_x:
-            pairs = [(dy, ctx.joined)] if ctx.joined is not None else list(zip(parts, ctx.weights))
+            pairs = [(dy, joined)] if joined is not None else list(zip(parts, weights))
             for d, w in pairs:
                 step = ops.gemm(d, w.t()) if ops.gemm_supported(d, w.t()) else d @ w
                 dx = step if dx is None else dx.add_(step)
@@ -130,7 +134,7 @@ class _LoRALinearFn(torch.autograd.Function):
             if not ctx.has_adapter[i]:
                 continue
             k = len(grads)
-            _, da, db = ops.lora_bwd(d, x, zs[k // 2], halves[k], halves[k + 1], scales, ctx.rows.offsets, base=dx, row_ids=ctx.rows.row_ids, grad_x=dx, want_x=want_x,
+            _, da, db = ops.lora_bwd(d, x, zs[k // 2], halves[k], halves[k + 1], scales, offsets, base=dx, row_ids=row_ids, grad_x=dx, want_x=want_x,
                                      want_factors=want_factors)
             grads += [da, db]
         if not want_factors:
@@ -140,15 +144,20 @@ class _LoRALinearFn(torch.autograd.Function):
 
 def lora_linear(x: Tensor, linears: Sequence[nn.Linear], adapters: Sequence[LoRAAdapters | None] | None = None) -> Tensor:
     """cat([linear_i(x)], dim=-1) with the projections' adapters for x [N, in] bf16 rows of the pass that `LoRAState.set_rows` described.  The shared weights are
-    frozen: gradients go to x and the adapters."""
+    frozen: gradients go to x and the adapters.  In a captured graph only without gradients: accumulating into leaves that an earlier eager pass holds too would wait for that
+    pass' stream, which ends the process (a captured training step calls `ops.lora_fwd` and `ops.lora_bwd` on buffers of its own)."""
     adapters = adapters if adapters is not None else adapters_of(linears)
     if adapters is None:
         raise ValueError("none of the projections has adapters")
     if any(p is not None and p.requires_grad for lin in linears for p in (lin.weight, lin.bias)):
         raise ValueError("the projections beside adapters are frozen: requires_grad_(False) their weight and bias (attach_lora does)")
     state = next(a.state for a in adapters if a is not None)
+    if any(a is not None and a.state is not state for a in adapters):
+        raise ValueError("the projections' adapters belong to different states")
     if state.rows is None:
         raise ValueError("LoRAState.set_rows says which rows of the pass belong to which adapter: call it before the model")
+    if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise ValueError("a captured pass through adapters runs under torch.no_grad()")
     x = x if x.is_contiguous() else x.contiguous()
     factors = [f for a in adapters if a is not None for f in (a.a, a.b)]
     return _LoRALinearFn.apply(x, state.rows, state.scales, [a is not None for a in adapters], [lin.weight.detach() for lin in linears],
@@ -160,13 +169,15 @@ TARGETS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down
 
 def attach_lora(model: nn.Module, n_adapters: int, rank: int, alpha: float | Sequence[float], targets: Sequence[str] = TARGETS) -> LoRAState:
     """Hangs adapters on every projection of the attention and dense MLP seams that `targets` names, freezes all other parameters, and returns the state whose
-    `set_rows` describes each pass."""
+    `set_rows` describes each pass.  A model has one set of adapters: it is attached once."""
     from .attn import HipVarlenAttention
     from .mlp import MLP
 
     unknown = set(targets) - set(TARGETS)
     if unknown:
         raise ValueError(f"targets: expected names among {TARGETS}, got {sorted(unknown)}")
+    if any(isinstance(m, LoRAAdapters) for m in model.modules()):
+        raise ValueError("the model has adapters already")
     device = next(model.parameters()).device
     state = LoRAState(n_adapters, rank, alpha, device)
     linears = [lin for m in model.modules() if isinstance(m, (HipVarlenAttention, MLP)) for name, lin in m.named_children() if name in targets]

@@ -85,6 +85,56 @@ def test_lora_linear_matches_the_formula_and_its_gradients(n, d_in, widths, has,
     assert ((x.grad.double() - dx).abs() <= dx_tol + roundings * E8 * (parts + dx_tol)).all()
 
 
+def _one_linear():
+    from prime_rl_amd.trainer.models.layers.lora import LoRAAdapters, LoRARows, LoRAState, lora_linear
+
+    state = LoRAState(2, 8, 16.0, DEV)
+    (lin,) = _linears((128,), 256, False, False, 3)
+    lin.lora = LoRAAdapters(lin, state)
+    lin.lora.b.data.normal_(0, 0.3)
+    state.set_rows(LoRARows.packed([40, 30], DEV))
+    x = torch.randn(72, 256, device=DEV).to(BF16).requires_grad_(True)
+    return lin, state, x, lambda: lora_linear(x, [lin])
+
+
+def test_a_gradient_that_is_one_row_for_all():
+    """The gradient of a sum over rows arrives with a row stride of zero: the same results as from rows of their own."""
+    lin, _, x, run = _one_linear()
+    v = torch.randn(128, device=DEV).to(BF16)
+    leaves = (x, lin.lora.a, lin.lora.b)
+    got = torch.autograd.grad(run(), leaves, v.expand(72, 128))
+    want = torch.autograd.grad(run(), leaves, v.expand(72, 128).contiguous())
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("what", ["offsets", "weight", "scales"])
+def test_a_backward_of_tables_or_weights_changed_since_raises(what):
+    lin, state, _, run = _one_linear()
+    y = run()
+    {"offsets": state.rows.offsets, "weight": lin.weight, "scales": state.scales}[what].mul_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_captured_passes_are_without_gradients():
+    """Replays follow what the buffers hold; a captured pass with gradients is refused."""
+    _, _, x, run = _one_linear()
+    with torch.no_grad():
+        run()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="no_grad"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        held = run()
+    for turn in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(72, 256, device=DEV))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, run()), turn
+
+
 def test_gradients_against_differences():
     """d(sum y * dy) / d factor against differences of the whole seam in the factor, in the directions of the gradients themselves."""
     from prime_rl_amd.trainer.models.layers.lora import LoRAAdapters, LoRARows, LoRAState, lora_linear
