@@ -566,8 +566,9 @@ int pm_gemm_debug_set_variant(int32_t value);
  * Rows are grouped by adapter: adapter g owns the POSITIONS [offsets[g], offsets[g+1]) (int32 [n_adapters + 1] on the device, offsets[0] = 0, not decreasing);
  * position p is row row_ids[p] of the row tensors (row_ids int32 [n_rows], each row at most once; NULL: position p is row p).  Positions behind the last offset belong to
  * no adapter: their rows of the result are the base's.  Both factors are rank-major: a [n_adapters, rank, d_in], b [n_adapters, rank, d_out] (bf16, contiguous), scales f32.
- * Row tensors are bf16 with their own row strides (elements, multiples of 8, rows 16-byte aligned).  d_in, d_out multiples of 8, rank 1 .. 128 (zero rows of both
- * factors give a smaller rank).  Offsets and row ids out of range are clamped: such a table gives wrong results, never an access out of range.  Deterministic.
+ * Row tensors are bf16 with their own row strides (elements, multiples of 8, rows 16-byte aligned).  n_rows up to 2^28, d_in, d_out multiples of 8 up to 2^22, rank 1 .. 128 (zero rows of
+ * both factors give a smaller rank).  Offsets and row ids out of range are clamped: such a table gives wrong results, never an access out of range.  Deterministic.  NaN and infinities stay
+ * in their rows (grad_x, out) and their adapter (grad_a, grad_b), where an infinity may come out as a NaN.
  *   fwd:   z[p] = scales[g] * x[row] . a[g]^T (f32, [n_rows, pm_lora_z_columns(rank)] in the order of the positions, the columns past the rank zero; rows of no adapter are
  *          not written); out[row] = bf16(base[row] + z[p] . b[g]).  out may be base (in place); base NULL = zeros.
  *   bwd:   dz[p] = scales[g] * grad_out[row] . b[g]^T; grad_x[row] = bf16(base[row] + dz[p] . a[g]) (grad_x NULL: not wanted; base as above);

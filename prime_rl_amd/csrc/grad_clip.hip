@@ -202,7 +202,8 @@ using namespace pm;
 
 extern "C" int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32_t* group_offsets, int32_t n_groups, const int64_t* pieces, int64_t n_pieces, const double* sumsq_in,
                             float max_norm, const float* max_norms, double* partials, double* sumsq_out, float* norms, float* coefs, void* stream) {
-  PM_REQUIRE(n_chunks >= 0 && n_chunks <= INT32_MAX && n_pieces >= 0 && n_pieces <= INT32_MAX && n_groups >= 1, PM_ERR_INVALID_ARG, "pm_grad_clip: %lld chunks, %lld pieces, %d groups",
+  constexpr int64_t kLaunch = (int64_t)1 << 23;  // workgroups of a launch, which holds less than 2^32 threads
+  PM_REQUIRE(n_chunks >= 0 && n_chunks < kLaunch && n_pieces >= 0 && n_pieces <= INT32_MAX && n_groups >= 1 && n_groups <= 1 << 20, PM_ERR_INVALID_ARG, "pm_grad_clip: %lld chunks, %lld pieces, %d groups",
              (long long)n_chunks, (long long)n_pieces, n_groups);
   PM_REQUIRE(group_offsets && (n_chunks == 0 || chunks) && (n_pieces == 0 || pieces) && (sumsq_in || n_chunks == 0 || partials), PM_ERR_INVALID_ARG, "pm_grad_clip: null pointer");
   PM_REQUIRE((norms != nullptr) == (coefs != nullptr) && (norms || (sumsq_out && n_pieces == 0)), PM_ERR_INVALID_ARG, "pm_grad_clip: norms and coefs go together, scaling needs them");
@@ -220,8 +221,9 @@ extern "C" int pm_grad_clip(const int64_t* chunks, int64_t n_chunks, const int32
   }
   hipLaunchKernelGGL(gclip::coef_kernel, dim3(n_groups), dim3(1024), 0, st, sumsq_in ? sumsq_in : partials, sumsq_in ? nullptr : group_offsets, max_norm, max_norms, sumsq_out, norms, coefs);
   PM_CHECK_LAUNCH("pm_grad_clip");
-  if (n_pieces > 0) {
-    hipLaunchKernelGGL(gclip::scale_kernel, dim3((unsigned)n_pieces), dim3(256), 0, st, scaled, coefs);
+  for (int64_t end = n_pieces; end > 0; end -= kLaunch) {
+    const int64_t count = end < kLaunch ? end : kLaunch;
+    hipLaunchKernelGGL(gclip::scale_kernel, dim3((unsigned)count), dim3(256), 0, st, scaled + (end - count), coefs);
     PM_CHECK_LAUNCH("pm_grad_clip");
   }
   return PM_OK;

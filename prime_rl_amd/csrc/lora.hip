@@ -29,6 +29,7 @@ typedef __attribute__((address_space(3))) void* lds_void_ptr;
 typedef __attribute__((address_space(1))) void* glb_void_ptr;
 
 constexpr int kMaxRank = 128;
+constexpr int64_t kMaxRows = (int64_t)1 << 28;
 constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
 constexpr int kOuterCols = 512;  // columns of an outer workgroup
 
@@ -849,6 +850,7 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
 template <int RT, bool MERGE>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
                           int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t stream) {
+  static_assert(ExpandShape<RT>::kCols == (RT <= 4 ? 256 : 128), "check_launch counts these");
   const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
   const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
   hipLaunchKernelGGL((expand_kernel<RT, MERGE>), dim3(grid), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
@@ -863,11 +865,18 @@ static void launch_expand(const float* z, int parts, float* z_out, const void* z
   }
 
 static int check_shape(const char* who, int64_t n, int64_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank) {
-  PM_REQUIRE(n >= 0 && n <= INT32_MAX - 4096, PM_ERR_INVALID_ARG, "%s: n_rows %lld", who, (long long)n);
+  PM_REQUIRE(n >= 0 && n <= kMaxRows, PM_ERR_INVALID_ARG, "%s: n_rows %lld (at most %lld)", who, (long long)n, (long long)kMaxRows);
   PM_REQUIRE(n_adapters >= 1 && n_adapters <= 65535, PM_ERR_INVALID_ARG, "%s: n_adapters %lld (1 .. 65535)", who, (long long)n_adapters);
   PM_REQUIRE(rank >= 1 && rank <= kMaxRank, PM_ERR_UNSUPPORTED, "%s: rank %lld (1 .. %d)", who, (long long)rank, kMaxRank);
   PM_REQUIRE(d_in >= 8 && d_in % 8 == 0 && d_in <= (1 << 22) && d_out >= 8 && d_out % 8 == 0 && d_out <= (1 << 22), PM_ERR_UNSUPPORTED,
              "%s: d_in %lld, d_out %lld (multiples of 8, at most 2^22)", who, (long long)d_in, (long long)d_out);
+  return PM_OK;
+}
+// a launch holds less than 2^32 threads; expand's is the largest
+static int check_launch(const char* who, int64_t tiles, int64_t d, int rank) {
+  const int64_t cols = rank <= 64 ? 256 : 128;
+  PM_REQUIRE(tiles * cdiv(d, cols) * 256 <= UINT32_MAX, PM_ERR_UNSUPPORTED, "%s: too many rows and columns for one call: %lld tiles of %d rows by %lld columns", who, (long long)tiles,
+             kExpandRows, (long long)d);
   return PM_OK;
 }
 static int check_rows(const char* who, const char* name, const void* p, int64_t ld, int64_t d) {
@@ -902,6 +911,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
                            int64_t workspace_bytes, void* stream) {
   PM_TRY(check_shape("pm_lora_fwd", n_rows, n_adapters, d_in, d_out, rank));
   if (n_rows == 0) return PM_OK;
+  PM_TRY(check_launch("pm_lora_fwd", max_tiles(n_rows, n_adapters, kExpandRows), d_out, rank));
   PM_REQUIRE(a && b && scales && offsets && z, PM_ERR_INVALID_ARG, "pm_lora_fwd: null pointer");
   PM_TRY(check_rows("pm_lora_fwd", "x", x, ldx, d_in));
   PM_TRY(check_rows("pm_lora_fwd", "out", out, ldout, d_out));
@@ -959,10 +969,12 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
                            const int32_t* row_ids, int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base, int64_t ldbase, void* grad_x,
                            int64_t ldgx, float* grad_a, float* grad_b, int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
   PM_TRY(check_shape("pm_lora_bwd", n_rows, n_adapters, d_in, d_out, rank));
+  PM_TRY(check_launch("pm_lora_bwd", max_tiles(n_rows, n_adapters, kExpandRows), d_in, rank));
   PM_REQUIRE((grad_a != nullptr) == (grad_b != nullptr), PM_ERR_INVALID_ARG, "pm_lora_bwd: grad_a and grad_b go together");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z | (uintptr_t)grad_a | (uintptr_t)grad_b) & 15) == 0, PM_ERR_INVALID_ARG,
              "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
   PM_REQUIRE(offsets, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
+  if (!grad_x && !grad_a) return PM_OK;  // nothing is wanted
   hipStream_t st = as_stream(stream);
   unsigned char* ws = (unsigned char*)workspace;
   BwdPlan p{};
@@ -1021,6 +1033,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
 extern "C" int pm_lora_merge(const void* weight, int64_t ldw, const void* a, const void* b, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out, int64_t ldo,
                              void* stream) {
   PM_TRY(check_shape("pm_lora_merge", d_out, 1, d_in, d_out, rank));
+  PM_TRY(check_launch("pm_lora_merge", cdiv(d_out, kExpandRows), d_in, rank));
   PM_REQUIRE(a && b, PM_ERR_INVALID_ARG, "pm_lora_merge: null pointer");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_merge: a and b must be 16-byte aligned");
   PM_TRY(check_rows("pm_lora_merge", "weight", weight, ldw, d_in));

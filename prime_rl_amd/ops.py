@@ -1139,7 +1139,7 @@ def _lora_factors(a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, row_ids
 
 def lora_rows(adapter_ids: Tensor, n_adapters: int) -> tuple[Tensor, Tensor]:
     """(offsets [n_adapters + 1], row_ids [N]) of rows in any order, `adapter_ids` [N] holding each row's adapter; an id outside [0, n_adapters) is a row of no
-    adapter.  Rows of one adapter keep their order."""
+    adapter.  Rows of one adapter keep their order.  The tables of a captured graph are made before it."""
     ids = _req(adapter_ids, None, "adapter_ids").reshape(-1).to(torch.int64)
     ids = torch.where((ids >= 0) & (ids < n_adapters), ids, n_adapters)
     ids, order = torch.sort(ids, stable=True)  # plumbing: index sort only
@@ -1152,7 +1152,7 @@ def lora_fwd(x: Tensor, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, b
     base's row for rows of no adapter (pm_lora_fwd).
 
     x [N, d_in], base [N, d_out] (None: zeros) bf16, with row strides; a [n, rank, d_in], b [n, rank, d_out] bf16; scales [n] f32.  Position p, in
-    [offsets[g], offsets[g + 1]) of adapter g, is row `row_ids[p]` (`lora_rows`), or row p without row_ids.  `out` may be `base` (in place).  z is what `lora_bwd` takes."""
+    [offsets[g], offsets[g + 1]) of adapter g, is row `row_ids[p]` (`lora_rows`; each row once), or row p without row_ids.  `out` may be `base` (in place).  z is what `lora_bwd` takes."""
     lib = _lib.load()
     rows = x.shape[0]
     n, rank, d_in, d_out = _lora_factors(a, b, scales, offsets, row_ids, rows)
@@ -1244,7 +1244,8 @@ class GradClipPlan:
 
     `grads`: contiguous f32 | bf16 GPU tensors; `groups[i]` in [0, n_groups) is the group of grads[i] (None: one group).  `out[i]`, f32 | bf16 of the same size,
     receives the clipped grads[i] — e.g. a slice of the flat f32 gradient that `adamw_step` reads; without `out` the gradients are clipped in place.  The plan
-    holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are."""
+    holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are, and keep it as long as a captured graph of
+    its calls."""
 
     _CHUNK_MOST, _PIECE = 65536, 2048
 
@@ -1296,6 +1297,7 @@ class GradClipPlan:
         _, pieces = cut(self._PIECE)
         self.n_chunks, self.n_pieces = len(chunks), len(pieces)
         self._table, self._pieces = (torch.from_numpy(np.ascontiguousarray(t)).to(self.device) for t in (chunks, pieces))
+        self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)  # the tables' own
         self._offsets = torch.from_numpy(np.searchsorted(np.array(groups, dtype=np.int64)[of], np.arange(self.n_groups + 1)).astype(np.int32)).to(self.device)
 
     def _run(self, max_norm, sumsq: Tensor | None, want_sumsq: bool, scale: bool) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
@@ -1308,6 +1310,9 @@ class GradClipPlan:
         for t, nm in ((limits, "max_norm"), (sumsq, "sumsq")):
             if t is not None and (t.numel() != self.n_groups or t.device != self.device):
                 raise PrimeMI355XError(f"{nm}: expected {self.n_groups} values on {self.device}, got {t.numel()} on {t.device}")
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:  # the tables' memory is not given away before this stream is done with them
+            for t in (self._table, self._pieces, self._offsets):
+                t.record_stream(torch.cuda.current_stream(self.device))
         partials = torch.empty(self.n_chunks + 1, dtype=torch.float64, device=self.device) if sumsq is None else None
         sums = both = norms = coefs = None
         if want_sumsq:

@@ -165,3 +165,21 @@ def test_plans_refuse_what_they_cannot_hold(ops):
         ops.GradClipPlan([t]).clip(torch.ones(1))
     with pytest.raises(E):
         ops.GradClipPlan([t]).clip(1.0, sumsq=torch.ones(1, device=DEV))
+
+
+def test_a_plan_that_goes_while_another_stream_runs_it(ops):
+    """Its tables' memory, of the stream that made it, is not given to other tensors before the stream that runs the plan has read them."""
+    t = torch.full((1 << 20,), 2.0, device=DEV)
+    busy, side = torch.randn(4096, 4096, device=DEV), torch.cuda.Stream()
+    plan = ops.GradClipPlan([t])
+    sizes = [u.numel() for u in (plan._table, plan._pieces)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+        plan.clip(1024.0)
+    del plan
+    for _ in range(8):  # the same sizes from the same stream's memory
+        others = [torch.zeros(n, dtype=torch.int64, device=DEV) for n in sizes]
+    torch.cuda.synchronize()
+    assert ((t - 1.0).abs() <= 8 * 2.0**-24).all(), others  # a norm of 2048

@@ -72,6 +72,21 @@ def test_clip_refuses(lib):
         assert clip(**kw) == -1 and lib.pm_last_error(), kw
 
 
+def test_more_than_a_launch_holds_is_refused(lib):
+    """2^32 threads: 64 x 256 elements for each 256 of them."""
+    wide = dict(n=1 << 28, d_in=64, d_out=1 << 22, ldo=1 << 22, ldb=1 << 22)
+    assert _fwd(lib, **wide) == -2 and b"too many" in lib.pm_last_error()
+    assert _fwd(lib, n=(1 << 28) + 1) == -1
+    assert _bwd(lib, n=1 << 28, d_in=1 << 22, ldx=1 << 22, ldb=1 << 22, ldgx=1 << 22) == -2 and b"too many" in lib.pm_last_error()
+    assert lib.pm_lora_merge(P, 1 << 22, P, P, 1.0, 1 << 22, 1 << 22, 8, P, 1 << 22, None) == -2 and b"too many" in lib.pm_last_error()
+    assert lib.pm_grad_clip(P, 1 << 23, P, 1, P, 3, None, 1.0, None, P, None, P, P, None) == -1
+    assert lib.pm_grad_clip(P, 3, P, (1 << 20) + 1, P, 3, None, 1.0, None, P, None, P, P, None) == -1
+
+
+def test_a_backward_of_nothing_is_no_work(lib):
+    assert _bwd(lib, dx=None, da=None, db=None, ws=None) == 0
+
+
 def test_workspaces_follow_the_sizes(lib):
     assert [lib.pm_lora_z_columns(r) for r in (0, 1, 16, 17, 128, 129)] == [0, 16, 16, 32, 128, 0]
     assert lib.pm_lora_fwd_workspace_bytes(0, 4, 4096, 16) == 0 and lib.pm_lora_fwd_workspace_bytes(16384, 4, 4096, 16) == 0  # enough rows: the long axis stays whole
@@ -136,3 +151,17 @@ def test_attaching_adapters():
     state.rows = object()
     with pytest.raises(ValueError, match="frozen"):
         lora_linear(torch.zeros(3, 32), [mlp.gate_proj])
+
+
+def test_a_model_has_one_set_of_adapters():
+    from prime_rl_amd.trainer.models.layers.lora import LoRAAdapters, LoRAState, attach_lora, lora_linear
+    from prime_rl_amd.trainer.models.layers.mlp import MLP, MLPConfig
+
+    mlp = MLP(MLPConfig(32, 64))
+    attach_lora(mlp, 2, 4, 8.0, targets=("gate_proj",))
+    with pytest.raises(ValueError, match="already"):
+        attach_lora(mlp, 2, 4, 8.0, targets=("down_proj",))
+    other = LoRAState(2, 4, 16.0, "cpu")
+    mlp.up_proj.lora = LoRAAdapters(mlp.up_proj, other)
+    with pytest.raises(ValueError, match="different states"):
+        lora_linear(torch.zeros(3, 32), [mlp.gate_proj, mlp.up_proj])
