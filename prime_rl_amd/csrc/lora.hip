@@ -129,6 +129,7 @@ __device__ __forceinline__ f32x4 sum_parts(const float* __restrict__ at, int64_t
 // of a fragment read lie in different banks.  The factor's chunk is read once for each tile (from L2), which bounds how small a tile may be.
 // All tiles run at once and walk the columns together.  Each begins at a chunk of its own: in step they would ask for the same columns of every row, which lie on few
 // of the memory channels (reading 32 768 x 4096 this way: 63 us in step, 46 with the turn; a linear read takes 44).
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }  // of the memory accesses before and after: what is counted below
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // at most n DMA instructions of this wave outstanding
 __device__ __forceinline__ void wait_dma(int n) {
@@ -543,6 +544,14 @@ __device__ __forceinline__ void tr_read_tile(const uint32_t (&a)[4], u32x2 (&v)[
       : "memory");
 }
 
+// 16 bytes at each of a[0], a[1] and 16 rows on, likewise
+__device__ __forceinline__ void read_tile(const uint32_t (&a)[2], u32x4 (&v)[4]) {
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:16384\n\tds_read_b128 %3, %5 offset:16384\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+               : "v"(a[0]), "v"(a[1])
+               : "memory");
+}
+
 template <int RT, bool DZ>
 __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
                                                     int n_adapters, int rank, int rp) {
@@ -555,16 +564,20 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
   __shared__ __attribute__((aligned(16))) unsigned char lz[2][3][SP * kZs];
   __shared__ int li[kOuterIds];
   __shared__ __attribute__((aligned(16))) float lp[DZ ? 2 : 1][DZ ? 8 * SP * 16 : 4];  // dz of a stage, from each wave
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
-  const int split = blockIdx.x / tiles01, col_tile = blockIdx.x % tiles01;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lq = lane >> 4;
+  // an XCD (workgroups go round the eight of them) takes neighbouring ranges with all their columns: whole rows, and a range's z once
+  const int xcd = blockIdx.x & 7, block = xcd * (int)(gridDim.x >> 3) + min(xcd, (int)(gridDim.x & 7)) + (int)(blockIdx.x >> 3);
+  const int split = block / tiles01, col_tile = block % tiles01;
   const bool second = col_tile >= tiles0;
   const OuterSide s = second ? s1 : s0;
   const int c0 = (second ? col_tile - tiles0 : col_tile) * kOuterCols;
   const int begin = split * s.range, end = min(begin + s.range, n);
-  // the first adapter whose positions reach past `begin`
-  int g = n_adapters;
-  for (int e0 = 0; e0 < n_adapters; e0 += 64) {
-    const unsigned long long hit = __ballot(e0 + lane < n_adapters && offsets[min(e0 + lane, n_adapters - 1) + 1] > begin);
+  // the first adapter whose positions reach past `begin`; lane i holds the offsets of adapter e0 + i
+  int g = n_adapters, e0 = 0, from = 0, upto = 0;
+  auto look = [&]() { from = offsets[min(e0 + lane, n_adapters)], upto = offsets[min(e0 + lane + 1, n_adapters)]; };
+  for (; e0 < n_adapters; e0 += 64) {
+    look();
+    const unsigned long long hit = __ballot(e0 + lane < n_adapters && upto > begin);
     if (hit) {
       g = e0 + __ffsll((long long)hit) - 1;
       break;
@@ -576,9 +589,10 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
     const int row = lq * 4 + (lr >> 2);
     ta[i] = (uint32_t)(uintptr_t)(lds_void_ptr)lt + row * kRowBytes + (((wave * 4 + i) ^ (row & 7)) << 5) + (lr & 3) * 8;
   }
-  int lo = g < n_adapters ? min(max(offsets[g], begin), end) : end;
+  int lo = g < n_adapters ? min(max(__builtin_amdgcn_readlane(from, g - e0), begin), end) : end;
   for (; g < n_adapters && lo < end; ++g) {
-    const int hi = min(max(offsets[g + 1], lo), end);
+    if (g - e0 == 64) e0 = g, look();
+    const int hi = min(max(__builtin_amdgcn_readlane(upto, g - e0), lo), end);
     if (hi == lo) continue;
     f32x4 acc[4][RT];
 #pragma unroll
@@ -588,12 +602,6 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
     u32x4 wf[2];
     float scale = 0.f;
     const int wcol = c0 + wave * 64 + lq * 8;
-    if constexpr (DZ) {
-      scale = s.scales[g];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        wf[k] = lr < rank && wcol + k * 32 < s.d ? *reinterpret_cast<const u32x4*>(s.w + ((int64_t)g * rank + lr) * s.d + wcol + k * 32) : u32x4{0, 0, 0, 0};
-    }
     for (int first = lo, last; first < hi; first = last) {
       last = row_ids ? min(first + kOuterIds, hi) : hi;
       const int stages = (last - first + SP - 1) / SP, full = (last - first) / SP;
@@ -610,8 +618,10 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         for (int i = 0; i < kDma; ++i) {
           const int p = st * SP + i * 8 + wave;
           if (whole || first + p < last) {
-            const int row = row_ids ? li[p] : first + p;
-            dma16(s.t + (int64_t)row * s.ldt + col, to + i * 8 * kRowBytes);
+            const int row = row_ids ? __builtin_amdgcn_readfirstlane(li[p]) : first + p;
+            // a buffer access: the compiler cannot count past global accesses that write LDS, and would wait for all of them with each z
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(s.t + (int64_t)row * s.ldt), 0, s.d * 2, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void_ptr)(to + i * 8 * kRowBytes), 16, col * 2, 0, 0, 0);
           } else {  // positions behind the last are zeros on both sides
             *reinterpret_cast<u32x4*>(to + i * 8 * kRowBytes + lane * 16) = u32x4{0, 0, 0, 0};
           }
@@ -655,15 +665,15 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
       };
       // this wave's 64 columns of dz, 32 positions x 16 ranks; and a value of the last stage's dz from all waves for each thread
       auto contract = [&](int st) {
-        const unsigned char* at = lt + st % kOuterRing * kBuf;
+        const uint32_t at = (uint32_t)(uintptr_t)(lds_void_ptr)lt + st % kOuterRing * kBuf + lr * kRowBytes + (((wave * 8 + lq) ^ ((lr & 7) << 1)) << 4);
+        const uint32_t a[2] = {at, at ^ 64};
+        u32x4 v[4];
+        read_tile(a, v);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(at + (i * 16 + lr) * kRowBytes + (((wave * 8 + k * 4 + lq) ^ ((lr & 7) << 1)) << 4));
-            sum = mfma(wf[k], wcol + k * 32 < s.d ? v : u32x4{0, 0, 0, 0}, sum);
-          }
+          for (int k = 0; k < 2; ++k) sum = mfma(wf[k], wcol + k * 32 < s.d ? v[2 * i + k] : u32x4{0, 0, 0, 0}, sum);
           *reinterpret_cast<f32x4*>(&lp[st & 1][(wave * SP + i * 16 + lr) * 16 + lq * 4]) = sum;
         }
       };
@@ -674,30 +684,33 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         const int p = first + st * SP + (tid >> 4);
         if (whole || p < last) s.dz[((int64_t)col_tile * n + p) * 16 + (tid & 15)] = (tid & 15) < rank ? sum * scale : 0.f;
       };
+      if constexpr (DZ) {
+        if (first == lo) {
+          scale = s.scales[g];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            wf[k] = lr < rank && wcol + k * 32 < s.d ? *reinterpret_cast<const u32x4*>(s.w + ((int64_t)g * rank + lr) * s.d + wcol + k * 32) : u32x4{0, 0, 0, 0};
+        }
+      }
       // stage st: t comes two stages ahead, z three (it is split one stage ahead)
-      f32x4 za[kZp], zb[kZp];
-      fetch(0, full > 0);
-      load_z(0, za, s.parts);
-      if (stages > 1) fetch(1, full > 1);
-      split_z(0, za);
-      load_z(min(1, stages - 1), zb, s.parts);
-      load_z(min(2, stages - 1), za, s.parts);
+      f32x4 z0[kZp], za[kZp], zb[kZp];
       int st = 0;
       auto stage = [&](auto steady, f32x4 (&next)[kZp]) {  // `next` holds z of stage st + 1, and gets that of st + 3
         if constexpr (decltype(steady)::value) {
           wait_dma(kDma + kZp + (DZ ? 1 : 0));  // younger than t of this stage: t of the next, z of the one after it, a store of dz
           lds_barrier();
+          split_z(st + 1, next);
           if constexpr (DZ)
             if (st > 0) store_dz(st - 1, true);
-          split_z(st + 1, next);
           fetch(st + 2, true);
+          keep_order();
           load_z(st + 3, next, 1);
         } else {
           wait_dma(0);
           lds_barrier();
+          if (st + 1 < stages) split_z(st + 1, next);
           if constexpr (DZ)
             if (st > 0) store_dz(st - 1, false);
-          if (st + 1 < stages) split_z(st + 1, next);
           if (st + 2 < stages) fetch(st + 2, st + 2 < full);
           if (st + 3 < stages) load_z(st + 3, next, s.parts);
         }
@@ -705,11 +718,31 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         if constexpr (DZ) contract(st);
         ++st;
       };
-      if (s.parts == 1)
-        while (st + 4 < full) {
+      // z and t are asked for in the order in which the loop goes on, every time: the compiler takes the least it sees on any way into the loop for the number of accesses younger than a
+      // z that it waits for, and would drain everything in every second stage
+      if (s.parts == 1 && full > 3) {
+        load_z(0, z0, 1);
+        keep_order();
+        fetch(0, true);
+        keep_order();
+        load_z(1, zb, 1);
+        keep_order();
+        fetch(1, true);
+        keep_order();
+        load_z(2, za, 1);
+        split_z(0, z0);
+        do {
           stage(std::true_type{}, zb);
           stage(std::true_type{}, za);
-        }
+        } while (st + 3 < full);
+      } else {
+        load_z(0, z0, s.parts);
+        fetch(0, full > 0);
+        load_z(min(1, stages - 1), zb, s.parts);
+        if (stages > 1) fetch(1, full > 1);
+        load_z(min(2, stages - 1), za, s.parts);
+        split_z(0, z0);
+      }
       while (st < stages) {
         stage(std::false_type{}, zb);
         if (st < stages) stage(std::false_type{}, za);
@@ -784,10 +817,13 @@ struct ShrinkPlan {
   int rows, depth, parts, chunks_per_part;
   int64_t tiles;
 };
-// Narrow: 32 positions a tile; where the tiles are fewer than the 512 workgroups that run at once, the long axis is cut into parts of at least two chunks.
+// Narrow: 32 positions a tile; where the tiles are fewer than the 512 workgroups that run at once, the long axis is cut into parts of at least two chunks.  Workgroups that
+// all run at once end at very different times (16 384 x 12288: the first at 68, the last at 105 us), so long rows of up to two rounds are cut into parts of 12 chunks and more, which later
+// workgroups take where there is room: the forward from 12288 to 4096 columns 158 -> 146 us at 16 384 rows, 91 -> 75 at 8192 (shorter parts or more rounds: no gain).  The
+// backward's dz stays whole: outer would add the parts up in each column tile (+15 %).
 // Wide: a tile's rows and the parts are chosen together to make the busiest CU's work least: rounds of 256 workgroups (257 tiles of 128 rows take 1.5 times as long as 256) times
 // what one moves (its rows and the factor, 256 bytes each in a chunk, and a start as long as 160 of these), and the parts of z, which are written and read again.
-static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank) {
+static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank, bool forward) {
   ShrinkPlan p;
   const bool narrow = rank <= 16;
   const int factor = rank_tiles(rank) * 16, chunks = (int)cdiv(d, narrow ? kNarrowChunk : kWideChunk), most = chunks / 2 < kMostParts ? (chunks / 2 > 1 ? chunks / 2 : 1) : kMostParts;
@@ -795,6 +831,10 @@ static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank)
   if (narrow) {
     p.rows = kNarrowRows, p.depth = kRing, p.tiles = max_tiles(n, n_adapters, p.rows);
     p.parts = parts_of(p.tiles > 0 ? p.tiles : 1, 512);
+    if (forward && p.tiles > 0 && p.tiles <= 1024) {
+      const int even = chunks / 12 < 2200 / (int)p.tiles ? chunks / 12 : 2200 / (int)p.tiles;
+      p.parts = even > kMostParts ? kMostParts : even > p.parts ? even : p.parts;
+    }
   } else {
     double least = 0.0;
     p.rows = 0;
@@ -902,7 +942,7 @@ extern "C" int64_t pm_lora_z_columns(int32_t rank) { return rank >= 1 && rank <=
 
 extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank) {
   if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
-  const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank).parts;
+  const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true).parts;
   return parts > 1 ? (int64_t)parts * n_rows * padded_rank(rank) * 4 : 0;
 }
 
@@ -918,7 +958,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   if (base) PM_TRY(check_rows("pm_lora_fwd", "base", base, ldbase, d_out));
   PM_REQUIRE(base != out || ldbase == ldout, PM_ERR_INVALID_ARG, "pm_lora_fwd: base and out are the same rows with different strides");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
-  const ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank);
+  const ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true);
   const int parts = plan.parts;
   const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, rank);
   PM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PM_ERR_WORKSPACE, "pm_lora_fwd: workspace of %lld bytes, %lld needed",
@@ -947,7 +987,7 @@ BwdPlan bwd_plan(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int ran
   const int rp = padded_rank(rank);
   p.tiles0 = (int)cdiv(d_out, kOuterCols), p.tiles1 = (int)cdiv(d_in, kOuterCols);
   p.fused = factors && rank <= 16 && n * d_out >= kFusedElements;
-  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
+  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank, false);
   if (p.fused) p.shrink.parts = 1;
   p.range0 = outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
   p.range1 = p.fused ? outer_range(n, n_adapters, p.tiles1, rank) : p.range0;
