@@ -78,13 +78,13 @@ __device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int 
     const unsigned long long hit = __ballot(base + incl > t);
     if (hit) {
       const int src = __ffsll((long long)hit) - 1;
-      const int first = base + __shfl(incl, src, 64) - __shfl(tiles, src, 64);
+      const int first = base + __builtin_amdgcn_readlane(incl, src) - __builtin_amdgcn_readlane(tiles, src);
       adapter = e0 + src < n_adapters ? e0 + src : -1;
-      p0 = __shfl(lo, src, 64) + (t - first) * rows;
-      p1 = min(p0 + rows, __shfl(hi, src, 64));
+      p0 = __builtin_amdgcn_readlane(lo, src) + (t - first) * rows;
+      p1 = min(p0 + rows, __builtin_amdgcn_readlane(hi, src));
       return true;
     }
-    base += __shfl(incl, 63, 64);
+    base += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
 }
@@ -127,6 +127,7 @@ __device__ __forceinline__ f32x4 sum_parts(const float* __restrict__ at, int64_t
 // Chunks of columns of a tile's rows and of the factor come into LDS by DMA (global_load_lds: no registers, and one instruction takes whole stretches of a
 // row), a ring of mostly three deep, so that two are in flight while the matrix cores work on one.  16-byte slots of a row are permuted by its row number: the 16 rows
 // of a fragment read lie in different banks.  The factor's chunk is read once for each tile (from L2), which bounds how small a tile may be.
+// What is the same for a wave (its number, the tile) is held as a scalar (readfirstlane, readlane): the waits' switch and the pieces' conditions cost no lanes.
 // All tiles run at once and walk the columns together.  Each begins at a chunk of its own: in step they would ask for the same columns of every row, which lie on few
 // of the memory channels (reading 32 768 x 4096 this way: 63 us in step, 46 with the turn; a linear read takes 44).
 __device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }  // of the memory accesses before and after: what is counted below
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __r
                                                                int parts, int chunks_per_part, float* __restrict__ z) {
   constexpr int kRowBytes = kNarrowChunk * 2, kBytes = (kNarrowRows + 16) * kRowBytes;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kRing * kBytes];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
   const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
   int adapter, p0, p1;
   if (!locate(offsets, n_adapters, n, kNarrowRows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restri
                                                           int rows, int depth, int parts, int chunks_per_part, float* __restrict__ z) {
   constexpr int kRowBytes = kWideChunk * 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
   const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
   int adapter, p0, p1;
   if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
                                                         int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place) {
   using S = ExpandShape<RT>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lq = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lq = lane >> 4;
   const int col_tiles = (d + S::kCols - 1) / S::kCols, row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x % col_tiles;
   int adapter = 0, p0 = row_tile * kExpandRows, p1 = min(p0 + kExpandRows, n);
   if constexpr (!MERGE) {
