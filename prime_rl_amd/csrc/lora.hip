@@ -144,59 +144,70 @@ __device__ __forceinline__ void wait_dma(int n) {
     default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
   }
 }
-__device__ __forceinline__ void dma16(const bf16_t* from, unsigned char* to) { __builtin_amdgcn_global_load_lds((glb_void_ptr)from, (lds_void_ptr)to, 16, 0, 0); }
+constexpr int kStream = 2;  // cache policy of an access: do not keep
+template <int POLICY>
+__device__ __forceinline__ void dma16(const bf16_t* from, unsigned char* to) { __builtin_amdgcn_global_load_lds((glb_void_ptr)from, (lds_void_ptr)to, 16, 0, POLICY); }
 
 // The ring: chunk i of `count` is chunk turn + i of the part's full ones (round and round), the last, shorter one stays last and comes through registers.
-// NT + NW instructions of a wave fill a chunk: instruction i of t (i < nt) takes tp[i] to to + i * 4 KiB, of w to `wofs` behind that.
-template <int KC, int NT, int NW>
+// NT + NW instructions of each of WAVES waves fill a chunk: instruction i of t (i < nt) takes tp[i] to to + i * kStep, of w to `wofs` behind that.
+template <int KC, int WAVES, int NT, int NW>
 struct Ring {
+  static constexpr int kStep = WAVES * 1024;
   const bf16_t* tp[NT];  // this lane's 16 bytes of chunk 0
   const bf16_t* wp[NW];
   int tcol[NT], wcol[NW], nt, wofs, c0, full, turn, d;
+  bool stream;
   __device__ __forceinline__ void fetch(int c, unsigned char* to, int lane) const {
     if (c < full) {
       const int k = (c0 + (c + turn < full ? c + turn : c + turn - full)) * KC;
+      if (stream) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        if (i < nt) dma16(tp[i] + k, to + i * 4096);
+        for (int i = 0; i < NT; ++i)
+          if (i < nt) dma16<kStream>(tp[i] + k, to + i * kStep);
+      } else {
 #pragma unroll
-      for (int i = 0; i < NW; ++i) dma16(wp[i] + k, to + wofs + i * 4096);
+        for (int i = 0; i < NT; ++i)
+          if (i < nt) dma16<0>(tp[i] + k, to + i * kStep);
+      }
+#pragma unroll
+      for (int i = 0; i < NW; ++i) dma16<0>(wp[i] + k, to + wofs + i * kStep);
     } else {  // columns past the end are zeros
       const int k = (c0 + c) * KC;
 #pragma unroll
       for (int i = 0; i < NT; ++i)
-        if (i < nt) *reinterpret_cast<u32x4*>(to + i * 4096 + lane * 16) = k + tcol[i] < d ? *reinterpret_cast<const u32x4*>(tp[i] + k) : u32x4{0, 0, 0, 0};
+        if (i < nt) *reinterpret_cast<u32x4*>(to + i * kStep + lane * 16) = k + tcol[i] < d ? *reinterpret_cast<const u32x4*>(tp[i] + k) : u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < NW; ++i) *reinterpret_cast<u32x4*>(to + wofs + i * 4096 + lane * 16) = k + wcol[i] < d ? *reinterpret_cast<const u32x4*>(wp[i] + k) : u32x4{0, 0, 0, 0};
+      for (int i = 0; i < NW; ++i) *reinterpret_cast<u32x4*>(to + wofs + i * kStep + lane * 16) = k + wcol[i] < d ? *reinterpret_cast<const u32x4*>(wp[i] + k) : u32x4{0, 0, 0, 0};
     }
   }
 };
 
-// One instruction fills 1 KiB: kPer rows of KC columns.  Instruction i of wave v is piece 4 i + v.
-template <int KC, int NT, int NW>
-__device__ __forceinline__ void ring_setup(Ring<KC, NT, NW>& ring, const bf16_t* t, int64_t ldt, const bf16_t* w, const int32_t* row_ids, int n, int adapter, int rank, int d, int p0,
-                                           int p1, int nt, int rows_lds, int wave, int lane) {
+// One instruction fills 1 KiB: kPer rows of KC columns.  Instruction i of wave v is piece WAVES i + v.
+template <int KC, int WAVES, int NT, int NW>
+__device__ __forceinline__ void ring_setup(Ring<KC, WAVES, NT, NW>& ring, const bf16_t* t, int64_t ldt, const bf16_t* w, const int32_t* row_ids, int n, int adapter, int rank, int d, int p0,
+                                           int p1, int nt, int rows_lds, int wave, int lane, bool stream) {
   constexpr int kSlots = KC / 8, kPer = 64 / kSlots, kMask = kSlots < 16 ? kSlots - 1 : 15;
   const int sub = lane / kSlots, slot = lane % kSlots;
   int pos[NT], row[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {  // positions past the tile's end repeat its first row and are not stored
-    const int p = p0 + (i * 4 + wave) * kPer + sub;
+    const int p = p0 + (i * WAVES + wave) * kPer + sub;
     pos[i] = p < p1 ? p : p0;
   }
   rows_of(row_ids, pos, n, row);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    ring.tcol[i] = (slot ^ (((i * 4 + wave) * kPer + sub) & kMask)) * 8;
+    ring.tcol[i] = (slot ^ (((i * WAVES + wave) * kPer + sub) & kMask)) * 8;
     ring.tp[i] = t + (int64_t)row[i] * ldt + ring.tcol[i];
   }
 #pragma unroll
   for (int i = 0; i < NW; ++i) {  // factor rows past the rank repeat the first; what they give is not stored
-    const int r = (i * 4 + wave) * kPer + sub;
+    const int r = (i * WAVES + wave) * kPer + sub;
     ring.wcol[i] = (slot ^ (r & kMask)) * 8;
     ring.wp[i] = w + ((int64_t)adapter * rank + (r < rank ? r : 0)) * d + ring.wcol[i];
   }
   ring.nt = nt;
+  ring.stream = stream;
   ring.wofs = rows_lds * KC * 2;
   ring.d = d;
 }
@@ -212,7 +223,7 @@ __device__ __forceinline__ void store_z(float* zp, f32x4 v, int p, int p1, int r
 constexpr int kNarrowRows = 32, kNarrowChunk = 256, kRing = 3;
 __global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
                                                                const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank,
-                                                               int parts, int chunks_per_part, float* __restrict__ z) {
+                                                               int parts, int chunks_per_part, int stream, float* __restrict__ z) {
   constexpr int kRowBytes = kNarrowChunk * 2, kBytes = (kNarrowRows + 16) * kRowBytes;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[kRing * kBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
@@ -220,8 +231,8 @@ __global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __r
   int adapter, p0, p1;
   if (!locate(offsets, n_adapters, n, kNarrowRows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
   constexpr int NT = kNarrowRows * kRowBytes / 4096, NW = 16 * kRowBytes / 4096;
-  Ring<kNarrowChunk, NT, NW> ring;
-  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, NT, kNarrowRows, wave, lane);
+  Ring<kNarrowChunk, 4, NT, NW> ring;
+  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, NT, kNarrowRows, wave, lane, stream != 0);
   const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + kNarrowChunk - 1) / kNarrowChunk - c0);
   ring.c0 = c0;
   ring.full = min(count, d / kNarrowChunk - c0);
@@ -260,33 +271,33 @@ __global__ __launch_bounds__(256, 2) void shrink_narrow_kernel(const bf16_t* __r
   }
 }
 
-// rank > 16: `rows` positions (a multiple of 4 up to 192, chosen on the host), chunks of 128 columns, a ring as deep as the LDS takes (2 to 4); the waves take every
-// fourth 16 positions and all columns.
+// rank > 16: `rows` positions (a multiple of 4 up to 192, chosen on the host), chunks of 128 columns, a ring as deep as the LDS takes (2 to 4); of the eight waves four take
+// every fourth 16 positions and the first half of a chunk, four the second half, and their results are added up through LDS (two waves on a SIMD wait for LDS in turn).
 constexpr int kWideRows = 192, kWideChunk = 128;
 template <int RT>
-__global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
+__global__ __launch_bounds__(512) void shrink_wide_kernel(const bf16_t* __restrict__ t, int64_t ldt, const bf16_t* __restrict__ w, const float* __restrict__ scales,
                                                           const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n, int n_adapters, int d, int rank, int rp,
-                                                          int rows, int depth, int parts, int chunks_per_part, float* __restrict__ z) {
-  constexpr int kRowBytes = kWideChunk * 2;
+                                                          int rows, int depth, int parts, int chunks_per_part, int stream, float* __restrict__ z) {
+  constexpr int kRowBytes = kWideChunk * 2, NW = RT / 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
   const int part = blockIdx.x % parts, row_tile = blockIdx.x / parts;
   int adapter, p0, p1;
   if (!locate(offsets, n_adapters, n, rows, row_tile, lane, adapter, p0, p1) || adapter < 0) return;
-  const int nt = (p1 - p0 + 15 - 4 * wave) >> 4;  // instructions of this wave that bring rows, four each; every fourth is its own
-  const int held = (rows + 15) & ~15;
-  Ring<kWideChunk, kWideRows / 16, RT> ring;
-  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, nt, held, wave, lane);
+  const int nt = (p1 - p0 + 31 - 4 * wave) >> 5;  // instructions of this wave that bring rows, four each; every eighth is its own
+  const int held = (rows + 15) & ~15, own = wave & 3, half = wave >> 2;
+  Ring<kWideChunk, 8, kWideRows / 32, NW> ring;
+  ring_setup(ring, t, ldt, w, row_ids, n, adapter, rank, d, p0, p1, nt, held, wave, lane, stream != 0);
   const int c0 = part * chunks_per_part, count = min(chunks_per_part, (d + kWideChunk - 1) / kWideChunk - c0);
   ring.c0 = c0;
   ring.full = min(count, d / kWideChunk - c0);
-  ring.turn = ring.full > 0 ? row_tile % ring.full : 0;
+  ring.turn = ring.full > 0 ? (int)(blockIdx.x / 32 * 8 + blockIdx.x % 8) % ring.full : 0;
   f32x4 acc[3][RT];
 #pragma unroll
   for (int i = 0; i < 3; ++i)
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int bytes = (held + RT * 16) * kRowBytes, newer = (depth - 2) * (nt + RT);
+  const int bytes = (held + RT * 16) * kRowBytes, newer = (depth - 2) * (nt + NW);
   unsigned char* mine = lds + wave * 1024;
   for (int c = 0; c < depth - 1 && c < count; ++c) ring.fetch(c, mine + c * bytes, lane);
   for (int c = 0, buf = 0; c < count; ++c) {
@@ -295,14 +306,14 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restri
     if (c + depth - 1 < count) ring.fetch(c + depth - 1, mine + (buf > 0 ? buf - 1 : depth - 1) * bytes, lane);
     const unsigned char* at = lds + buf * bytes;
 #pragma unroll
-    for (int k = 0; k < kWideChunk / 32; ++k) {
-      const int off = lr * kRowBytes + (((k * 4 + lq) ^ lr) << 4);
+    for (int k = 0; k < kWideChunk / 64; ++k) {
+      const int off = lr * kRowBytes + ((((half * 2 + k) * 4 + lq) ^ lr) << 4);
       u32x4 wf[RT];
 #pragma unroll
       for (int j = 0; j < RT; ++j) wf[j] = *reinterpret_cast<const u32x4*>(at + (held + j * 16) * kRowBytes + off);
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        const int group = i * 4 + wave;
+        const int group = i * 4 + own;
         if (group * 16 >= p1 - p0) break;
         const u32x4 tf = *reinterpret_cast<const u32x4*>(at + group * 16 * kRowBytes + off);
 #pragma unroll
@@ -311,11 +322,21 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const bf16_t* __restri
     }
     buf = buf + 1 < depth ? buf + 1 : 0;
   }
+  lds_barrier();
+  f32x4* red = reinterpret_cast<f32x4*>(lds) + own * 3 * RT * 64;
+  if (half)
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) red[(i * RT + j) * 64 + lane] = acc[i][j];
+  lds_barrier();
+  if (half) return;
   const float scale = scales[adapter];
 #pragma unroll
   for (int i = 0; i < 3; ++i)
 #pragma unroll
-    for (int j = 0; j < RT; ++j) store_z(z + (int64_t)part * n * rp, acc[i][j], p0 + (i * 4 + wave) * 16 + lr, p1, j * 16 + lq * 4, rank, rp, scale);
+    for (int j = 0; j < RT; ++j)
+      store_z(z + (int64_t)part * n * rp, acc[i][j] + red[(i * RT + j) * 64 + lane], p0 + (i * 4 + own) * 16 + lr, p1, j * 16 + lq * 4, rank, rp, scale);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -345,7 +366,7 @@ struct ExpandShape {
 template <int RT, bool MERGE>
 __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict__ z, int parts, float* __restrict__ z_out, const bf16_t* __restrict__ zb, float merge_scale,
                                                         const bf16_t* __restrict__ w, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
-                                                        int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place) {
+                                                        int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place, int stream) {
   using S = ExpandShape<RT>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lq = lane >> 4;
@@ -377,9 +398,19 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
   u32x4 bv[2 * S::kMoves];
   auto load_base = [&]() {
     rows_of(row_ids, pos, n, row);
+    auto load = [&](auto streams) {
 #pragma unroll
-    for (int i = 0; i < 2 * S::kMoves; ++i)
-      bv[i] = base && c < d && (i < S::kMoves || p1 - p0 > 32) ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c) : u32x4{0, 0, 0, 0};
+      for (int i = 0; i < 2 * S::kMoves; ++i) {
+        bv[i] = u32x4{0, 0, 0, 0};
+        if (base && c < d && (i < S::kMoves || p1 - p0 > 32)) {
+          const u32x4* from = reinterpret_cast<const u32x4*>(base + (int64_t)row[i] * ldb + c);
+          if constexpr (decltype(streams)::value) bv[i] = __builtin_nontemporal_load(from);
+          else bv[i] = *from;
+        }
+      }
+    };
+    if (stream) load(std::true_type{});
+    else load(std::false_type{});
   };
   if (parts > 1) load_base();  // adding z's parts up waits for them: the base is asked for first
   // z, split into its two bf16 terms on the way to LDS
@@ -553,7 +584,7 @@ __device__ __forceinline__ void read_tile(const uint32_t (&a)[2], u32x4 (&v)[4])
                : "memory");
 }
 
-template <int RT, bool DZ>
+template <int RT, bool DZ, int POLICY>
 __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
                                                     int n_adapters, int rank, int rp) {
   static_assert(!DZ || RT == 1, "dz beside dB: one 16-row block of ranks");
@@ -622,7 +653,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
             const int row = row_ids ? __builtin_amdgcn_readfirstlane(li[p]) : first + p;
             // a buffer access: the compiler cannot count past global accesses that write LDS, and would wait for all of them with each z
             const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(s.t + (int64_t)row * s.ldt), 0, s.d * 2, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void_ptr)(to + i * 8 * kRowBytes), 16, col * 2, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void_ptr)(to + i * 8 * kRowBytes), 16, col * 2, 0, 0, POLICY);
           } else {  // positions behind the last are zeros on both sides
             *reinterpret_cast<u32x4*>(to + i * 8 * kRowBytes + lane * 16) = u32x4{0, 0, 0, 0};
           }
@@ -814,6 +845,11 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 static inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 static inline int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
 constexpr int kLdsBytes = 160 * 1024;  // of a CU
+// Row tensors of this many elements are read past the caches (which then keep the factors, z and what is to come): shrink and outer from 24 Mi (forward 16 384 rows 4096 -> 4096 rank
+// 16 88 -> 77 us, 32 768 rows 12288 -> 4096 rank 64 287 -> 257; 4096 rows of 4096, read again while they are cached: +3 %), expand's base, which a product may have left there, from 80 Mi (forward
+// 16 384 rows 4096 -> 6144 105 -> 98 us, 4096 rows 34 -> 36).
+constexpr int64_t kStreamRows = (int64_t)24 << 20, kStreamBase = (int64_t)80 << 20;
+static inline int streamed(int64_t n, int64_t d) { return n * d >= kStreamRows ? 1 : 0; }
 struct ShrinkPlan {
   int rows, depth, parts, chunks_per_part;
   int64_t tiles;
@@ -875,7 +911,7 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
   const dim3 grid((unsigned)(plan.tiles * plan.parts));
   if constexpr (RT == 1)
     hipLaunchKernelGGL(shrink_narrow_kernel, grid, dim3(256), 0, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets, row_ids, (int)n, n_adapters, d, rank, plan.parts,
-                       plan.chunks_per_part, z);
+                       plan.chunks_per_part, streamed(n, d), z);
   else {
     static bool attr_done[64] = {};  // per device: more than 64 KiB of LDS has to be asked for
     int dev = 0;
@@ -884,8 +920,9 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
       (void)hipFuncSetAttribute((const void*)shrink_wide_kernel<RT>, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
       attr_done[dev & 63] = true;
     }
-    hipLaunchKernelGGL((shrink_wide_kernel<RT>), grid, dim3(256), plan.depth * ((plan.rows + 15) / 16 * 16 + RT * 16) * kWideChunk * 2, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets,
-                       row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.depth, plan.parts, plan.chunks_per_part, z);
+    const int ring = plan.depth * ((plan.rows + 15) / 16 * 16 + RT * 16) * kWideChunk * 2, sums = 12 * RT * 1024;
+    hipLaunchKernelGGL((shrink_wide_kernel<RT>), grid, dim3(512), ring > sums ? ring : sums, stream, (const bf16_t*)t, ldt, (const bf16_t*)w, scales, offsets,
+                       row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.depth, plan.parts, plan.chunks_per_part, streamed(n, d), z);
   }
 }
 template <int RT, bool MERGE>
@@ -895,7 +932,16 @@ static void launch_expand(const float* z, int parts, float* z_out, const void* z
   const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
   const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
   hipLaunchKernelGGL((expand_kernel<RT, MERGE>), dim3(grid), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
-                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0);
+                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0, n * d >= kStreamBase ? 1 : 0);
+}
+template <int RT, bool DZ>
+static void launch_outer(const OuterSide& s0, const OuterSide& s1, int tiles0, int tiles01, unsigned splits, int stream, const int32_t* offsets, const int32_t* row_ids, int64_t n,
+                         int n_adapters, int rank, hipStream_t hip_stream) {
+  const dim3 grid(splits * tiles01);
+  if (stream)
+    hipLaunchKernelGGL((outer_kernel<RT, DZ, kStream>), grid, dim3(512), 0, hip_stream, s0, s1, tiles0, tiles01, offsets, row_ids, (int)n, n_adapters, rank, padded_rank(rank));
+  else
+    hipLaunchKernelGGL((outer_kernel<RT, DZ, 0>), grid, dim3(512), 0, hip_stream, s0, s1, tiles0, tiles01, offsets, row_ids, (int)n, n_adapters, rank, padded_rank(rank));
 }
 #define PM_BY_RANK(rank, CALL)          \
   switch (::pm::lora::rank_tiles(rank)) { \
@@ -1042,18 +1088,17 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     const OuterSide s1{dz, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
     const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
     if (p.fused) {
-      hipLaunchKernelGGL((outer_kernel<1, true>), dim3(splits0 * p.tiles0), dim3(512), 0, st, s0, s0, p.tiles0, p.tiles0, offsets, row_ids, (int)n_rows, n_adapters, rank, 16);
+      launch_outer<1, true>(s0, s0, p.tiles0, p.tiles0, splits0, streamed(n_rows, d_out), offsets, row_ids, n_rows, n_adapters, rank, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
       hipLaunchKernelGGL(sum_dz_kernel, dim3((unsigned)cdiv(n_rows * 4, 256)), dim3(256), 0, st, dz_parts, p.tiles0, n_rows * 16, dz);
       PM_CHECK_LAUNCH("pm_lora_bwd");
-      hipLaunchKernelGGL((outer_kernel<1, false>), dim3(splits1 * p.tiles1), dim3(512), 0, st, s1, s1, p.tiles1, p.tiles1, offsets, row_ids, (int)n_rows, n_adapters, rank, 16);
+      launch_outer<1, false>(s1, s1, p.tiles1, p.tiles1, splits1, streamed(n_rows, d_in), offsets, row_ids, n_rows, n_adapters, rank, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
     } else {
       PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
       PM_CHECK_LAUNCH("pm_lora_bwd");
       if (grad_a) {
-        PM_BY_RANK(rank, hipLaunchKernelGGL((outer_kernel<RT, false>), dim3(splits0 * (p.tiles0 + p.tiles1)), dim3(512), 0, st, s0, s1, p.tiles0, p.tiles0 + p.tiles1, offsets, row_ids,
-                                            (int)n_rows, n_adapters, rank, padded_rank(rank)));
+        PM_BY_RANK(rank, (launch_outer<RT, false>(s0, s1, p.tiles0, p.tiles0 + p.tiles1, splits0, streamed(n_rows, (d_in + d_out) / 2), offsets, row_ids, n_rows, n_adapters, rank, st)));
         PM_CHECK_LAUNCH("pm_lora_bwd");
       }
     }
