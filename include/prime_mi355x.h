@@ -589,7 +589,8 @@ int pm_lora_bwd(const void* grad_out_bf16, int64_t ldg, const void* x_bf16, int6
 int pm_lora_merge(const void* weight_bf16, int64_t ldw, const void* a_bf16, const void* b_bf16, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out_bf16, int64_t ldo,
                   void* stream);
 /* Gradient norms of many tensors by group, and clipping (torch clip_grad_norm_ over each group; trainer/utils.py:88-98).  `chunks` and `pieces`: int64 [n][4] on the device, rows
- * {source address, destination address (0: none), elements, (group << 8) | source is bf16 (bit 0) | destination is bf16 (bit 1)}, f32 where a bit is clear.  The chunks (what is
+ * {source address, destination address (0: none), elements, (group << 8) | source is bf16 (bit 0) | destination is bf16 (bit 1) | sources read (bit 2), destinations written (bit 3) past the
+ * caches, which are too small for all of them}, f32 where bits 0 and 1 are clear.  The chunks (what is
  * added up) of one group stand together, group g's at [group_offsets[g], group_offsets[g+1]) (int32 [n_groups + 1]); the pieces (what is scaled; n_pieces 0: nothing) are any cut of the
  * same memory, about 2048 elements each.  Destinations are their source (same type) or memory of their own.
  *   sumsq_out[g] = sum of squares in 64 bits (nullable); norms[g] = sqrt of it; coefs[g] = min(1, max_norm / (norms[g] + 1e-6)), 1 for max_norm <= 0 (max_norms [n_groups], where it

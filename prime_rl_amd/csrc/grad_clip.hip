@@ -10,33 +10,48 @@
 namespace pm {
 namespace gclip {
 
-struct Chunk {  // one row of the table: int64 [4]
-  const unsigned char* src;
-  unsigned char* dst;  // null: nothing is written
+typedef __attribute__((address_space(1))) unsigned char global_byte;
+struct Chunk {  // one row of the table: int64 [4]; global addresses: the compiler would take others for any kind of memory
+  const global_byte* src;
+  global_byte* dst;  // null: nothing is written
   int64_t n;
-  int64_t flags;  // bit 0: src is bf16, bit 1: dst is bf16, bits 8 and up: group
+  int64_t flags;  // bit 0: src is bf16, bit 1: dst is bf16, bit 2: src is read past the caches, bit 3: dst is written past them, bits 8 and up: group
 };
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
+// outputs start anywhere in a flat buffer: the card takes wide stores at any element (961 MB of 2016 tensors: 545 -> 468 us against one store for each element)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef __attribute__((address_space(1))) f32x4_any global_f32x4_any;
+typedef __attribute__((address_space(1))) u32x2_any global_u32x2_any;
 constexpr int kLoads = 8;  // 16-byte loads of a thread that are in flight together
 
+template <typename T>
+using global = __attribute__((address_space(1))) T;
+
 template <bool BF16>
-__device__ __forceinline__ float one(const unsigned char* p, int64_t i) {
-  if constexpr (BF16) return bf16_to_f32(reinterpret_cast<const bf16_t*>(p)[i]);
-  else return reinterpret_cast<const float*>(p)[i];
+__device__ __forceinline__ float one(const global_byte* p, int64_t i) {
+  if constexpr (BF16) return bf16_to_f32(((const global<bf16_t>*)p)[i]);
+  else return ((const global<float>*)p)[i];
 }
 // elements before the first 16-byte boundary
 template <bool BF16>
-__device__ __forceinline__ int64_t head_of(const unsigned char* p, int64_t n) {
+__device__ __forceinline__ int64_t head_of(const global_byte* p, int64_t n) {
   const int64_t h = (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (BF16 ? 2 : 4);
   return h < n ? h : n;
 }
 
-template <bool BF16>
+template <bool STREAM, typename T>
+__device__ __forceinline__ T load_of(const global<T>* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
+template <bool BF16, bool STREAM>
 __device__ __forceinline__ double chunk_squares(const Chunk& c) {
   constexpr int V = BF16 ? 8 : 4;
   const int64_t head = head_of<BF16>(c.src, c.n), vecs = (c.n - head) / V;
-  const u32x4* body = reinterpret_cast<const u32x4*>(c.src + head * (BF16 ? 2 : 4));
+  const global<u32x4>* body = (const global<u32x4>*)(c.src + head * (BF16 ? 2 : 4));
   double sum[4] = {0.0, 0.0, 0.0, 0.0};
   auto add = [&](const u32x4& v) {
 #pragma unroll
@@ -55,12 +70,12 @@ __device__ __forceinline__ double chunk_squares(const Chunk& c) {
   for (; i + (kLoads - 1) * 256 < vecs; i += kLoads * 256) {
     u32x4 v[kLoads];
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) v[k] = body[i + k * 256];
+    for (int k = 0; k < kLoads; ++k) v[k] = load_of<STREAM, u32x4>(body + i + k * 256);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) add(v[k]);
   }
-  for (; i < vecs; i += 256) add(body[i]);
+  for (; i < vecs; i += 256) add(load_of<STREAM, u32x4>(body + i));
   const int64_t tail = head + vecs * V;
   if (threadIdx.x < head) {
     const double x = one<BF16>(c.src, threadIdx.x);
@@ -88,7 +103,10 @@ __device__ __forceinline__ double block_sum_f64(double v, double* smem) {
 __global__ __launch_bounds__(256) void squares_kernel(const Chunk* __restrict__ chunks, double* __restrict__ partials) {
   __shared__ double smem[4];
   const Chunk c = chunks[blockIdx.x];
-  const double s = block_sum_f64(c.flags & 1 ? chunk_squares<true>(c) : chunk_squares<false>(c), smem);
+  double s;
+  if (c.flags & 4) s = c.flags & 1 ? chunk_squares<true, true>(c) : chunk_squares<false, true>(c);
+  else s = c.flags & 1 ? chunk_squares<true, false>(c) : chunk_squares<false, false>(c);
+  s = block_sum_f64(s, smem);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
@@ -123,56 +141,59 @@ __global__ __launch_bounds__(1024) void coef_kernel(const double* __restrict__ p
 }
 
 // Four elements a thread and turn: 16-byte stores in one stretch (32 bits), and one access at a time, which writes faster than a group of loads before a group of stores
-// (200 M values f32 -> f32: 5.6 TB/s against 5.3).
-template <bool SRC_BF16, bool DST_BF16>
+// (200 M values f32 -> f32: 5.6 TB/s against 5.3).  Past the caches (where flags say so) both ways: 6.3 TB/s, and squares read 6.7 against 5.8.
+template <bool SRC_BF16, bool DST_BF16, bool READ_PAST, bool WRITE_PAST>
 __device__ __forceinline__ void scale_chunk(const Chunk& c, float coef) {
   auto put = [&](int64_t i, float x) {
-    if constexpr (DST_BF16) reinterpret_cast<bf16_t*>(c.dst)[i] = f32_to_bf16(x);
-    else reinterpret_cast<float*>(c.dst)[i] = x;
+    if constexpr (DST_BF16) ((global<bf16_t>*)c.dst)[i] = f32_to_bf16(x);
+    else ((global<float>*)c.dst)[i] = x;
   };
   constexpr int kAlign = SRC_BF16 ? 8 : 16;
   int64_t head = (int64_t)((kAlign - ((uintptr_t)c.src & (kAlign - 1))) & (kAlign - 1)) / (SRC_BF16 ? 2 : 4);
   head = head < c.n ? head : c.n;
   const int64_t vecs = (c.n - head) / 4, tail = head + vecs * 4;
-  const unsigned char* body = c.src + head * (SRC_BF16 ? 2 : 4);
-  unsigned char* to = c.dst + head * (DST_BF16 ? 2 : 4);
-  const bool aligned = ((uintptr_t)to & (DST_BF16 ? 7 : 15)) == 0;
+  const global_byte* body = c.src + head * (SRC_BF16 ? 2 : 4);
+  global_byte* to = c.dst + head * (DST_BF16 ? 2 : 4);
   for (int64_t i = threadIdx.x; i < vecs; i += 256) {
     f32x4v x;
     if constexpr (SRC_BF16) {
-      const u32x2 v = reinterpret_cast<const u32x2*>(body)[i];
+      const u32x2 v = load_of<READ_PAST, u32x2>((const global<u32x2>*)body + i);
       x = f32x4v{bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y)};
     } else {
-      x = reinterpret_cast<const f32x4v*>(body)[i];
+      x = load_of<READ_PAST, f32x4v>((const global<f32x4v>*)body + i);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) x[q] *= coef;
-    if (!aligned) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) put(head + i * 4 + q, x[q]);
-    } else if constexpr (DST_BF16) {
-      reinterpret_cast<u32x2*>(to)[i] = u32x2{pack_bf16_hw(x[0], x[1]), pack_bf16_hw(x[2], x[3])};
+    if constexpr (DST_BF16) {
+      const u32x2_any v = {pack_bf16_hw(x[0], x[1]), pack_bf16_hw(x[2], x[3])};
+      if constexpr (WRITE_PAST) __builtin_nontemporal_store(v, ((global_u32x2_any*)to) + i);
+      else ((global_u32x2_any*)to)[i] = v;
     } else {
-      reinterpret_cast<f32x4v*>(to)[i] = x;
+      if constexpr (WRITE_PAST) __builtin_nontemporal_store((f32x4_any)x, ((global_f32x4_any*)to) + i);
+      else ((global_f32x4_any*)to)[i] = x;
     }
   }
   if (threadIdx.x < head) put(threadIdx.x, one<SRC_BF16>(c.src, threadIdx.x) * coef);
   if (tail + threadIdx.x < c.n) put(tail + threadIdx.x, one<SRC_BF16>(c.src, tail + threadIdx.x) * coef);
 }
 
+template <bool READ_PAST, bool WRITE_PAST>
 __device__ __forceinline__ void scale_any(const Chunk& c, float coef) {
   if (!c.dst || (coef == 1.0f && c.dst == c.src)) return;  // in place, nothing to clip: every value times one is itself
   switch (c.flags & 3) {
-    case 0: scale_chunk<false, false>(c, coef); break;
-    case 1: scale_chunk<true, false>(c, coef); break;
-    case 2: scale_chunk<false, true>(c, coef); break;
-    default: scale_chunk<true, true>(c, coef); break;
+    case 0: scale_chunk<false, false, READ_PAST, WRITE_PAST>(c, coef); break;
+    case 1: scale_chunk<true, false, READ_PAST, WRITE_PAST>(c, coef); break;
+    case 2: scale_chunk<false, true, READ_PAST, WRITE_PAST>(c, coef); break;
+    default: scale_chunk<true, true, READ_PAST, WRITE_PAST>(c, coef); break;
   }
 }
 // The last pieces come first: they were read last and are still in the caches.
 __global__ __launch_bounds__(256) void scale_kernel(const Chunk* __restrict__ pieces, const float* __restrict__ coefs) {
   const Chunk c = pieces[gridDim.x - 1 - blockIdx.x];
-  scale_any(c, coefs[c.flags >> 8]);
+  const float coef = coefs[c.flags >> 8];
+  if (c.flags & 4) scale_any<true, true>(c, coef);
+  else if (c.flags & 8) scale_any<false, true>(c, coef);
+  else scale_any<false, false>(c, coef);
 }
 // The same where groups are of few chunks: every workgroup adds up its group's partials itself, which takes less than a launch for it would.  The first workgroups write the
 // groups' norms and factors.
@@ -192,7 +213,7 @@ __global__ __launch_bounds__(256) void coef_scale_kernel(const Chunk* __restrict
       coefs[g] = coef_of(norms[g], limit_of(g, max_norm, max_norms));
     }
   }
-  scale_any(c, coef);
+  scale_any<false, false>(c, coef);  // few pieces fit the caches
 }
 
 }  // namespace gclip

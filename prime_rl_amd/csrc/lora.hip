@@ -848,6 +848,7 @@ constexpr int kLdsBytes = 160 * 1024;  // of a CU
 // Row tensors of this many elements are read past the caches (which then keep the factors, z and what is to come): shrink and outer from 24 Mi (forward 16 384 rows 4096 -> 4096 rank
 // 16 88 -> 77 us, 32 768 rows 12288 -> 4096 rank 64 287 -> 257; 4096 rows of 4096, read again while they are cached: +3 %), expand's base, which a product may have left there, from 80 Mi (forward
 // 16 384 rows 4096 -> 6144 105 -> 98 us, 4096 rows 34 -> 36).
+// A weight on its way to another buffer has not been touched before, and streams from 24 Mi as well (12288 x 4096: 40 -> 38 us).
 constexpr int64_t kStreamRows = (int64_t)24 << 20, kStreamBase = (int64_t)80 << 20;
 static inline int streamed(int64_t n, int64_t d) { return n * d >= kStreamRows ? 1 : 0; }
 struct ShrinkPlan {
@@ -932,7 +933,8 @@ static void launch_expand(const float* z, int parts, float* z_out, const void* z
   const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
   const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
   hipLaunchKernelGGL((expand_kernel<RT, MERGE>), dim3(grid), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
-                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0, n * d >= kStreamBase ? 1 : 0);
+                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0,
+                     n * d >= (MERGE && base != out ? kStreamRows : kStreamBase) ? 1 : 0);
 }
 template <int RT, bool DZ>
 static void launch_outer(const OuterSide& s0, const OuterSide& s1, int tiles0, int tiles01, unsigned splits, int stream, const int32_t* offsets, const int32_t* row_ids, int64_t n,
