@@ -577,7 +577,7 @@ int pm_gemm_debug_set_variant(int32_t value);
  *   merge: out = bf16(weight + scale * b^T . a) for a weight [d_out, d_in] and ONE adapter a [rank, d_in], b [rank, d_out]: what the weight push sends.  out may be weight.
  * ------------------------------------------------------------------------------------------ */
 int64_t pm_lora_z_columns(int32_t rank);
-int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank);
+int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank);
 int pm_lora_fwd(const void* x_bf16, int64_t ldx, const void* a_bf16, const void* b_bf16, const float* scales, const int32_t* offsets, const int32_t* row_ids /* nullable */,
                 int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base_bf16 /* nullable */, int64_t ldbase, void* out_bf16, int64_t ldout,
                 float* z, void* workspace, int64_t workspace_bytes, void* stream);

@@ -160,7 +160,7 @@ SIGNATURES: dict[str, tuple] = {
     "pm_gemm_swiglu_bwd_bf16": (I, [P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I32, P]),
     "pm_gemm_debug_set_variant": (I, [I32]),
     "pm_lora_z_columns": (I64, [I32]),
-    "pm_lora_fwd_workspace_bytes": (I64, [I64, I32, I64, I32]),
+    "pm_lora_fwd_workspace_bytes": (I64, [I64, I32, I64, I64, I32]),
     "pm_lora_fwd": (I, [P, I64, P, P, P, P, P, I64, I32, I64, I64, I32, P, I64, P, I64, P, P, I64, P]),
     "pm_lora_bwd_workspace_bytes": (I64, [I64, I32, I64, I64, I32, I32]),
     "pm_lora_bwd": (I, [P, I64, P, I64, P, P, P, P, P, P, I64, I32, I64, I64, I32, P, I64, P, I64, P, P, I32, P, I64, P]),

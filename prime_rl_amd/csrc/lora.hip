@@ -31,6 +31,7 @@ typedef __attribute__((address_space(1))) void* glb_void_ptr;
 constexpr int kMaxRank = 128;
 constexpr int64_t kMaxRows = (int64_t)1 << 28;
 constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
+constexpr int kFewWaves = 8;     // of a few_rows workgroup
 constexpr int kOuterCols = 512;  // columns of an outer workgroup
 
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -539,6 +540,103 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// shrink and expand in one launch, for few rows (a token or a few for each adapter) and rank <= 16, where launches are what counts: the forward, and the backward's dz and grad_x.
+// A workgroup takes up to 16 positions of one adapter and 32 BLOCKS columns of out for each of its waves.  It contracts the whole of d_in itself (a wave takes every WAVES-th
+// 64 columns, fragments straight from global memory), though all workgroups of the tile do the same: the factor comes from L2 faster than a second launch would start.  Its share of
+// the other factor and the base are asked for before that, and each lane adds the waves' results up in the layout that the second product takes.
+template <int WAVES, int BLOCKS>
+__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __restrict__ x, int64_t ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b,
+                                                              const float* __restrict__ scales, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                              int n_adapters, int d_in, int d_out, int rank, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place,
+                                                              int groups, float* __restrict__ z) {
+  constexpr int U = 4;
+  __shared__ __attribute__((aligned(16))) f32x4 red[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
+  const int group = blockIdx.x % groups;
+  int adapter, p0, p1;
+  if (!locate(offsets, n_adapters, n, 16, blockIdx.x / groups, lane, adapter, p0, p1) || (adapter < 0 && in_place)) return;
+  const int pos[1] = {p0 + lr < p1 ? p0 + lr : p0};
+  int row[1];
+  rows_of(row_ids, pos, n, row);
+  const int c0 = (group * WAVES + wave) * 32 * BLOCKS;
+  u32x4 bv[BLOCKS];
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i) {
+    const int c = c0 + i * 32 + lq * 8;
+    bv[i] = base && c < d_out ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[0] * ldb + c) : u32x4{0, 0, 0, 0};
+  }
+  if (adapter < 0) {  // rows of no adapter
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+      if (c0 + i * 32 + lq * 8 < d_out && p0 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[0] * ldo + c0 + i * 32 + lq * 8) = bv[i];
+    return;
+  }
+  bf16_t bf[BLOCKS][2][4];  // column 8 (lr / 4) + 4 h + lr % 4 of the block, ranks 4 lq .. 4 lq + 3
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = lq * 4 + q, c = c0 + i * 32 + (lr >> 2) * 8 + h * 4 + (lr & 3);
+        bf[i][h][q] = r < rank && c < d_out ? b[((int64_t)adapter * rank + r) * d_out + c] : (bf16_t)0;
+      }
+  const float scale = scales[adapter];
+  const bf16_t* xp = x + (int64_t)row[0] * ldx + lq * 8;
+  const bf16_t* ap = a + ((int64_t)adapter * rank + (lr < rank ? lr : 0)) * d_in + lq * 8;  // ranks past the last repeat the first; what they give is not used
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int full = d_in >> 6;
+  int s = wave;
+  for (; s + WAVES * (U - 1) < full; s += WAVES * U) {
+    u32x4 xf[U][2], af[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        xf[u][h] = *reinterpret_cast<const u32x4*>(xp + (s + WAVES * u) * 64 + h * 32);
+        af[u][h] = *reinterpret_cast<const u32x4*>(ap + (s + WAVES * u) * 64 + h * 32);
+      }
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc = mfma(af[u][h], xf[u][h], acc);
+  }
+  for (; s * 64 < d_in; s += WAVES) {  // what is left, columns past the end as zeros on both sides
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = s * 64 + h * 32;
+      const bool in = k + lq * 8 < d_in;
+      acc = mfma(in ? *reinterpret_cast<const u32x4*>(ap + k) : u32x4{0, 0, 0, 0}, in ? *reinterpret_cast<const u32x4*>(xp + k) : u32x4{0, 0, 0, 0}, acc);
+    }
+  }
+  red[wave][lane] = acc;  // position lr, ranks 4 lq .. 4 lq + 3
+  __syncthreads();
+  f32x4 v = red[0][lane];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v += red[w][lane];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = lq * 4 + q < rank ? v[q] * scale : 0.f;
+  if (group == 0 && wave == 0 && p0 + lr < p1) *reinterpret_cast<f32x4*>(z + (int64_t)(p0 + lr) * 16 + lq * 4) = v;
+  const u32x2 lead = take_terms(v), rest = to_bf16(v);
+  const u32x4 zf = {lead.x, lead.y, rest.x, rest.y};
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i) {
+    f32x4 sum[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = bf[i][h][0] | (uint32_t)bf[i][h][1] << 16, hi = bf[i][h][2] | (uint32_t)bf[i][h][3] << 16;
+      sum[h] = mfma(u32x4{lo, hi, lo, hi}, zf, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    u32x4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(bv[i][q]) + sum[q >> 1][(q & 1) * 2], bf16hi(bv[i][q]) + sum[q >> 1][(q & 1) * 2 + 1]);
+    const int c = c0 + i * 32 + lq * 8;
+    if (c < d_out && p0 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[0] * ldo + c) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // outer: dW[adapter][r][c] = sum over the adapter's positions of z[p][r] * t[row(p)][c].
 // Both products of the backward (dB from z and dy, dA from dz and x) are one launch.  A workgroup takes 512 columns and one of equal ranges of positions, whatever
 // adapters these belong to: the ranges are cut so that all workgroups run in one round, one on each CU, with the same work each.  At the end of an adapter's positions
@@ -556,6 +654,7 @@ struct OuterSide {
   int d;
   float* part;         // [ranges + adapters][rank][d]
   int range;           // positions of a workgroup
+  int direct;          // 1: one range, `part` is the gradient itself; 2: it is added to
   const bf16_t* w;     // DZ: the factor and scales of dz
   const float* scales;
   float* dz;           // DZ: [column tiles][n][16]
@@ -607,7 +706,11 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
   // the first adapter whose positions reach past `begin`; lane i holds the offsets of adapter e0 + i
   int g = n_adapters, e0 = 0, from = 0, upto = 0;
   auto look = [&]() { from = offsets[min(e0 + lane, n_adapters)], upto = offsets[min(e0 + lane + 1, n_adapters)]; };
-  for (; e0 < n_adapters; e0 += 64) {
+  if (s.direct) {  // all (two at most), those without rows too
+    look();
+    g = 0;
+  }
+  for (; g == n_adapters && e0 < n_adapters; e0 += 64) {
     look();
     const unsigned long long hit = __ballot(e0 + lane < n_adapters && upto > begin);
     if (hit) {
@@ -622,10 +725,14 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
     ta[i] = (uint32_t)(uintptr_t)(lds_void_ptr)lt + row * kRowBytes + (((wave * 4 + i) ^ (row & 7)) << 5) + (lr & 3) * 8;
   }
   int lo = g < n_adapters ? min(max(__builtin_amdgcn_readlane(from, g - e0), begin), end) : end;
-  for (; g < n_adapters && lo < end; ++g) {
+  for (; g < n_adapters && (lo < end || s.direct); ++g) {
     if (g - e0 == 64) e0 = g, look();
     const int hi = min(max(__builtin_amdgcn_readlane(upto, g - e0), lo), end);
-    if (hi == lo) continue;
+    if (hi == lo) {
+      if (s.direct == 1 && c0 + tid < s.d)
+        for (int r = 0; r < rank; ++r) s.part[((int64_t)g * rank + r) * s.d + c0 + tid] = 0.f;
+      continue;
+    }
     f32x4 acc[4][RT];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -784,7 +891,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         store_dz(stages - 1, false);
       }
     }
-    float* part = s.part + (int64_t)(split + g) * rank * s.d;
+    float* part = s.part + (int64_t)(s.direct ? g : split + g) * rank * s.d;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       const int r = j * 16 + lr;
@@ -792,7 +899,8 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = c0 + wave * 64 + i * 16 + lq * 4;
-        if (c < s.d) *reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c) = acc[i][j];
+        f32x4* to = reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c);
+        if (c < s.d) *to = s.direct == 2 ? *to + acc[i][j] : acc[i][j];
       }
     }
     lo = hi;
@@ -906,6 +1014,23 @@ static inline int outer_range(int64_t n, int n_adapters, int col_tiles, int rank
   return best;
 }
 
+// Few rows: column blocks of a wave (1 or 4) where both products run in one launch, 0 where they take one each.  All workgroups have to run at once, and d_in must not be long: the card
+// takes as long either way (1 row 4096 -> 4096 8.4 us in a graph against 8.8, 64 rows of 32 adapters 10.9 against 9.9, 1 row of 12288 columns 16.8 against 9.1), the host less (12.7 us a
+// call against 17.3).
+static inline int few_rows(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int rank) {
+  if (n > 64 || rank > 16 || d_in > 6144) return 0;
+  const int64_t tiles = max_tiles(n, n_adapters, 16);
+  return tiles * cdiv(d_out, 32 * kFewWaves) <= 256 ? 1 : tiles * cdiv(d_out, 128 * kFewWaves) <= 256 ? 4 : 0;
+}
+template <int BLOCKS>
+static void launch_few_rows(const void* x, int64_t ldx, const void* a, const void* b, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n, int n_adapters,
+                            int64_t d_in, int64_t d_out, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, float* z, hipStream_t stream) {
+  const int groups = (int)cdiv(d_out, 32 * kFewWaves * BLOCKS);
+  hipLaunchKernelGGL((few_rows_kernel<kFewWaves, BLOCKS>), dim3((unsigned)(max_tiles(n, n_adapters, 16) * groups)), dim3(kFewWaves * 64), 0, stream, (const bf16_t*)x, ldx,
+                     (const bf16_t*)a, (const bf16_t*)b, scales, offsets, row_ids, (int)n, n_adapters, (int)d_in, (int)d_out, rank, (const bf16_t*)base, ldb, (bf16_t*)out, ldo,
+                     base == out ? 1 : 0, groups, z);
+}
+
 template <int RT>
 static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, const void* w, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n,
                           int n_adapters, int d, int rank, float* z, hipStream_t stream) {
@@ -975,6 +1100,12 @@ static int check_rows(const char* who, const char* name, const void* p, int64_t 
   return PM_OK;
 }
 
+// whether two row tensors lie apart as a whole
+static bool apart(const void* p, int64_t ldp, int64_t dp, const void* q, int64_t ldq, int64_t dq, int64_t n) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return a + ((n - 1) * ldp + dp) * 2 <= b || b + ((n - 1) * ldq + dq) * 2 <= a;
+}
+
 }  // namespace lora
 }  // namespace pm
 
@@ -989,8 +1120,8 @@ using namespace pm::lora;
 
 extern "C" int64_t pm_lora_z_columns(int32_t rank) { return rank >= 1 && rank <= kMaxRank ? padded_rank(rank) : 0; }
 
-extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int32_t rank) {
-  if (n_rows <= 0 || rank < 1 || rank > kMaxRank) return 0;
+extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank) {
+  if (n_rows <= 0 || rank < 1 || rank > kMaxRank || few_rows(n_rows, n_adapters, d_in, d_out, rank)) return 0;
   const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true).parts;
   return parts > 1 ? (int64_t)parts * n_rows * padded_rank(rank) * 4 : 0;
 }
@@ -1007,12 +1138,20 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   if (base) PM_TRY(check_rows("pm_lora_fwd", "base", base, ldbase, d_out));
   PM_REQUIRE(base != out || ldbase == ldout, PM_ERR_INVALID_ARG, "pm_lora_fwd: base and out are the same rows with different strides");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
-  const ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true);
+  const int blocks = few_rows(n_rows, n_adapters, d_in, d_out, rank);
+  ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true);
+  if (blocks) plan.parts = 1, plan.chunks_per_part = (int)cdiv(d_in, kNarrowChunk);
   const int parts = plan.parts;
-  const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, rank);
+  const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, d_out, rank);
   PM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PM_ERR_WORKSPACE, "pm_lora_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)need);
   hipStream_t st = as_stream(stream);
+  if (blocks && apart(out, ldout, d_out, x, ldx, d_in, n_rows)) {  // every workgroup reads x to the end
+    auto launch = blocks == 1 ? launch_few_rows<1> : launch_few_rows<4>;
+    launch(x, ldx, a, b, scales, offsets, row_ids, n_rows, n_adapters, d_in, d_out, rank, base, ldbase, out, ldout, z, st);
+    PM_CHECK_LAUNCH("pm_lora_fwd");
+    return PM_OK;
+  }
   float* zs = parts > 1 ? (float*)workspace : z;
   PM_BY_RANK(rank, (launch_shrink<RT>(plan, x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, zs, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
@@ -1025,8 +1164,11 @@ namespace {
 // dz beside dB in one pass over grad_out pays from about 64 Mi elements of it, where the caches no longer hold it for the second pass (rank 16, all of the backward, two passes
 // against one: 16 384 rows 4096 -> 4096 155 and 149 us, -> 12288 259 and 215, 32 768 rows 449 and 371; 8192 rows 4096 -> 4096 92 and 97).
 constexpr int64_t kFusedElements = (int64_t)64 << 20;
+// Up to this many rows of one or two adapters outer runs in one range and writes the gradients itself, without partials and their join: it takes adapters one after the other
+// (64 rows of one adapter 4096 -> 4096: 22.6 -> 16.7 us in a graph; 100 rows of four: 26 -> 31).
+constexpr int64_t kDirectRows = 128;
 struct BwdPlan {
-  bool fused;
+  bool fused, direct;
   ShrinkPlan shrink;
   int tiles0, tiles1, range0, range1;
   int64_t dz_bytes, dz_parts_bytes, part0_bytes, part1_bytes;
@@ -1038,12 +1180,13 @@ BwdPlan bwd_plan(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int ran
   p.fused = factors && rank <= 16 && n * d_out >= kFusedElements;
   p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank, false);
   if (p.fused) p.shrink.parts = 1;
-  p.range0 = outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
+  p.direct = !p.fused && n <= kDirectRows && n_adapters <= 2;
+  p.range0 = p.direct ? (int)n : outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
   p.range1 = p.fused ? outer_range(n, n_adapters, p.tiles1, rank) : p.range0;
   p.dz_bytes = (int64_t)p.shrink.parts * n * rp * 4;
   p.dz_parts_bytes = p.fused ? (int64_t)p.tiles0 * n * rp * 4 : 0;
-  p.part0_bytes = factors ? (cdiv(n, p.range0) + n_adapters) * rank * d_out * 4 : 0;
-  p.part1_bytes = factors ? (cdiv(n, p.range1) + n_adapters) * rank * d_in * 4 : 0;
+  p.part0_bytes = factors && !p.direct ? (cdiv(n, p.range0) + n_adapters) * rank * d_out * 4 : 0;
+  p.part1_bytes = factors && !p.direct ? (cdiv(n, p.range1) + n_adapters) * rank * d_in * 4 : 0;
   return p;
 }
 }  // namespace
@@ -1069,6 +1212,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
   BwdPlan p{};
   p.range0 = p.range1 = 1;
   float *dz = (float*)ws, *dz_parts = nullptr, *part0 = nullptr, *part1 = nullptr;
+  int blocks = 0;  // of few_rows
   if (n_rows > 0) {
     PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
     PM_TRY(check_rows("pm_lora_bwd", "grad_out", grad_out, ldg, d_out));
@@ -1086,8 +1230,13 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     dz_parts = (float*)(ws + p.dz_bytes);
     part0 = (float*)(ws + p.dz_bytes + p.dz_parts_bytes);
     part1 = (float*)(ws + p.dz_bytes + p.dz_parts_bytes + p.part0_bytes);
-    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
-    const OuterSide s1{dz, p.shrink.parts, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
+    // outer reads x and grad_out after grad_x here
+    if (grad_x && apart(grad_x, ldgx, d_in, grad_out, ldg, d_out, n_rows) && (!grad_a || apart(grad_x, ldgx, d_in, x, ldx, d_in, n_rows)))
+      blocks = few_rows(n_rows, n_adapters, d_out, d_in, rank);
+    const int dz_count = blocks ? 1 : p.shrink.parts, direct = !p.direct ? 0 : accumulate ? 2 : 1;
+    if (direct) part0 = grad_b, part1 = grad_a;
+    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, direct, (const bf16_t*)b, scales, dz_parts};
+    const OuterSide s1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, direct, nullptr, nullptr, nullptr};
     const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
     if (p.fused) {
       launch_outer<1, true>(s0, s0, p.tiles0, p.tiles0, splits0, streamed(n_rows, d_out), offsets, row_ids, n_rows, n_adapters, rank, st);
@@ -1097,7 +1246,12 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
       launch_outer<1, false>(s1, s1, p.tiles1, p.tiles1, splits1, streamed(n_rows, d_in), offsets, row_ids, n_rows, n_adapters, rank, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
     } else {
-      PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
+      if (blocks) {
+        auto launch = blocks == 1 ? launch_few_rows<1> : launch_few_rows<4>;
+        launch(grad_out, ldg, b, a, scales, offsets, row_ids, n_rows, n_adapters, d_out, d_in, rank, base, ldbase, grad_x, ldgx, dz, st);
+      } else {
+        PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
+      }
       PM_CHECK_LAUNCH("pm_lora_bwd");
       if (grad_a) {
         PM_BY_RANK(rank, (launch_outer<RT, false>(s0, s1, p.tiles0, p.tiles0 + p.tiles1, splits0, streamed(n_rows, (d_in + d_out) / 2), offsets, row_ids, n_rows, n_adapters, rank, st)));
@@ -1105,13 +1259,13 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
       }
     }
   }
-  if (grad_a) {
+  if (grad_a && !p.direct) {
     const int64_t e0 = rank * d_out, e1 = rank * d_in;
     hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, p.range0, p.range1,
                        accumulate);
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
-  if (n_rows > 0 && grad_x) {
+  if (n_rows > 0 && grad_x && !blocks) {
     PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }

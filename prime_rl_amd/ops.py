@@ -1166,7 +1166,7 @@ def lora_fwd(x: Tensor, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, b
         if base is not None and not (base.data_ptr() == out.data_ptr() and ldb == ldo) and _share_memory(base, ldb, out, ldo):
             raise PrimeMI355XError("out overlaps base: it may be base itself or memory of its own")
     z = torch.empty((rows, (rank + 15) // 16 * 16), dtype=torch.float32, device=x.device)
-    nbytes = lib.pm_lora_fwd_workspace_bytes(rows, n, d_in, rank)
+    nbytes = lib.pm_lora_fwd_workspace_bytes(rows, n, d_in, d_out, rank)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None  # of its own for each call: a captured graph keeps it
     _launch(lib.pm_lora_fwd, "pm_lora_fwd", (x, a, b, scales, offsets, row_ids, base, out), x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), offsets.data_ptr(),
             _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb, out.data_ptr(), ldo, z.data_ptr(), _p(ws), nbytes)

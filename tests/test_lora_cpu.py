@@ -89,8 +89,9 @@ def test_a_backward_of_nothing_is_no_work(lib):
 
 def test_workspaces_follow_the_sizes(lib):
     assert [lib.pm_lora_z_columns(r) for r in (0, 1, 16, 17, 128, 129)] == [0, 16, 16, 32, 128, 0]
-    assert lib.pm_lora_fwd_workspace_bytes(0, 4, 4096, 16) == 0 and lib.pm_lora_fwd_workspace_bytes(16384, 4, 4096, 16) == 0  # enough rows: the long axis stays whole
-    assert lib.pm_lora_fwd_workspace_bytes(1, 1, 4096, 16) == 8 * 16 * 4  # one row: eight parts
+    assert lib.pm_lora_fwd_workspace_bytes(0, 4, 4096, 4096, 16) == 0 and lib.pm_lora_fwd_workspace_bytes(16384, 4, 4096, 4096, 16) == 0  # enough rows: the long axis stays whole
+    assert lib.pm_lora_fwd_workspace_bytes(1, 1, 4096, 4096, 16) == 0  # one row of not too many columns: one launch
+    assert lib.pm_lora_fwd_workspace_bytes(1, 1, 16384, 4096, 16) == 8 * 16 * 4  # of many: eight parts
     assert lib.pm_lora_bwd_workspace_bytes(0, 4, 4096, 4096, 16, 1) == 0 and lib.pm_lora_bwd_workspace_bytes(100, 4, 4096, 4096, 16, 1) > 100 * 16 * 4
 
 

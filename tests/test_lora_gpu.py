@@ -336,3 +336,50 @@ def test_lora_on_another_stream_and_in_graphs(ops):
         torch.cuda.synchronize()
         for graph, c, held in graphs:
             assert all(torch.equal(u, v) for u, v in zip(held, step(c))), turn
+
+
+FEW = [
+    ([1], 4096, 520, 16, 0, False),
+    ([1], 520, 4096, 16, 0, True),
+    ([0, 1, 0, 2], 72, 8, 5, 1, False),
+    ([16, 17, 31], 1032, 264, 16, 0, True),
+    ([64], 6144, 72, 1, 0, False),
+    ([0, 0, 5, 0], 328, 6144, 12, 3, True),
+    ([1] * 64, 264, 2056, 16, 0, True),
+    ([2] * 25, 512, 1024, 8, 14, False),
+    ([63], 64, 64, 16, 1, False),
+    ([1] * 70, 136, 128, 16, 2, True),  # more adapters than outer takes without partials
+    ([100, 28], 264, 136, 16, 0, True),  # outer alone without partials
+    ([50, 0, 70], 136, 264, 48, 8, False),
+    ([129], 72, 136, 16, 0, False),
+]
+
+
+@pytest.mark.parametrize("counts,d_in,d_out,rank,without,mixed", FEW)
+def test_lora_of_few_rows(ops, counts, d_in, d_out, rank, without, mixed):
+    c = _case(counts, d_in, d_out, rank, without, mixed, seed=9)
+    out, z = ops.lora_fwd(c["x"], c["a"], c["b"], c["scales"], c["offsets"], base=c["base"], row_ids=c["row_ids"])
+    _check_fwd(c, out, z)
+    grads = ops.lora_bwd(c["dy"], c["x"], z, c["a"], c["b"], c["scales"], c["offsets"], base=c["bx"], row_ids=c["row_ids"])
+    _check_bwd(c, z, *grads)
+    start = [torch.randn_like(g) for g in grads[1:]]
+    into = [t.clone() for t in start]
+    dx, *_ = ops.lora_bwd(c["dy"], c["x"], z, c["a"], c["b"], c["scales"], c["offsets"], base=c["bx"], row_ids=c["row_ids"], grad_a=into[0], grad_b=into[1], accumulate=True)
+    _check_bwd(c, z, dx, *into, *start)
+
+
+@pytest.mark.parametrize("n", [3, 40, 300])
+def test_lora_results_in_their_own_inputs_memory(ops, n):
+    """out over x, grad_x over grad_out or over x (d_in = d_out): read to the end before they are written."""
+    c = _case([n // 2, n - n // 2], 256, 256, 16, seed=4)
+    args = (c["a"], c["b"], c["scales"], c["offsets"])
+    out, z = ops.lora_fwd(c["x"], *args, base=c["base"])
+    x = c["x"].clone()
+    over, z2 = ops.lora_fwd(x, *args, base=c["base"], out=x)
+    assert over is x
+    _check_fwd(c, over, z2)
+    for name in ("dy", "x"):
+        t = {k: c[k].clone() for k in ("dy", "x")}
+        got = ops.lora_bwd(t["dy"], t["x"], z, *args, base=c["bx"], grad_x=t[name])
+        assert got[0] is t[name]
+        _check_bwd(c, z, *got)
