@@ -1159,15 +1159,15 @@ def lora_fwd(x: Tensor, a: Tensor, b: Tensor, scales: Tensor, offsets: Tensor, b
     ldx = _lora_rows(x, rows, d_in, "x")
     ldb = _lora_rows(base, rows, d_out, "base") if base is not None else 0
     if out is None:
-        out = torch.empty((rows, d_out), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty(rows, d_out)
         ldo = d_out
     else:
         ldo = _lora_rows(out, rows, d_out, "out")
         if base is not None and not (base.data_ptr() == out.data_ptr() and ldb == ldo) and _share_memory(base, ldb, out, ldo):
             raise PrimeMI355XError("out overlaps base: it may be base itself or memory of its own")
-    z = torch.empty((rows, (rank + 15) // 16 * 16), dtype=torch.float32, device=x.device)
+    z = scales.new_empty(rows, (rank + 15) // 16 * 16)
     nbytes = lib.pm_lora_fwd_workspace_bytes(rows, n, d_in, d_out, rank)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None  # of its own for each call: a captured graph keeps it
+    ws = scales.new_empty(nbytes >> 2) if nbytes else None  # of its own for each call: a captured graph keeps it
     _launch(lib.pm_lora_fwd, "pm_lora_fwd", (x, a, b, scales, offsets, row_ids, base, out), x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), offsets.data_ptr(),
             _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb, out.data_ptr(), ldo, z.data_ptr(), _p(ws), nbytes)
     return out, z
@@ -1194,7 +1194,7 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
         if (grad_a is None) != (grad_b is None) or (accumulate and grad_a is None):
             raise PrimeMI355XError("grad_a and grad_b go together, and accumulating needs them")
         if grad_a is None:
-            grad_a, grad_b = (torch.empty(t.shape, dtype=torch.float32, device=grad_out.device) for t in (a, b))
+            grad_a, grad_b = scales.new_empty(n, rank, d_in), scales.new_empty(n, rank, d_out)
         for t, of, nm in ((grad_a, a, "grad_a"), (grad_b, b, "grad_b")):
             _req(t, torch.float32, nm)
             if t.shape != of.shape:
@@ -1204,7 +1204,7 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
     if want_x:
         ldb = _lora_rows(base, rows, d_in, "base") if base is not None else 0
         if grad_x is None:
-            grad_x = torch.empty((rows, d_in), dtype=torch.bfloat16, device=grad_out.device)
+            grad_x = grad_out.new_empty(rows, d_in)
             ldgx = d_in
         else:
             ldgx = _lora_rows(grad_x, rows, d_in, "grad_x")
@@ -1213,7 +1213,7 @@ def lora_bwd(grad_out: Tensor, x: Tensor | None, z: Tensor | None, a: Tensor, b:
     else:
         base = grad_x = None
     nbytes = lib.pm_lora_bwd_workspace_bytes(rows, n, d_in, d_out, rank, 1 if want_factors else 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=grad_out.device) if nbytes else None
+    ws = scales.new_empty(nbytes >> 2) if nbytes else None
     _launch(lib.pm_lora_bwd, "pm_lora_bwd", (grad_out, x, z, a, b, scales, offsets, row_ids, base, grad_x, grad_a, grad_b), _p(grad_out), ldg, _p(x), ldx, _p(z), _p(a), _p(b), _p(scales), _p(offsets), _p(row_ids), rows, n, d_in, d_out, rank, _p(base), ldb,
             _p(grad_x), ldgx, _p(grad_a), _p(grad_b), 1 if accumulate else 0, _p(ws), nbytes)
     return grad_x, grad_a, grad_b
@@ -1229,7 +1229,7 @@ def lora_merge(weight: Tensor, a: Tensor, b: Tensor, scale: float, out: Tensor |
     (rank, d_in), d_out = a.shape, b.shape[1]
     ldw = _lora_rows(weight, d_out, d_in, "weight")
     if out is None:
-        out = torch.empty((d_out, d_in), dtype=torch.bfloat16, device=weight.device)
+        out = weight.new_empty(d_out, d_in)
         ldo = d_in
     else:
         ldo = _lora_rows(out, d_out, d_in, "out")
