@@ -340,6 +340,38 @@ __global__ __launch_bounds__(512) void shrink_wide_kernel(const bf16_t* __restri
       store_z(z + (int64_t)part * n * rp, acc[i][j] + red[(i * RT + j) * 64 + lane], p0 + (i * 4 + own) * 16 + lr, p1, j * 16 + lq * 4, rank, rp, scale);
 }
 
+// join: grad[adapter][r][c] (+)= the adapter's partials of outer, added in the order of its positions; zero for an adapter without rows.  A block of 256 threads takes 1024 elements.
+struct Join {
+  const float *part0, *part1;  // of grad_b and grad_a
+  float *grad0, *grad1;
+  int64_t elems0, elems1;  // of an adapter
+  const int32_t* offsets;
+  int n, range0, range1, accumulate, per_adapter;  // per_adapter: blocks
+};
+__device__ __forceinline__ void join(const Join& j, int block) {
+  const int g = block / j.per_adapter;
+  const int lo = min(max(j.offsets[g], 0), j.n), hi = min(max(j.offsets[g + 1], lo), j.n);
+  const int64_t at = ((int64_t)(block % j.per_adapter) * 256 + threadIdx.x) * 4;
+  if (at >= j.elems0 + j.elems1) return;
+  const bool second = at >= j.elems0;
+  const int64_t e = second ? at - j.elems0 : at, elems = second ? j.elems1 : j.elems0;
+  const int range = second ? j.range1 : j.range0;
+  const float* part = (second ? j.part1 : j.part0) + e;
+  float* grad = (second ? j.grad1 : j.grad0) + (int64_t)g * elems + e;
+  f32x4 v = j.accumulate ? *reinterpret_cast<const f32x4*>(grad) : f32x4{0.f, 0.f, 0.f, 0.f};
+  if (lo < hi) {
+    const int last = (hi - 1) / range;
+    for (int split = lo / range; split <= last; split += 8) {  // eight at a time in flight
+      f32x4 p[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) p[q] = split + q <= last ? *reinterpret_cast<const f32x4*>(part + (int64_t)(split + q + g) * elems) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += p[q];
+    }
+  }
+  *reinterpret_cast<f32x4*>(grad) = v;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // expand: out[row][c] = bf16(base[row][c] + sum_r z[p][r] * w[adapter][r][c]).
 // A workgroup takes 64 positions x COLS columns.  The factor tile [r][COLS] and z's two bf16 terms go through LDS into fragments; the factor is read transposed
@@ -348,7 +380,9 @@ __global__ __launch_bounds__(512) void shrink_wide_kernel(const bf16_t* __restri
 // base is asked for before anything waits.  It and out move row by row (512 bytes of a row and more in one instruction), and the products, 32 positions at a time, come through
 // LDS into that order, over the factor tile's place: accesses in the fragments' own order (16 rows x 64 bytes) reach 4.5 TB/s where these reach 5.5 (copies of 16 384 x 6144).
 // Column tiles run fastest, so that workgroups that run together cover whole rows (5.5 TB/s against 4.2 with row tiles fastest).
-// Without base the sum starts from zero; rows of no adapter get the base as it is.  MERGE: positions are the rows of a weight, z[p][r] = scale * zb[r][p] (bf16).
+// The backward's last launch is expand with join's blocks behind its own: they fill its end, and the host launches one kernel less.
+// Without base the sum starts from zero; rows of no adapter get the base as it is.  kMerge: positions are the rows of a weight, z[p][r] = scale * zb[r][p] (bf16).
+enum Expand { kForward, kBackward, kMerge };
 template <int RT>
 struct ExpandShape {
   static constexpr int kCols = RT <= 4 ? 256 : 128;
@@ -364,10 +398,17 @@ struct ExpandShape {
   static constexpr int kLds = kIn > kSums ? kIn : kSums;
 };
 
-template <int RT, bool MERGE>
+template <int RT, Expand KIND>
 __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict__ z, int parts, float* __restrict__ z_out, const bf16_t* __restrict__ zb, float merge_scale,
                                                         const bf16_t* __restrict__ w, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
-                                                        int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place, int stream) {
+                                                        int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place, int stream, unsigned own, Join j) {
+  constexpr bool MERGE = KIND == kMerge;
+  if constexpr (KIND == kBackward) {
+    if (blockIdx.x >= own) {
+      join(j, blockIdx.x - own);
+      return;
+    }
+  }
   using S = ExpandShape<RT>;
   __shared__ __attribute__((aligned(16))) unsigned char lds[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lq = lane >> 4;
@@ -922,31 +963,7 @@ __global__ __launch_bounds__(256) void sum_dz_kernel(const float* __restrict__ p
   *reinterpret_cast<f32x4*>(dz + at) = v;
 }
 
-// grad[adapter][r][c] (+)= the adapter's partials, added in the order of its positions; zero for an adapter without rows.
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part0, float* __restrict__ grad0, int64_t elems0, const float* __restrict__ part1,
-                                                   float* __restrict__ grad1, int64_t elems1, const int32_t* __restrict__ offsets, int n, int range0, int range1, int accumulate) {
-  const int g = blockIdx.y;
-  const int lo = min(max(offsets[g], 0), n), hi = min(max(offsets[g + 1], lo), n);
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= elems0 + elems1) return;
-  const bool second = at >= elems0;
-  const int64_t e = second ? at - elems0 : at, elems = second ? elems1 : elems0;
-  const int range = second ? range1 : range0;
-  const float* part = (second ? part1 : part0) + e;
-  float* grad = (second ? grad1 : grad0) + (int64_t)g * elems + e;
-  f32x4 v = accumulate ? *reinterpret_cast<const f32x4*>(grad) : f32x4{0.f, 0.f, 0.f, 0.f};
-  if (lo < hi) {
-    const int last = (hi - 1) / range;
-    for (int split = lo / range; split <= last; split += 8) {  // eight at a time in flight
-      f32x4 p[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) p[q] = split + q <= last ? *reinterpret_cast<const f32x4*>(part + (int64_t)(split + q + g) * elems) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v += p[q];
-    }
-  }
-  *reinterpret_cast<f32x4*>(grad) = v;
-}
+__global__ __launch_bounds__(256) void join_kernel(Join j) { join(j, blockIdx.x); }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // host side
@@ -1051,15 +1068,15 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
                        row_ids, (int)n, n_adapters, d, rank, padded_rank(rank), plan.rows, plan.depth, plan.parts, plan.chunks_per_part, streamed(n, d), z);
   }
 }
-template <int RT, bool MERGE>
+template <int RT, Expand KIND>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
-                          int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t stream) {
+                          int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, const Join& join, unsigned join_blocks, hipStream_t stream) {
   static_assert(ExpandShape<RT>::kCols == (RT <= 4 ? 256 : 128), "check_launch counts these");
-  const int64_t tiles = MERGE ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
+  const int64_t tiles = KIND == kMerge ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
   const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
-  hipLaunchKernelGGL((expand_kernel<RT, MERGE>), dim3(grid), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n, n_adapters,
-                     d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0,
-                     n * d >= (MERGE && base != out ? kStreamRows : kStreamBase) ? 1 : 0);
+  hipLaunchKernelGGL((expand_kernel<RT, KIND>), dim3(grid + join_blocks), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n,
+                     n_adapters, d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0,
+                     n * d >= (KIND == kMerge && base != out ? kStreamRows : kStreamBase) ? 1 : 0, grid, join);
 }
 template <int RT, bool DZ>
 static void launch_outer(const OuterSide& s0, const OuterSide& s1, int tiles0, int tiles01, unsigned splits, int stream, const int32_t* offsets, const int32_t* row_ids, int64_t n,
@@ -1086,11 +1103,11 @@ static int check_shape(const char* who, int64_t n, int64_t n_adapters, int64_t d
              "%s: d_in %lld, d_out %lld (multiples of 8, at most 2^22)", who, (long long)d_in, (long long)d_out);
   return PM_OK;
 }
-// a launch holds less than 2^32 threads; expand's is the largest
-static int check_launch(const char* who, int64_t tiles, int64_t d, int rank) {
+// a launch holds less than 2^32 threads; expand's (and join's behind it) is the largest
+static int check_launch(const char* who, int64_t tiles, int64_t d, int rank, int64_t join_elems) {
   const int64_t cols = rank <= 64 ? 256 : 128;
-  PM_REQUIRE(tiles * cdiv(d, cols) * 256 <= UINT32_MAX, PM_ERR_UNSUPPORTED, "%s: too many rows and columns for one call: %lld tiles of %d rows by %lld columns", who, (long long)tiles,
-             kExpandRows, (long long)d);
+  PM_REQUIRE((tiles * cdiv(d, cols) + join_elems / 1024) * 256 <= UINT32_MAX, PM_ERR_UNSUPPORTED, "%s: too many rows and columns for one call: %lld tiles of %d rows by %lld columns", who,
+             (long long)tiles, kExpandRows, (long long)d);
   return PM_OK;
 }
 static int check_rows(const char* who, const char* name, const void* p, int64_t ld, int64_t d) {
@@ -1131,7 +1148,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
                            int64_t workspace_bytes, void* stream) {
   PM_TRY(check_shape("pm_lora_fwd", n_rows, n_adapters, d_in, d_out, rank));
   if (n_rows == 0) return PM_OK;
-  PM_TRY(check_launch("pm_lora_fwd", max_tiles(n_rows, n_adapters, kExpandRows), d_out, rank));
+  PM_TRY(check_launch("pm_lora_fwd", max_tiles(n_rows, n_adapters, kExpandRows), d_out, rank, 0));
   PM_REQUIRE(a && b && scales && offsets && z, PM_ERR_INVALID_ARG, "pm_lora_fwd: null pointer");
   PM_TRY(check_rows("pm_lora_fwd", "x", x, ldx, d_in));
   PM_TRY(check_rows("pm_lora_fwd", "out", out, ldout, d_out));
@@ -1155,7 +1172,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   float* zs = parts > 1 ? (float*)workspace : z;
   PM_BY_RANK(rank, (launch_shrink<RT>(plan, x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, zs, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
-  PM_BY_RANK(rank, (launch_expand<RT, false>(zs, parts, parts > 1 ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, st)));
+  PM_BY_RANK(rank, (launch_expand<RT, kForward>(zs, parts, parts > 1 ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, Join{}, 0, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
   return PM_OK;
 }
@@ -1201,7 +1218,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
                            const int32_t* row_ids, int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank, const void* base, int64_t ldbase, void* grad_x,
                            int64_t ldgx, float* grad_a, float* grad_b, int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
   PM_TRY(check_shape("pm_lora_bwd", n_rows, n_adapters, d_in, d_out, rank));
-  PM_TRY(check_launch("pm_lora_bwd", max_tiles(n_rows, n_adapters, kExpandRows), d_in, rank));
+  PM_TRY(check_launch("pm_lora_bwd", max_tiles(n_rows, n_adapters, kExpandRows), d_in, rank, n_adapters * (rank * (d_in + d_out) + 1024)));
   PM_REQUIRE((grad_a != nullptr) == (grad_b != nullptr), PM_ERR_INVALID_ARG, "pm_lora_bwd: grad_a and grad_b go together");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z | (uintptr_t)grad_a | (uintptr_t)grad_b) & 15) == 0, PM_ERR_INVALID_ARG,
              "pm_lora_bwd: a, b, z, grad_a and grad_b must be 16-byte aligned");
@@ -1259,14 +1276,18 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
       }
     }
   }
+  Join join{};
+  unsigned join_blocks = 0;
   if (grad_a && !p.direct) {
-    const int64_t e0 = rank * d_out, e1 = rank * d_in;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)cdiv((e0 + e1) / 4, 256), n_adapters), dim3(256), 0, st, part0, grad_b, e0, part1, grad_a, e1, offsets, (int)n_rows, p.range0, p.range1,
-                       accumulate);
-    PM_CHECK_LAUNCH("pm_lora_bwd");
+    join = Join{part0, part1, grad_b, grad_a, rank * d_out, rank * d_in, offsets, (int)n_rows, p.range0, p.range1, accumulate, (int)cdiv(rank * (d_in + d_out) / 4, 256)};
+    join_blocks = (unsigned)join.per_adapter * n_adapters;
   }
   if (n_rows > 0 && grad_x && !blocks) {
-    PM_BY_RANK(rank, (launch_expand<RT, false>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, st)));
+    PM_BY_RANK(rank, (launch_expand<RT, kBackward>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, join,
+                                                   join_blocks, st)));
+    PM_CHECK_LAUNCH("pm_lora_bwd");
+  } else if (join_blocks) {
+    hipLaunchKernelGGL(join_kernel, dim3(join_blocks), dim3(256), 0, st, join);
     PM_CHECK_LAUNCH("pm_lora_bwd");
   }
   return PM_OK;
@@ -1275,12 +1296,12 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
 extern "C" int pm_lora_merge(const void* weight, int64_t ldw, const void* a, const void* b, float scale, int64_t d_in, int64_t d_out, int32_t rank, void* out, int64_t ldo,
                              void* stream) {
   PM_TRY(check_shape("pm_lora_merge", d_out, 1, d_in, d_out, rank));
-  PM_TRY(check_launch("pm_lora_merge", cdiv(d_out, kExpandRows), d_in, rank));
+  PM_TRY(check_launch("pm_lora_merge", cdiv(d_out, kExpandRows), d_in, rank, 0));
   PM_REQUIRE(a && b, PM_ERR_INVALID_ARG, "pm_lora_merge: null pointer");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_merge: a and b must be 16-byte aligned");
   PM_TRY(check_rows("pm_lora_merge", "weight", weight, ldw, d_in));
   PM_TRY(check_rows("pm_lora_merge", "out", out, ldo, d_in));
-  PM_BY_RANK(rank, (launch_expand<RT, true>(nullptr, 0, nullptr, b, scale, a, nullptr, nullptr, d_out, 1, (int)d_in, rank, weight, ldw, out, ldo, as_stream(stream))));
+  PM_BY_RANK(rank, (launch_expand<RT, kMerge>(nullptr, 0, nullptr, b, scale, a, nullptr, nullptr, d_out, 1, (int)d_in, rank, weight, ldw, out, ldo, Join{}, 0, as_stream(stream))));
   PM_CHECK_LAUNCH("pm_lora_merge");
   return PM_OK;
 }
