@@ -374,7 +374,7 @@ __device__ __forceinline__ void join(const Join& j, int block) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // expand: out[row][c] = bf16(base[row][c] + sum_r z[p][r] * w[adapter][r][c]).
-// A workgroup takes 64 positions x COLS columns.  The factor tile [r][COLS] and z's two bf16 terms go through LDS into fragments; the factor is read transposed
+// Rank <= 64: a workgroup takes 64 positions x 256 columns.  The factor tile [r][256] and z's two bf16 terms go through LDS into fragments; the factor is read transposed
 // (ds_read_b64_tr_b16), as the matrix cores' A operand, so that a lane ends up with 8 consecutive columns of one position.  At rank <= 16 both terms of z fit the
 // 32-deep contraction of one instruction (its two halves read the same 16 factor rows).
 // base is asked for before anything waits.  It and out move row by row (512 bytes of a row and more in one instruction), and the products, 32 positions at a time, come through
@@ -385,7 +385,7 @@ __device__ __forceinline__ void join(const Join& j, int block) {
 enum Expand { kForward, kBackward, kMerge };
 template <int RT>
 struct ExpandShape {
-  static constexpr int kCols = RT <= 4 ? 256 : 128;
+  static constexpr int kCols = 256;
   static constexpr int kZStride = RT * 32 + (RT == 4 ? 16 : 32);  // bytes of a row of z's terms (rank 64: three workgroups still fit a CU's LDS)
   static constexpr int kStride = kCols * 2 + 32;  // bytes; a row shift of 32 bytes spreads the 8 rows that a transposed read takes at once over all banks
   static constexpr int kSumStride = kCols * 4 + 32;
@@ -576,6 +576,132 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(v[q]) + sum[q >> 1][(q & 1) * 2], bf16hi(v[q]) + sum[q >> 1][(q & 1) * 2 + 1]);
       store(half * S::kMoves + m, o);
+    }
+  }
+}
+
+// The same for rank > 64.  There the LDS bounds it, and z's fragments are most of what goes through it: a wave keeps those of 32 positions in registers, straight from memory, and
+// takes the factor's tiles of 128 columns one after the other, which the four waves of a workgroup share.  Tiles come by DMA, one ahead; base and out move in the fragments' order.
+// 16 384 x 6144 at rank 128: 128 us against 216 in the way of smaller ranks (a copy takes 75); at rank 64 that way is the faster one (32 768 x 4096: 125 us against 164).
+constexpr int kDeepRows = 128, kDeepCols = 128;
+// the transposed fragments of 64 ranks at 8 columns (two halves of 4): rows of 256 bytes, [2 k][2 halves][16 rows, 16 more].  One block with its own wait: the compiler would wait for
+// the tile in flight before such a read.
+__device__ __forceinline__ void tr_read_deep(uint32_t a, u32x2 (&v)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:4096\n\tds_read_b64_tr_b16 %2, %8 offset:8\n\tds_read_b64_tr_b16 %3, %8 offset:4104\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:8192\n\tds_read_b64_tr_b16 %5, %8 offset:12288\n\tds_read_b64_tr_b16 %6, %8 offset:8200\n\tds_read_b64_tr_b16 %7, %8 offset:12296\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a)
+      : "memory");
+}
+template <int RT, Expand KIND>
+__global__ __launch_bounds__(256, 2) void expand_deep_kernel(const float* __restrict__ z, int parts, float* __restrict__ z_out, const bf16_t* __restrict__ zb, float merge_scale,
+                                                             const bf16_t* __restrict__ w, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                             int n_adapters, int d, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place,
+                                                             int steps, unsigned own, Join j) {
+  if constexpr (KIND == kBackward) {
+    if (blockIdx.x >= own) {
+      join(j, blockIdx.x - own);
+      return;
+    }
+  }
+  constexpr int kRowBytes = kDeepCols * 2, kTile = RT * 16 * kRowBytes, kDma = kTile / 4096, kSteps = RT / 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
+  const int all = (d + kDeepCols - 1) / kDeepCols, groups = (all + steps - 1) / steps, row_tile = blockIdx.x / groups, group = blockIdx.x % groups;
+  int adapter = 0, p0 = row_tile * kDeepRows, p1 = min(p0 + kDeepRows, n);
+  if constexpr (KIND != kMerge) {
+    if (!locate(offsets, n_adapters, n, kDeepRows, row_tile, lane, adapter, p0, p1)) return;
+    if (adapter < 0 && in_place) return;
+  }
+  const int first = group * steps, last = min(first + steps, all);
+  int pos[2], row[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int p = p0 + wave * 32 + g * 16 + lr;
+    pos[g] = p < p1 ? p : p0;
+  }
+  rows_of(row_ids, pos, n, row);
+  const bool in[2] = {p0 + wave * 32 + lr < p1, p0 + wave * 32 + 16 + lr < p1};
+  if (adapter < 0) {  // rows of no adapter
+    for (int c = first * kDeepCols + lq * 8; c < min(last * kDeepCols, d); c += 32)
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (in[g]) *reinterpret_cast<u32x4*>(out + (int64_t)row[g] * ldo + c) = base ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[g] * ldb + c) : u32x4{0, 0, 0, 0};
+    return;
+  }
+  // a DMA instruction brings 4 rows of 256 bytes; slot pairs of row r are permuted by r % 8.  Rows past the rank repeat the first (z is zero there), columns past the end are not stored.
+  const __amdgpu_buffer_rsrc_t factor = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(w + (int64_t)adapter * rank * d), 0, rank * d * 2, 0x00020000);
+  auto fetch = [&](int step, unsigned char* to) {
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      const int r = (i * 4 + wave) * 4 + lq, c = step * kDeepCols + (lr ^ ((r & 7) << 1)) * 8;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(factor, (lds_void_ptr)(to + (i * 4 + wave) * 1024), 16, ((r < rank ? r : 0) * d + (c < d ? c : 0)) * 2, 0, 0, 0);
+    }
+  };
+  fetch(first, lds);
+  u32x4 zf[2][kSteps][2];  // two bf16 terms of ranks 32 k + 4 lq .. and 16 more
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      u32x2 term[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = k * 32 + h * 16 + lq * 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (KIND == kMerge) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = r + q < rank && in[g] ? merge_scale * bf16_to_f32(zb[(int64_t)(r + q) * n + pos[g]]) : 0.f;
+        } else if (r < rp && in[g]) {
+          v = sum_parts(z + (int64_t)pos[g] * rp + r, (int64_t)n * rp, parts);
+          if (z_out && group == 0) *reinterpret_cast<f32x4*>(z_out + (int64_t)pos[g] * rp + r) = v;
+        }
+        term[0][h] = take_terms(v);
+        term[1][h] = to_bf16(v);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) zf[g][k][t] = u32x4{term[t][0].x, term[t][0].y, term[t][1].x, term[t][1].y};
+    }
+  for (int step = first; step < last; ++step) {
+    const uint32_t at = (uint32_t)(uintptr_t)(lds_void_ptr)lds + (step - first & 1) * kTile;
+    if (step == first) wait_dma(0);  // (the others have been waited for below)
+    lds_barrier();  // this tile is there for every wave, and every wave is done with the other one
+    if (step + 1 < last) fetch(step + 1, lds + (step + 1 - first & 1) * kTile);
+    u32x4 bv[kDeepCols / 32][2];
+#pragma unroll
+    for (int b = 0; b < kDeepCols / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int c = step * kDeepCols + b * 32 + lq * 8;
+        bv[b][g] = base && c < d && in[g] ? *reinterpret_cast<const u32x4*>(base + (int64_t)row[g] * ldb + c) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int b = 0; b < kDeepCols / 32; ++b) {
+      f32x4 acc[2][2] = {};
+      const int r = lq * 4 + (lr >> 2), slot = b * 4 + (lr & 3);
+      const uint32_t q = at + r * kRowBytes + (((slot >> 1) ^ (r & 7)) << 5) + (slot & 1) * 16;
+#pragma unroll
+      for (int k = 0; k < kSteps; k += 2) {
+        u32x2 v[8];
+        tr_read_deep(q + k * 32 * kRowBytes, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 1; t >= 0; --t)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) acc[g][i & 1] = mfma(u32x4{v[2 * i].x, v[2 * i].y, v[2 * i + 1].x, v[2 * i + 1].y}, zf[g][k + i / 2][t], acc[g][i & 1]);
+      }
+      if (b == 0) wait_dma(0);  // the next tile and the base, before the first store
+      const int c = step * kDeepCols + b * 32 + lq * 8;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        u32x4 o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(bv[b][g][q]) + acc[g][q >> 1][(q & 1) * 2], bf16hi(bv[b][g][q]) + acc[g][q >> 1][(q & 1) * 2 + 1]);
+        if (c < d && in[g]) *reinterpret_cast<u32x4*>(out + (int64_t)row[g] * ldo + c) = o;
+      }
     }
   }
 }
@@ -1071,12 +1197,26 @@ static void launch_shrink(const ShrinkPlan& plan, const void* t, int64_t ldt, co
 template <int RT, Expand KIND>
 static void launch_expand(const float* z, int parts, float* z_out, const void* zb, float merge_scale, const void* w, const int32_t* offsets, const int32_t* row_ids, int64_t n,
                           int n_adapters, int d, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, const Join& join, unsigned join_blocks, hipStream_t stream) {
-  static_assert(ExpandShape<RT>::kCols == (RT <= 4 ? 256 : 128), "check_launch counts these");
-  const int64_t tiles = KIND == kMerge ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
-  const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
-  hipLaunchKernelGGL((expand_kernel<RT, KIND>), dim3(grid + join_blocks), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids, (int)n,
-                     n_adapters, d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0,
-                     n * d >= (KIND == kMerge && base != out ? kStreamRows : kStreamBase) ? 1 : 0, grid, join);
+  if constexpr (RT > 4) {
+    const int64_t tiles = KIND == kMerge ? cdiv(n, kDeepRows) : max_tiles(n, n_adapters, kDeepRows);
+    const int all = (int)cdiv(d, kDeepCols);
+    // tiles of columns of a workgroup: the fewest rounds of 512, each as long as the tiles and one more for z (a weight of 6144 x 4096: 42 us, with one tile each 62)
+    int steps = 1;
+    double least = 0.0;
+    for (int k = 1; k <= all && k <= 64; ++k) {
+      const double cost = (double)cdiv(tiles * cdiv(all, k), 512) * (k + 1.0);
+      if (k == 1 || cost < least) least = cost, steps = k;
+    }
+    const unsigned grid = (unsigned)(tiles * cdiv(all, steps));
+    hipLaunchKernelGGL((expand_deep_kernel<RT, KIND>), dim3(grid + join_blocks), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids,
+                       (int)n, n_adapters, d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0, steps, grid, join);
+  } else {
+    const int64_t tiles = KIND == kMerge ? cdiv(n, kExpandRows) : max_tiles(n, n_adapters, kExpandRows);
+    const unsigned grid = (unsigned)(tiles * cdiv(d, ExpandShape<RT>::kCols));
+    hipLaunchKernelGGL((expand_kernel<RT, KIND>), dim3(grid + join_blocks), dim3(256), 0, stream, z, parts, z_out, (const bf16_t*)zb, merge_scale, (const bf16_t*)w, offsets, row_ids,
+                       (int)n, n_adapters, d, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0,
+                       n * d >= (KIND == kMerge && base != out ? kStreamRows : kStreamBase) ? 1 : 0, grid, join);
+  }
 }
 template <int RT, bool DZ>
 static void launch_outer(const OuterSide& s0, const OuterSide& s1, int tiles0, int tiles01, unsigned splits, int stream, const int32_t* offsets, const int32_t* row_ids, int64_t n,
