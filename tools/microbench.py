@@ -694,8 +694,8 @@ def main():
             cases += [(f"own fwd variant {v} ({d})", own_v(v)) for v, d in ((1, "one WG per tile"), (4, "no setprio"), (7, "balanced reads"), (13, "ABLATION no DMA"), (21, "ABLATION no reads"), (29, "ABLATION no DMA, no reads"),
                                                                              (68, "4-wave kernel, persistent"), (64, "4-wave kernel, one WG per tile"), (76, "4-wave ABLATION no DMA"),
                                                                              (84, "4-wave ABLATION no reads"), (92, "4-wave ABLATION no DMA, no reads"),
-                                                                             (132, "4-wave kernel, register staging"), (260, "4-wave kernel, fine schedule"), (268, "4-wave fine ABLATION no DMA"),
-                                                                             (276, "4-wave fine ABLATION no reads"), (7 + 512, "8-wave core, nt result stores"), (260 + 512, "4-wave fine, nt result stores"),
+                                                                             (132, "4-wave kernel, register staging"),
+                                                                             (7 + 512, "8-wave core, nt result stores"),
                                                                              (7 + 2048, "8-wave, DMA piece 0 before the reads"), (7 + 4096, "8-wave, both DMA pieces before the reads"),
                                                                              (7 + 32768, "8-wave, two-phase K-tile, W0 pre-read"), (5 + 32768, "8-wave, two-phase K-tile, plain"),
                                                                              (5 + 32768 + 65536, "8-wave, two-phase, sc0 DMA"), (5 + 32768 + 131072, "8-wave, two-phase, split B segment"),
