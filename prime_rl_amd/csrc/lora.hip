@@ -717,7 +717,9 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
                                                               int n_adapters, int d_in, int d_out, int rank, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place,
                                                               int groups, float* __restrict__ z) {
   constexpr int U = 4;
+  constexpr int kStride = BLOCKS * 64 + 32;  // bytes of a rank's columns in LDS; the shift as in expand
   __shared__ __attribute__((aligned(16))) f32x4 red[WAVES][64];
+  __shared__ __attribute__((aligned(16))) unsigned char lb[WAVES][16 * kStride];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
   const int group = blockIdx.x % groups;
   int adapter, p0, p1;
@@ -738,16 +740,12 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
       if (c0 + i * 32 + lq * 8 < d_out && p0 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[0] * ldo + c0 + i * 32 + lq * 8) = bv[i];
     return;
   }
-  bf16_t bf[BLOCKS][2][4];  // column 8 (lr / 4) + 4 h + lr % 4 of the block, ranks 4 lq .. 4 lq + 3
+  u32x4 stage[BLOCKS];  // this wave's columns of the other factor: 16 ranks, those past the last as zeros
 #pragma unroll
-  for (int i = 0; i < BLOCKS; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = lq * 4 + q, c = c0 + i * 32 + (lr >> 2) * 8 + h * 4 + (lr & 3);
-        bf[i][h][q] = r < rank && c < d_out ? b[((int64_t)adapter * rank + r) * d_out + c] : (bf16_t)0;
-      }
+  for (int i = 0; i < BLOCKS; ++i) {
+    const int piece = i * 64 + lane, r = piece / (BLOCKS * 4), c = c0 + piece % (BLOCKS * 4) * 8;
+    stage[i] = r < rank && c < d_out ? *reinterpret_cast<const u32x4*>(b + ((int64_t)adapter * rank + r) * d_out + c) : u32x4{0, 0, 0, 0};
+  }
   const float scale = scales[adapter];
   const bf16_t* xp = x + (int64_t)row[0] * ldx + lq * 8;
   const bf16_t* ap = a + ((int64_t)adapter * rank + (lr < rank ? lr : 0)) * d_in + lq * 8;  // ranks past the last repeat the first; what they give is not used
@@ -778,7 +776,12 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
     }
   }
   red[wave][lane] = acc;  // position lr, ranks 4 lq .. 4 lq + 3
-  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i) {
+    const int piece = i * 64 + lane;
+    *reinterpret_cast<u32x4*>(lb[wave] + piece / (BLOCKS * 4) * kStride + piece % (BLOCKS * 4) * 16) = stage[i];
+  }
+  lds_barrier();
   f32x4 v = red[0][lane];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) v += red[w][lane];
@@ -792,8 +795,8 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
     f32x4 sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = bf[i][h][0] | (uint32_t)bf[i][h][1] << 16, hi = bf[i][h][2] | (uint32_t)bf[i][h][3] << 16;
-      sum[h] = mfma(u32x4{lo, hi, lo, hi}, zf, f32x4{0.f, 0.f, 0.f, 0.f});
+      const u32x2 w = tr_read(lb[wave] + (lq * 4 + (lr >> 2)) * kStride + i * 64 + (lr & 3) * 16 + h * 8);  // column 8 (lr / 4) + 4 h + lr % 4 of the block
+      sum[h] = mfma(u32x4{w.x, w.y, w.x, w.y}, zf, f32x4{0.f, 0.f, 0.f, 0.f});
     }
     u32x4 o;
 #pragma unroll
@@ -1158,8 +1161,8 @@ static inline int outer_range(int64_t n, int n_adapters, int col_tiles, int rank
 }
 
 // Few rows: column blocks of a wave (1 or 4) where both products run in one launch, 0 where they take one each.  All workgroups have to run at once, and d_in must not be long: the card
-// takes as long either way (1 row 4096 -> 4096 8.4 us in a graph against 8.8, 64 rows of 32 adapters 10.9 against 9.9, 1 row of 12288 columns 16.8 against 9.1), the host less (12.7 us a
-// call against 17.3).
+// takes as long either way (in a graph 1 row 4096 -> 4096 7.9 us against 8.8, 64 rows of 32 adapters 9.0 against 9.9, 64 of one 10.9 against 10.4, but 1 row of 12288 columns 16.8 against
+// 9.1), the host less (11.8 us a call against 16.5).
 static inline int few_rows(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int rank) {
   if (n > 64 || rank > 16 || d_in > 6144) return 0;
   const int64_t tiles = max_tiles(n, n_adapters, 16);
