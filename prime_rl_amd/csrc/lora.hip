@@ -9,8 +9,11 @@
 //   forward  = shrink(x, A), expand(base, z, B);   backward: dz = shrink(dy, B), dx = expand(base_dx, dz, A), dB = outer(z, dy), dA = outer(dz, x)
 //   merge    = expand(W, s B^T, A) with the rows of W in the place of tokens.
 //
-// All of it is bound by HBM traffic of the row tensors up to rank 128 (2 r operations per 2-byte element, far under the MFMA rate), so each kernel makes one
-// pass over its row tensor with 16-byte accesses, and the matrix cores are there to keep the arithmetic out of the way.
+// All of it is bound by HBM traffic of the row tensors (2 r operations per 2-byte element, far under the MFMA rate), so each kernel makes one pass over its row
+// tensor with 16-byte accesses, and the matrix cores are there to keep the arithmetic out of the way.  From rank 64 on the LDS has as much to do as the memory.  Measured, in the
+// kernels' own time (a large copy moves 5.7 TB/s, a read past the caches 6.7):
+//   shrink  16 384 x 4096 rank 16 23 us = 5.8 TB/s, 32 768 x 12288 rank 64 143 us = 5.6;   expand  16 384 x 6144 rank 16 66 us = 6.1, 32 768 x 4096 rank 64 107 us = 5.0
+//   outer   16 384 x 4096 rank 16 28 us = 4.8, with dz 16 384 x 6144 48 us = 4.5 (and dz's parts), 32 768 x (12288 + 4096) rank 64 220 us = 4.9
 //
 // Numerics: z and dz are f32 in memory.  Where they feed the matrix cores they are split into bf16 terms that add up to the f32 value: two terms (16 bits)
 // in expand, whose result is rounded to bf16 (8 bits) anyway, three terms (24 bits: all of it) in outer, whose results are f32 gradients.  Everything else in
@@ -814,6 +817,8 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
 // The positions are the contraction, so both operands are read transposed (ds_read_b64_tr_b16).  Stages of 32 positions go through LDS: t by DMA, a ring of three deep
 // (16-byte slot pairs permuted by the row's number, so that the 8 rows of half a transposed read lie in different banks), z through registers, where it is split into
 // three bf16 planes.  A wave takes 64 columns and all ranks.
+// Bound at rank 16 by memory, less what a workgroup waits for its first stage (7 us) and the spread of the ends (a fifth); at rank 64 by the LDS and the matrix cores, of which z's three terms
+// take two thirds (with rows that lie in the caches 32 768 x 12288 takes 173 us, without 194).
 // DZ (rank <= 16, many rows): the same pass over dy also gives dz, so that dy is read once: the tile's 512 columns are contracted with the factor's (from registers), the
 // waves' results are added up through LDS while the next stage runs, and dz comes in one part for each column tile (6 % of the bytes of dy, written and read once).
 struct OuterSide {
@@ -1321,9 +1326,9 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
 }
 
 namespace {
-// dz beside dB in one pass over grad_out pays from about 64 Mi elements of it, where the caches no longer hold it for the second pass (rank 16, all of the backward, two passes
-// against one: 16 384 rows 4096 -> 4096 155 and 149 us, -> 12288 259 and 215, 32 768 rows 449 and 371; 8192 rows 4096 -> 4096 92 and 97).
-constexpr int64_t kFusedElements = (int64_t)64 << 20;
+// dz beside dB in one pass over grad_out pays from about 32 Mi elements of it (rank 16, all of the backward, two passes against one: 4096 rows 4096 -> 4096 48 and 51 us, 8192 rows 76 and
+// 74, 4096 rows 4096 -> 12288 76 and 67, 16 384 rows 212 and 171, 32 768 rows 389 and 317).
+constexpr int64_t kFusedElements = (int64_t)32 << 20;
 // Up to this many rows of one or two adapters outer runs in one range and writes the gradients itself, without partials and their join: it takes adapters one after the other
 // (64 rows of one adapter 4096 -> 4096: 22.6 -> 16.7 us in a graph; 100 rows of four: 26 -> 31).
 constexpr int64_t kDirectRows = 128;
