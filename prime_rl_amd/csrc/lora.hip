@@ -34,7 +34,6 @@ typedef __attribute__((address_space(1))) void* glb_void_ptr;
 constexpr int kMaxRank = 128;
 constexpr int64_t kMaxRows = (int64_t)1 << 28;
 constexpr int kExpandRows = 64;  // positions of one adapter per expand tile
-constexpr int kFewWaves = 8;     // of a few_rows workgroup
 constexpr int kOuterCols = 512;  // columns of an outer workgroup
 
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -710,19 +709,20 @@ __global__ __launch_bounds__(256, 2) void expand_deep_kernel(const float* __rest
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// shrink and expand in one launch, for few rows (a token or a few for each adapter) and rank <= 16, where launches are what counts: the forward, and the backward's dz and grad_x.
-// A workgroup takes up to 16 positions of one adapter and 32 BLOCKS columns of out for each of its waves.  It contracts the whole of d_in itself (a wave takes every WAVES-th
+// shrink and expand in one launch, for few rows (a token or a few for each adapter) and rank <= 64, where launches are what counts: the forward, and the backward's dz and grad_x.
+// A workgroup takes up to 16 positions of one adapter and 32 BLOCKS columns of out for each of its eight waves.  It contracts the whole of d_in itself (a wave takes every eighth
 // 64 columns, fragments straight from global memory), though all workgroups of the tile do the same: the factor comes from L2 faster than a second launch would start.  Its share of
 // the other factor and the base are asked for before that, and each lane adds the waves' results up in the layout that the second product takes.
-template <int WAVES, int BLOCKS>
-__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __restrict__ x, int64_t ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b,
-                                                              const float* __restrict__ scales, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
-                                                              int n_adapters, int d_in, int d_out, int rank, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo, int in_place,
-                                                              int groups, float* __restrict__ z) {
-  constexpr int U = 4;
+constexpr int kFewWaves = 8;
+template <int RT, int BLOCKS>
+__global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(const bf16_t* __restrict__ x, int64_t ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b,
+                                                                  const float* __restrict__ scales, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                                  int n_adapters, int d_in, int d_out, int rank, int rp, const bf16_t* base, int64_t ldb, bf16_t* out, int64_t ldo,
+                                                                  int in_place, int groups, float* __restrict__ z) {
+  constexpr int W = kFewWaves, U = RT == 1 ? 4 : 2, kSteps = (RT + 1) / 2;
   constexpr int kStride = BLOCKS * 64 + 32;  // bytes of a rank's columns in LDS; the shift as in expand
-  __shared__ __attribute__((aligned(16))) f32x4 red[WAVES][64];
-  __shared__ __attribute__((aligned(16))) unsigned char lb[WAVES][16 * kStride];
+  __shared__ __attribute__((aligned(16))) f32x4 red[W][RT][64];
+  __shared__ __attribute__((aligned(16))) unsigned char lb[W][RT * 16 * kStride];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lq = lane >> 4;
   const int group = blockIdx.x % groups;
   int adapter, p0, p1;
@@ -730,7 +730,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
   const int pos[1] = {p0 + lr < p1 ? p0 + lr : p0};
   int row[1];
   rows_of(row_ids, pos, n, row);
-  const int c0 = (group * WAVES + wave) * 32 * BLOCKS;
+  const int c0 = (group * W + wave) * 32 * BLOCKS;
   u32x4 bv[BLOCKS];
 #pragma unroll
   for (int i = 0; i < BLOCKS; ++i) {
@@ -743,64 +743,90 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const bf16_t* __re
       if (c0 + i * 32 + lq * 8 < d_out && p0 + lr < p1) *reinterpret_cast<u32x4*>(out + (int64_t)row[0] * ldo + c0 + i * 32 + lq * 8) = bv[i];
     return;
   }
-  u32x4 stage[BLOCKS];  // this wave's columns of the other factor: 16 ranks, those past the last as zeros
+  u32x4 stage[RT * BLOCKS];  // this wave's columns of the other factor, ranks past the last as zeros
 #pragma unroll
-  for (int i = 0; i < BLOCKS; ++i) {
+  for (int i = 0; i < RT * BLOCKS; ++i) {
     const int piece = i * 64 + lane, r = piece / (BLOCKS * 4), c = c0 + piece % (BLOCKS * 4) * 8;
     stage[i] = r < rank && c < d_out ? *reinterpret_cast<const u32x4*>(b + ((int64_t)adapter * rank + r) * d_out + c) : u32x4{0, 0, 0, 0};
   }
   const float scale = scales[adapter];
   const bf16_t* xp = x + (int64_t)row[0] * ldx + lq * 8;
-  const bf16_t* ap = a + ((int64_t)adapter * rank + (lr < rank ? lr : 0)) * d_in + lq * 8;  // ranks past the last repeat the first; what they give is not used
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const bf16_t* ap[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j)  // ranks past the last repeat the first; what they give is not used
+    ap[j] = a + ((int64_t)adapter * rank + (j * 16 + lr < rank ? j * 16 + lr : 0)) * d_in + lq * 8;
+  f32x4 acc[RT];
+#pragma unroll
+  for (int j = 0; j < RT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int full = d_in >> 6;
   int s = wave;
-  for (; s + WAVES * (U - 1) < full; s += WAVES * U) {
-    u32x4 xf[U][2], af[U][2];
+  for (; s + W * (U - 1) < full; s += W * U) {
+    u32x4 xf[U][2], af[U][2][RT];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        xf[u][h] = *reinterpret_cast<const u32x4*>(xp + (s + WAVES * u) * 64 + h * 32);
-        af[u][h] = *reinterpret_cast<const u32x4*>(ap + (s + WAVES * u) * 64 + h * 32);
+        xf[u][h] = *reinterpret_cast<const u32x4*>(xp + (s + W * u) * 64 + h * 32);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) af[u][h][j] = *reinterpret_cast<const u32x4*>(ap[j] + (s + W * u) * 64 + h * 32);
       }
     __builtin_amdgcn_sched_barrier(0);  // all of them in flight
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc = mfma(af[u][h], xf[u][h], acc);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[j] = mfma(af[u][h][j], xf[u][h], acc[j]);
   }
-  for (; s * 64 < d_in; s += WAVES) {  // what is left, columns past the end as zeros on both sides
+  for (; s * 64 < d_in; s += W) {  // what is left, columns past the end as zeros on both sides
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = s * 64 + h * 32;
       const bool in = k + lq * 8 < d_in;
-      acc = mfma(in ? *reinterpret_cast<const u32x4*>(ap + k) : u32x4{0, 0, 0, 0}, in ? *reinterpret_cast<const u32x4*>(xp + k) : u32x4{0, 0, 0, 0}, acc);
+      const u32x4 xf = in ? *reinterpret_cast<const u32x4*>(xp + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < RT; ++j) acc[j] = mfma(in ? *reinterpret_cast<const u32x4*>(ap[j] + k) : u32x4{0, 0, 0, 0}, xf, acc[j]);
     }
   }
-  red[wave][lane] = acc;  // position lr, ranks 4 lq .. 4 lq + 3
 #pragma unroll
-  for (int i = 0; i < BLOCKS; ++i) {
+  for (int j = 0; j < RT; ++j) red[wave][j][lane] = acc[j];  // position lr, ranks 16 j + 4 lq .. 4 lq + 3
+#pragma unroll
+  for (int i = 0; i < RT * BLOCKS; ++i) {
     const int piece = i * 64 + lane;
     *reinterpret_cast<u32x4*>(lb[wave] + piece / (BLOCKS * 4) * kStride + piece % (BLOCKS * 4) * 16) = stage[i];
   }
   lds_barrier();
-  f32x4 v = red[0][lane];
+  u32x2 term[2][RT];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) v += red[w][lane];
+  for (int j = 0; j < RT; ++j) {
+    f32x4 v = red[0][j][lane];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) v[q] = lq * 4 + q < rank ? v[q] * scale : 0.f;
-  if (group == 0 && wave == 0 && p0 + lr < p1) *reinterpret_cast<f32x4*>(z + (int64_t)(p0 + lr) * 16 + lq * 4) = v;
-  const u32x2 lead = take_terms(v), rest = to_bf16(v);
-  const u32x4 zf = {lead.x, lead.y, rest.x, rest.y};
+    for (int w = 1; w < W; ++w) v += red[w][j][lane];
+    const int r = j * 16 + lq * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = r + q < rank ? v[q] * scale : 0.f;
+    if (group == 0 && wave == 0 && p0 + lr < p1 && r < rp) *reinterpret_cast<f32x4*>(z + (int64_t)(p0 + lr) * rp + r) = v;
+    term[0][j] = take_terms(v);
+    term[1][j] = to_bf16(v);
+  }
 #pragma unroll
   for (int i = 0; i < BLOCKS; ++i) {
-    f32x4 sum[2];
+    f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x2 w = tr_read(lb[wave] + (lq * 4 + (lr >> 2)) * kStride + i * 64 + (lr & 3) * 16 + h * 8);  // column 8 (lr / 4) + 4 h + lr % 4 of the block
-      sum[h] = mfma(u32x4{w.x, w.y, w.x, w.y}, zf, f32x4{0.f, 0.f, 0.f, 0.f});
-    }
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* at = lb[wave] + (k * 32 + lq * 4 + (lr >> 2)) * kStride + i * 64 + (lr & 3) * 16 + h * 8;  // column 8 (lr / 4) + 4 h + lr % 4 of the block
+        const u32x2 lo = tr_read(at);
+        if constexpr (RT == 1) {  // both terms in one instruction
+          sum[h] = mfma(u32x4{lo.x, lo.y, lo.x, lo.y}, u32x4{term[0][0].x, term[0][0].y, term[1][0].x, term[1][0].y}, sum[h]);
+        } else {
+          const u32x2 hi = tr_read(at + 16 * kStride);
+#pragma unroll
+          for (int t = 1; t >= 0; --t)
+            sum[h] = mfma(u32x4{lo.x, lo.y, hi.x, hi.y}, u32x4{term[t][2 * k].x, term[t][2 * k].y, term[t][2 * k + 1].x, term[t][2 * k + 1].y}, sum[h]);
+        }
+      }
     u32x4 o;
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q] = pack_bf16_hw(bf16lo(bv[i][q]) + sum[q >> 1][(q & 1) * 2], bf16hi(bv[i][q]) + sum[q >> 1][(q & 1) * 2 + 1]);
@@ -1165,21 +1191,21 @@ static inline int outer_range(int64_t n, int n_adapters, int col_tiles, int rank
   return best;
 }
 
-// Few rows: column blocks of a wave (1 or 4) where both products run in one launch, 0 where they take one each.  All workgroups have to run at once, and d_in must not be long: the card
-// takes as long either way (in a graph 1 row 4096 -> 4096 7.9 us against 8.8, 64 rows of 32 adapters 9.0 against 9.9, 64 of one 10.9 against 10.4, but 1 row of 12288 columns 16.8 against
-// 9.1), the host less (11.8 us a call against 16.5).
+// Few rows: column blocks of a wave (1 or 4) where both products run in one launch, 0 where they take one each.  All workgroups have to run at once, and what each reads of the first
+// factor must not be much: the card takes about as long either way (in a graph: 1 row 4096 -> 4096 rank 16 7.9 us against 8.8, 64 rows of 32 adapters 9.0 against 9.9, 64 of one 10.9
+// against 10.4, 32 rows 2048 -> 8192 rank 20 7.7 against 10.2; but 1 row of 12288 columns rank 16 16.8 against 9.1, of 4096 rank 64 19.6 against 12.0), the host less (11.5 us a call
+// against 16.3).
 static inline int few_rows(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int rank) {
-  if (n > 64 || rank > 16 || d_in > 6144) return 0;
+  if (n > 64 || rank > 64 || rank_tiles(rank) * 16 * d_in > 96 << 10) return 0;
   const int64_t tiles = max_tiles(n, n_adapters, 16);
-  return tiles * cdiv(d_out, 32 * kFewWaves) <= 256 ? 1 : tiles * cdiv(d_out, 128 * kFewWaves) <= 256 ? 4 : 0;
+  return tiles * cdiv(d_out, 32 * kFewWaves) <= 256 ? 1 : rank <= 32 && tiles * cdiv(d_out, 128 * kFewWaves) <= 256 ? 4 : 0;
 }
-template <int BLOCKS>
-static void launch_few_rows(const void* x, int64_t ldx, const void* a, const void* b, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n, int n_adapters,
-                            int64_t d_in, int64_t d_out, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, float* z, hipStream_t stream) {
-  const int groups = (int)cdiv(d_out, 32 * kFewWaves * BLOCKS);
-  hipLaunchKernelGGL((few_rows_kernel<kFewWaves, BLOCKS>), dim3((unsigned)(max_tiles(n, n_adapters, 16) * groups)), dim3(kFewWaves * 64), 0, stream, (const bf16_t*)x, ldx,
-                     (const bf16_t*)a, (const bf16_t*)b, scales, offsets, row_ids, (int)n, n_adapters, (int)d_in, (int)d_out, rank, (const bf16_t*)base, ldb, (bf16_t*)out, ldo,
-                     base == out ? 1 : 0, groups, z);
+static void launch_few_rows(int blocks, const void* x, int64_t ldx, const void* a, const void* b, const float* scales, const int32_t* offsets, const int32_t* row_ids, int64_t n,
+                            int n_adapters, int64_t d_in, int64_t d_out, int rank, const void* base, int64_t ldb, void* out, int64_t ldo, float* z, hipStream_t stream) {
+  const int groups = (int)cdiv(d_out, 32 * kFewWaves * blocks);
+  auto kernel = rank <= 16 ? (blocks == 1 ? few_rows_kernel<1, 1> : few_rows_kernel<1, 4>) : rank <= 32 ? (blocks == 1 ? few_rows_kernel<2, 1> : few_rows_kernel<2, 4>) : few_rows_kernel<4, 1>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(max_tiles(n, n_adapters, 16) * groups)), dim3(kFewWaves * 64), 0, stream, (const bf16_t*)x, ldx, (const bf16_t*)a, (const bf16_t*)b, scales,
+                     offsets, row_ids, (int)n, n_adapters, (int)d_in, (int)d_out, rank, padded_rank(rank), (const bf16_t*)base, ldb, (bf16_t*)out, ldo, base == out ? 1 : 0, groups, z);
 }
 
 template <int RT>
@@ -1305,15 +1331,14 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
   const int blocks = few_rows(n_rows, n_adapters, d_in, d_out, rank);
   ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true);
-  if (blocks) plan.parts = 1, plan.chunks_per_part = (int)cdiv(d_in, kNarrowChunk);
+  if (blocks) plan.parts = 1, plan.chunks_per_part = (int)cdiv(d_in, rank <= 16 ? kNarrowChunk : kWideChunk);
   const int parts = plan.parts;
   const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, d_out, rank);
   PM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), PM_ERR_WORKSPACE, "pm_lora_fwd: workspace of %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)need);
   hipStream_t st = as_stream(stream);
   if (blocks && apart(out, ldout, d_out, x, ldx, d_in, n_rows)) {  // every workgroup reads x to the end
-    auto launch = blocks == 1 ? launch_few_rows<1> : launch_few_rows<4>;
-    launch(x, ldx, a, b, scales, offsets, row_ids, n_rows, n_adapters, d_in, d_out, rank, base, ldbase, out, ldout, z, st);
+    launch_few_rows(blocks, x, ldx, a, b, scales, offsets, row_ids, n_rows, n_adapters, d_in, d_out, rank, base, ldbase, out, ldout, z, st);
     PM_CHECK_LAUNCH("pm_lora_fwd");
     return PM_OK;
   }
@@ -1412,8 +1437,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
       PM_CHECK_LAUNCH("pm_lora_bwd");
     } else {
       if (blocks) {
-        auto launch = blocks == 1 ? launch_few_rows<1> : launch_few_rows<4>;
-        launch(grad_out, ldg, b, a, scales, offsets, row_ids, n_rows, n_adapters, d_out, d_in, rank, base, ldbase, grad_x, ldgx, dz, st);
+        launch_few_rows(blocks, grad_out, ldg, b, a, scales, offsets, row_ids, n_rows, n_adapters, d_out, d_in, rank, base, ldbase, grad_x, ldgx, dz, st);
       } else {
         PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
       }

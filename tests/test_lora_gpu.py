@@ -348,6 +348,10 @@ FEW = [
     ([1] * 64, 264, 2056, 16, 0, True),
     ([2] * 25, 512, 1024, 8, 14, False),
     ([63], 64, 64, 16, 1, False),
+    ([3, 20, 0, 17], 520, 1032, 32, 2, True),
+    ([1, 0, 2], 4096, 520, 48, 1, False),
+    ([30, 9], 72, 4096, 64, 0, True),
+    ([1] * 40, 136, 2056, 20, 0, False),
     ([1] * 70, 136, 128, 16, 2, True),  # more adapters than outer takes without partials
     ([100, 28], 264, 136, 16, 0, True),  # outer alone without partials
     ([50, 0, 70], 136, 264, 48, 8, False),
