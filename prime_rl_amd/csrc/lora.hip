@@ -855,7 +855,6 @@ struct OuterSide {
   int d;
   float* part;         // [ranges + adapters][rank][d]
   int range;           // positions of a workgroup
-  int direct;          // 1: one range, `part` is the gradient itself; 2: it is added to
   const bf16_t* w;     // DZ: the factor and scales of dz
   const float* scales;
   float* dz;           // DZ: [column tiles][n][16]
@@ -907,11 +906,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
   // the first adapter whose positions reach past `begin`; lane i holds the offsets of adapter e0 + i
   int g = n_adapters, e0 = 0, from = 0, upto = 0;
   auto look = [&]() { from = offsets[min(e0 + lane, n_adapters)], upto = offsets[min(e0 + lane + 1, n_adapters)]; };
-  if (s.direct) {  // all (two at most), those without rows too
-    look();
-    g = 0;
-  }
-  for (; g == n_adapters && e0 < n_adapters; e0 += 64) {
+  for (; e0 < n_adapters; e0 += 64) {
     look();
     const unsigned long long hit = __ballot(e0 + lane < n_adapters && upto > begin);
     if (hit) {
@@ -926,14 +921,10 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
     ta[i] = (uint32_t)(uintptr_t)(lds_void_ptr)lt + row * kRowBytes + (((wave * 4 + i) ^ (row & 7)) << 5) + (lr & 3) * 8;
   }
   int lo = g < n_adapters ? min(max(__builtin_amdgcn_readlane(from, g - e0), begin), end) : end;
-  for (; g < n_adapters && (lo < end || s.direct); ++g) {
+  for (; g < n_adapters && lo < end; ++g) {
     if (g - e0 == 64) e0 = g, look();
     const int hi = min(max(__builtin_amdgcn_readlane(upto, g - e0), lo), end);
-    if (hi == lo) {
-      if (s.direct == 1 && c0 + tid < s.d)
-        for (int r = 0; r < rank; ++r) s.part[((int64_t)g * rank + r) * s.d + c0 + tid] = 0.f;
-      continue;
-    }
+    if (hi == lo) continue;
     f32x4 acc[4][RT];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -1092,7 +1083,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         store_dz(stages - 1, false);
       }
     }
-    float* part = s.part + (int64_t)(s.direct ? g : split + g) * rank * s.d;
+    float* part = s.part + (int64_t)(split + g) * rank * s.d;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
       const int r = j * 16 + lr;
@@ -1100,11 +1091,89 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = c0 + wave * 64 + i * 16 + lq * 4;
-        f32x4* to = reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c);
-        if (c < s.d) *to = s.direct == 2 ? *to + acc[i][j] : acc[i][j];
+        if (c < s.d) *reinterpret_cast<f32x4*>(part + (int64_t)r * s.d + c) = acc[i][j];
       }
     }
     lo = hi;
+  }
+}
+
+// The same for few rows, where the stages' latency is all there is: a workgroup takes 128 columns and 16 ranks of one adapter, in f32 arithmetic, and writes the gradient itself.  z's rows
+// lie in LDS (32 instructions for each position); its waves (four, or one where adapters have few rows each) take eight rows of t in turn, asked for together, and
+// their sums are added up through LDS.  64 rows 4096 -> 4096 rank 16, all of the backward in a graph: of one adapter 19.0 us against outer's 22.0 (with one wave 28), of 64 14.8 against 29.1
+// (with four waves 21.5); 100 rows of four adapters 16.4 against 23.5, of one 22.4 against 20.3.
+constexpr int kFewOuterRows = 128;
+struct FewSide {
+  const float* z;  // [parts][n][rp]
+  int parts;
+  const bf16_t* t;
+  int64_t ldt;
+  int d;
+  float* grad;  // [adapters][rank][d]
+};
+template <int W>
+__global__ __launch_bounds__(W * 64) void outer_few_kernel(FewSide s0, FewSide s1, int tiles0, int tiles01, const int32_t* __restrict__ offsets, const int32_t* __restrict__ row_ids, int n,
+                                                       int rank, int rp, int accumulate) {
+  __shared__ __attribute__((aligned(16))) f32x4 lz[kFewOuterRows][4];
+  __shared__ float red[W > 1 ? W - 1 : 1][W > 1 ? 32 : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = blockIdx.y, rank0 = (int)(blockIdx.x / tiles01) * 16, tile = blockIdx.x % tiles01;
+  const FewSide s = tile >= tiles0 ? s1 : s0;
+  const int c = (tile >= tiles0 ? tile - tiles0 : tile) * 128 + lane * 2;
+  const int lo = min(max(offsets[g], 0), n), hi = min(max(offsets[g + 1], lo), n);
+  float* const grad = s.grad + ((int64_t)g * rank + rank0) * s.d + c;
+  const int ranks = min(16, rank - rank0);
+  if (lo == hi) {
+    if (!accumulate && c < s.d)
+      for (int r = wave; r < ranks; r += W) *reinterpret_cast<float2*>(grad + (int64_t)r * s.d) = float2{0.f, 0.f};
+    return;
+  }
+  for (int i = threadIdx.x; i < (hi - lo) * 4; i += W * 64) lz[i >> 2][i & 3] = sum_parts(s.z + (int64_t)(lo + (i >> 2)) * rp + rank0 + (i & 3) * 4, (int64_t)n * rp, s.parts);
+  lds_barrier();
+  float acc[16][2];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r][0] = acc[r][1] = 0.f;
+  const bf16_t* const t = s.t + (c < s.d ? c : 0);
+  for (int p = lo + wave * 8; p < hi; p += W * 8) {
+    int pos[8], row[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pos[i] = min(p + i, hi - 1);
+    rows_of(row_ids, pos, n, row);
+    uint32_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const uint32_t*>(t + (int64_t)row[i] * s.ldt);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (p + i >= hi) break;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 z = lz[p - lo + i][q];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[q * 4 + r][0] = fmaf(z[r], bf16lo(v[i]), acc[q * 4 + r][0]);
+          acc[q * 4 + r][1] = fmaf(z[r], bf16hi(v[i]), acc[q * 4 + r][1]);
+        }
+      }
+    }
+  }
+  if constexpr (W > 1) {
+    const int sums = min((hi - lo - 1) >> 3, W - 1);  // waves behind the first that had rows
+    if (wave && wave <= sums)
+#pragma unroll
+      for (int r = 0; r < 32; ++r) red[wave - 1][r][lane] = acc[r >> 1][r & 1];
+    lds_barrier();
+    if (wave) return;
+    for (int w = 0; w < sums; ++w)
+#pragma unroll
+      for (int r = 0; r < 32; ++r) acc[r >> 1][r & 1] += red[w][r][lane];
+  }
+  if (c < s.d) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (r < ranks) {
+        float2* to = reinterpret_cast<float2*>(grad + (int64_t)r * s.d);
+        const float2 old = accumulate ? *to : float2{0.f, 0.f};
+        *to = float2{old.x + acc[r][0], old.y + acc[r][1]};
+      }
   }
 }
 
@@ -1354,11 +1423,9 @@ namespace {
 // dz beside dB in one pass over grad_out pays from about 32 Mi elements of it (rank 16, all of the backward, two passes against one: 4096 rows 4096 -> 4096 48 and 51 us, 8192 rows 76 and
 // 74, 4096 rows 4096 -> 12288 76 and 67, 16 384 rows 212 and 171, 32 768 rows 389 and 317).
 constexpr int64_t kFusedElements = (int64_t)32 << 20;
-// Up to this many rows of one or two adapters outer runs in one range and writes the gradients itself, without partials and their join: it takes adapters one after the other
-// (64 rows of one adapter 4096 -> 4096: 22.6 -> 16.7 us in a graph; 100 rows of four: 26 -> 31).
-constexpr int64_t kDirectRows = 128;
+static inline int64_t few_tiles(int64_t d_in, int64_t d_out, int rank) { return (cdiv(d_out, 128) + cdiv(d_in, 128)) * (padded_rank(rank) / 16); }
 struct BwdPlan {
-  bool fused, direct;
+  bool fused, few;  // few: outer_few
   ShrinkPlan shrink;
   int tiles0, tiles1, range0, range1;
   int64_t dz_bytes, dz_parts_bytes, part0_bytes, part1_bytes;
@@ -1370,13 +1437,13 @@ BwdPlan bwd_plan(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int ran
   p.fused = factors && rank <= 16 && n * d_out >= kFusedElements;
   p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank, false);
   if (p.fused) p.shrink.parts = 1;
-  p.direct = !p.fused && n <= kDirectRows && n_adapters <= 2;
-  p.range0 = p.direct ? (int)n : outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
+  p.few = !p.fused && n <= (n_adapters > 1 ? kFewOuterRows : kFewOuterRows / 2) && few_tiles(d_in, d_out, rank) * n_adapters <= 1 << 20;
+  p.range0 = outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
   p.range1 = p.fused ? outer_range(n, n_adapters, p.tiles1, rank) : p.range0;
   p.dz_bytes = (int64_t)p.shrink.parts * n * rp * 4;
   p.dz_parts_bytes = p.fused ? (int64_t)p.tiles0 * n * rp * 4 : 0;
-  p.part0_bytes = factors && !p.direct ? (cdiv(n, p.range0) + n_adapters) * rank * d_out * 4 : 0;
-  p.part1_bytes = factors && !p.direct ? (cdiv(n, p.range1) + n_adapters) * rank * d_in * 4 : 0;
+  p.part0_bytes = factors && !p.few ? (cdiv(n, p.range0) + n_adapters) * rank * d_out * 4 : 0;
+  p.part1_bytes = factors && !p.few ? (cdiv(n, p.range1) + n_adapters) * rank * d_in * 4 : 0;
   return p;
 }
 }  // namespace
@@ -1423,10 +1490,9 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     // outer reads x and grad_out after grad_x here
     if (grad_x && apart(grad_x, ldgx, d_in, grad_out, ldg, d_out, n_rows) && (!grad_a || apart(grad_x, ldgx, d_in, x, ldx, d_in, n_rows)))
       blocks = few_rows(n_rows, n_adapters, d_out, d_in, rank);
-    const int dz_count = blocks ? 1 : p.shrink.parts, direct = !p.direct ? 0 : accumulate ? 2 : 1;
-    if (direct) part0 = grad_b, part1 = grad_a;
-    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, direct, (const bf16_t*)b, scales, dz_parts};
-    const OuterSide s1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, direct, nullptr, nullptr, nullptr};
+    const int dz_count = blocks ? 1 : p.shrink.parts;
+    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
+    const OuterSide s1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
     const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
     if (p.fused) {
       launch_outer<1, true>(s0, s0, p.tiles0, p.tiles0, splits0, streamed(n_rows, d_out), offsets, row_ids, n_rows, n_adapters, rank, st);
@@ -1442,7 +1508,14 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
         PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
       }
       PM_CHECK_LAUNCH("pm_lora_bwd");
-      if (grad_a) {
+      if (grad_a && p.few) {
+        const int t0 = (int)cdiv(d_out, 128), t01 = t0 + (int)cdiv(d_in, 128);
+        const FewSide f0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, grad_b}, f1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, grad_a};
+        const bool many = n_rows > 8 * n_adapters;
+        hipLaunchKernelGGL((many ? outer_few_kernel<4> : outer_few_kernel<1>), dim3((unsigned)few_tiles(d_in, d_out, rank), n_adapters), dim3(many ? 256 : 64), 0, st, f0, f1, t0, t01, offsets, row_ids, (int)n_rows, rank,
+                           padded_rank(rank), accumulate);
+        PM_CHECK_LAUNCH("pm_lora_bwd");
+      } else if (grad_a) {
         PM_BY_RANK(rank, (launch_outer<RT, false>(s0, s1, p.tiles0, p.tiles0 + p.tiles1, splits0, streamed(n_rows, (d_in + d_out) / 2), offsets, row_ids, n_rows, n_adapters, rank, st)));
         PM_CHECK_LAUNCH("pm_lora_bwd");
       }
@@ -1450,7 +1523,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
   }
   Join join{};
   unsigned join_blocks = 0;
-  if (grad_a && !p.direct) {
+  if (grad_a && !p.few) {
     join = Join{part0, part1, grad_b, grad_a, rank * d_out, rank * d_in, offsets, (int)n_rows, p.range0, p.range1, accumulate, (int)cdiv(rank * (d_in + d_out) / 4, 256)};
     join_blocks = (unsigned)join.per_adapter * n_adapters;
   }
