@@ -1301,6 +1301,7 @@ class GradClipPlan:
         _, pieces = cut(self._PIECE)
         self.n_chunks, self.n_pieces = len(chunks), len(pieces)
         self._table, self._pieces = (torch.from_numpy(np.ascontiguousarray(t)).to(self.device) for t in (chunks, pieces))
+        self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
         self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)  # the tables' own
         self._offsets = torch.from_numpy(np.searchsorted(np.array(groups, dtype=np.int64)[of], np.arange(self.n_groups + 1)).astype(np.int32)).to(self.device)
 
@@ -1317,15 +1318,19 @@ class GradClipPlan:
         if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:  # the tables' memory is not given away before this stream is done with them
             for t in (self._table, self._pieces, self._offsets):
                 t.record_stream(torch.cuda.current_stream(self.device))
-        partials = torch.empty(self.n_chunks + 1, dtype=torch.float64, device=self.device) if sumsq is None else None
-        sums = both = norms = coefs = None
+        # of its own for each call: the chunks' sums, and behind them the factors where nobody wants them
+        work = self._table.new_empty(self.n_chunks + 1 + (self.n_groups + 1) // 2)
+        sums = norms = coefs = None
+        at = None if want_sumsq else work.data_ptr() + 8 * (self.n_chunks + 1)
         if want_sumsq:
             sums = torch.empty(self.n_groups, dtype=torch.float64, device=self.device)
         else:
-            both = torch.empty((2, self.n_groups), dtype=torch.float32, device=self.device)
-            norms, coefs = both.unbind()
+            norms = self._f32.new_empty(self.n_groups)
+            if not scale:
+                coefs = self._f32.new_empty(self.n_groups)
+                at = coefs.data_ptr()
         _launch(lib.pm_grad_clip, "pm_grad_clip", (self._table,), _p(self._table), self.n_chunks, _p(self._offsets), self.n_groups, _p(self._pieces), self.n_pieces if scale else 0,
-                _p(sumsq), max_norm, _p(limits), _p(partials), _p(sums), _p(norms), _p(coefs))
+                _p(sumsq), max_norm, _p(limits), work.data_ptr(), _p(sums), _p(norms), at)
         return sums, norms, coefs
 
     def sumsq(self) -> Tensor:
