@@ -982,17 +982,30 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
         for (int i = 0; i < 4; ++i) a[i] = ta[i] + st % kOuterRing * kBuf;
         u32x2 tv[8];
         tr_read_tile(a, tv);
+        // z's fragments are asked for two ahead (the schedule says so: left to itself it waits for each; rank 128 16 384 rows 4096 -> 12288 396 -> 371 us, rank 16 4096 -> 6144 86 -> 84)
         const int zrow = (lq * 4 + (lr >> 2)) * kZs + (lr & 3) * 8;
+        constexpr int kAhead = 2, kFragments = RT * 3;
+        u32x2 zl[kAhead + 1], zh[kAhead + 1];
+        auto ask = [&](int i) {  // fragment i: ranks of block i / 3, term 2 - i % 3
+          const unsigned char* q = &lz[st & 1][2 - i % 3][zrow + i / 3 * 32];
+          zl[i % (kAhead + 1)] = tr_read(q), zh[i % (kAhead + 1)] = tr_read(q + 16 * kZs);
+        };
 #pragma unroll
-        for (int j = 0; j < RT; ++j)
+        for (int i = 0; i < kAhead && i < kFragments; ++i) ask(i);
 #pragma unroll
-          for (int term = 2; term >= 0; --term) {
-            const unsigned char* q = &lz[st & 1][term][zrow + j * 32];
-            const u32x2 l = tr_read(q), h = tr_read(q + 16 * kZs);
-            const u32x4 zf = {l.x, l.y, h.x, h.y};
+        for (int i = 0; i < kFragments; ++i) {
+          if (i + kAhead < kFragments) ask(i + kAhead);
+          const u32x2 l = zl[i % (kAhead + 1)], h = zh[i % (kAhead + 1)];
+          const u32x4 zf = {l.x, l.y, h.x, h.y};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i][j] = mfma(u32x4{tv[2 * i].x, tv[2 * i].y, tv[2 * i + 1].x, tv[2 * i + 1].y}, zf, acc[i][j]);
-          }
+          for (int c = 0; c < 4; ++c) acc[c][i / 3] = mfma(u32x4{tv[2 * c].x, tv[2 * c].y, tv[2 * c + 1].x, tv[2 * c + 1].y}, zf, acc[c][i / 3]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * (kAhead + 1), 0);
+#pragma unroll
+        for (int i = 0; i < kFragments; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
       };
       // this wave's 64 columns of dz, 32 positions x 16 ranks; and a value of the last stage's dz from all waves for each thread
       auto contract = [&](int st) {
