@@ -569,8 +569,8 @@ int pm_gemm_debug_set_variant(int32_t value);
  * Row tensors are bf16 with their own row strides (elements, multiples of 8, rows 16-byte aligned).  n_rows up to 2^28, d_in, d_out multiples of 8 up to 2^22, rank 1 .. 128 (zero rows of
  * both factors give a smaller rank).  Offsets and row ids out of range are clamped: such a table gives wrong results, never an access out of range.  Deterministic.  NaN and infinities stay
  * in their rows (grad_x, out) and their adapter (grad_a, grad_b), where an infinity may come out as a NaN.
- *   fwd:   z[p] = scales[g] * x[row] . a[g]^T (f32, [n_rows, pm_lora_z_columns(rank)] in the order of the positions, the columns past the rank zero; rows of no adapter are
- *          not written); out[row] = bf16(base[row] + z[p] . b[g]).  out may be base (in place); base NULL = zeros.
+ *   fwd:   z[p] = scales[g] * x[row] . a[g]^T (f32, [n_rows, pm_lora_z_columns(rank)] in the order of the positions, the columns past the rank zero; undefined in
+ *          rows of no adapter); out[row] = bf16(base[row] + z[p] . b[g]).  out may be base (in place); base NULL = zeros.
  *   bwd:   dz[p] = scales[g] * grad_out[row] . b[g]^T; grad_x[row] = bf16(base[row] + dz[p] . a[g]) (grad_x NULL: not wanted; base as above);
  *          grad_a[g] (+)= dz^T . x, grad_b[g] (+)= z^T . grad_out, f32 in the factors' layout, written (accumulate 0; zero for an adapter without rows) or added to (1); both
  *          NULL: not wanted, then x and z may be NULL.  z is what the forward left.

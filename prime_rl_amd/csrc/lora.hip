@@ -848,8 +848,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(const bf16_t* 
 // DZ (rank <= 16, many rows): the same pass over dy also gives dz, so that dy is read once: the tile's 512 columns are contracted with the factor's (from registers), the
 // waves' results are added up through LDS while the next stage runs, and dz comes in one part for each column tile (6 % of the bytes of dy, written and read once).
 struct OuterSide {
-  const float* z;      // [parts][n][rp]
-  int parts;
+  const float* z;      // [n][rp]
   const bf16_t* t;     // [*, ldt]
   int64_t ldt;
   int d;
@@ -958,12 +957,11 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
           }
         }
       };
-      auto load_z = [&](int st, f32x4 (&zv)[kZp], int parts) {
+      auto load_z = [&](int st, f32x4 (&zv)[kZp]) {
 #pragma unroll
         for (int i = 0; i < kZp; ++i) {
           const int piece = (i * 512 + tid) % (SP * RT * 4), p = min(first + st * SP + piece / (RT * 4), last - 1), r = min(piece % (RT * 4) * 4, rp - 4);
-          const float* at = s.z + (int64_t)p * rp + r;
-          zv[i] = sum_parts(at, (int64_t)n * rp, parts);
+          zv[i] = *reinterpret_cast<const f32x4*>(s.z + (int64_t)p * rp + r);
         }
       };
       auto split_z = [&](int st, f32x4 (&zv)[kZp]) {
@@ -1048,7 +1046,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
             if (st > 0) store_dz(st - 1, true);
           fetch(st + 2, true);
           keep_order();
-          load_z(st + 3, next, 1);
+          load_z(st + 3, next);
         } else {
           wait_dma(0);
           lds_barrier();
@@ -1056,7 +1054,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
           if constexpr (DZ)
             if (st > 0) store_dz(st - 1, false);
           if (st + 2 < stages) fetch(st + 2, st + 2 < full);
-          if (st + 3 < stages) load_z(st + 3, next, s.parts);
+          if (st + 3 < stages) load_z(st + 3, next);
         }
         multiply(st);
         if constexpr (DZ) contract(st);
@@ -1064,27 +1062,27 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
       };
       // z and t are asked for in the order in which the loop goes on, every time: the compiler takes the least it sees on any way into the loop for the number of accesses younger than a
       // z that it waits for, and would drain everything in every second stage
-      if (s.parts == 1 && full > 3) {
-        load_z(0, z0, 1);
+      if (full > 3) {
+        load_z(0, z0);
         keep_order();
         fetch(0, true);
         keep_order();
-        load_z(1, zb, 1);
+        load_z(1, zb);
         keep_order();
         fetch(1, true);
         keep_order();
-        load_z(2, za, 1);
+        load_z(2, za);
         split_z(0, z0);
         do {
           stage(std::true_type{}, zb);
           stage(std::true_type{}, za);
         } while (st + 3 < full);
       } else {
-        load_z(0, z0, s.parts);
+        load_z(0, z0);
         fetch(0, full > 0);
-        load_z(min(1, stages - 1), zb, s.parts);
+        load_z(min(1, stages - 1), zb);
         if (stages > 1) fetch(1, full > 1);
-        load_z(min(2, stages - 1), za, s.parts);
+        load_z(min(2, stages - 1), za);
         split_z(0, z0);
       }
       while (st < stages) {
@@ -1190,8 +1188,8 @@ __global__ __launch_bounds__(W * 64) void outer_few_kernel(FewSide s0, FewSide s
   }
 }
 
-// dz of 4 ranks: the column tiles' parts, added in their order
-__global__ __launch_bounds__(256) void sum_dz_kernel(const float* __restrict__ parts, int count, int64_t elems, float* __restrict__ dz) {
+// z or dz of 4 ranks: its parts, added in their order (dz may be the first part)
+__global__ __launch_bounds__(256) void sum_z_kernel(const float* parts, int count, int64_t elems, float* dz) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= elems) return;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
@@ -1217,6 +1215,14 @@ constexpr int kLdsBytes = 160 * 1024;  // of a CU
 // 16 384 rows 4096 -> 6144 105 -> 98 us, 4096 rows 34 -> 36).
 // A weight on its way to another buffer has not been touched before, and streams from 24 Mi as well (12288 x 4096: 40 -> 38 us).
 constexpr int64_t kStreamRows = (int64_t)24 << 20, kStreamBase = (int64_t)80 << 20;
+// Parts of z are added up by a launch of their own before outer, whose stages go on without a pause only over one part, and where expand's column tiles would read more than this of them
+// again and again (rank 64, 4096 rows 4096 -> 4096: forward 44 -> 35 us, backward 82 -> 68; rank 16, 1000 rows: backward 29 -> 27, but the forward, 14 MB, 15.6 -> 18.3).
+constexpr int64_t kPartsBytes = (int64_t)24 << 20;
+static inline bool sum_first(int64_t n, int rank, int parts, int64_t d) { return parts > 1 && n * padded_rank(rank) * 4 * parts * cdiv(d, 256) > kPartsBytes; }
+static void launch_sum_z(const float* from, int parts, int64_t n, int rank, float* z, hipStream_t stream) {
+  const int64_t elems = n * padded_rank(rank);
+  hipLaunchKernelGGL(sum_z_kernel, dim3((unsigned)cdiv(elems, 1024)), dim3(256), 0, stream, from, parts, elems, z);
+}
 static inline int streamed(int64_t n, int64_t d) { return n * d >= kStreamRows ? 1 : 0; }
 struct ShrinkPlan {
   int rows, depth, parts, chunks_per_part;
@@ -1224,11 +1230,10 @@ struct ShrinkPlan {
 };
 // Narrow: 32 positions a tile; where the tiles are fewer than the 512 workgroups that run at once, the long axis is cut into parts of at least two chunks.  Workgroups that
 // all run at once end at very different times (16 384 x 12288: the first at 68, the last at 105 us), so long rows of up to two rounds are cut into parts of 12 chunks and more, which later
-// workgroups take where there is room: the forward from 12288 to 4096 columns 158 -> 146 us at 16 384 rows, 91 -> 75 at 8192 (shorter parts or more rounds: no gain).  The
-// backward's dz stays whole: outer would add the parts up in each column tile (+15 %).
+// workgroups take where there is room: the forward from 12288 to 4096 columns 158 -> 146 us at 16 384 rows, 91 -> 75 at 8192 (shorter parts or more rounds: no gain).
 // Wide: a tile's rows and the parts are chosen together to make the busiest CU's work least: rounds of 256 workgroups (257 tiles of 128 rows take 1.5 times as long as 256) times
 // what one moves (its rows and the factor, 256 bytes each in a chunk, and a start as long as 160 of these), and the parts of z, which are written and read again.
-static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank, bool forward) {
+static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank) {
   ShrinkPlan p;
   const bool narrow = rank <= 16;
   const int factor = rank_tiles(rank) * 16, chunks = (int)cdiv(d, narrow ? kNarrowChunk : kWideChunk), most = chunks / 2 < kMostParts ? (chunks / 2 > 1 ? chunks / 2 : 1) : kMostParts;
@@ -1236,7 +1241,7 @@ static inline ShrinkPlan shrink_plan(int64_t n, int n_adapters, int d, int rank,
   if (narrow) {
     p.rows = kNarrowRows, p.depth = kRing, p.tiles = max_tiles(n, n_adapters, p.rows);
     p.parts = parts_of(p.tiles > 0 ? p.tiles : 1, 512);
-    if (forward && p.tiles > 0 && p.tiles <= 1024) {
+    if (p.tiles > 0 && p.tiles <= 1024) {
       const int even = chunks / 12 < 2200 / (int)p.tiles ? chunks / 12 : 2200 / (int)p.tiles;
       p.parts = even > kMostParts ? kMostParts : even > p.parts ? even : p.parts;
     }
@@ -1395,7 +1400,7 @@ extern "C" int64_t pm_lora_z_columns(int32_t rank) { return rank >= 1 && rank <=
 
 extern "C" int64_t pm_lora_fwd_workspace_bytes(int64_t n_rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int32_t rank) {
   if (n_rows <= 0 || rank < 1 || rank > kMaxRank || few_rows(n_rows, n_adapters, d_in, d_out, rank)) return 0;
-  const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true).parts;
+  const int parts = shrink_plan(n_rows, n_adapters, (int)d_in, rank).parts;
   return parts > 1 ? (int64_t)parts * n_rows * padded_rank(rank) * 4 : 0;
 }
 
@@ -1412,7 +1417,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   PM_REQUIRE(base != out || ldbase == ldout, PM_ERR_INVALID_ARG, "pm_lora_fwd: base and out are the same rows with different strides");
   PM_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)z) & 15) == 0, PM_ERR_INVALID_ARG, "pm_lora_fwd: a, b and z must be 16-byte aligned");
   const int blocks = few_rows(n_rows, n_adapters, d_in, d_out, rank);
-  ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank, true);
+  ShrinkPlan plan = shrink_plan(n_rows, n_adapters, (int)d_in, rank);
   if (blocks) plan.parts = 1, plan.chunks_per_part = (int)cdiv(d_in, rank <= 16 ? kNarrowChunk : kWideChunk);
   const int parts = plan.parts;
   const int64_t need = pm_lora_fwd_workspace_bytes(n_rows, n_adapters, d_in, d_out, rank);
@@ -1427,7 +1432,12 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   float* zs = parts > 1 ? (float*)workspace : z;
   PM_BY_RANK(rank, (launch_shrink<RT>(plan, x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, zs, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
-  PM_BY_RANK(rank, (launch_expand<RT, kForward>(zs, parts, parts > 1 ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, Join{}, 0, st)));
+  const bool sum = sum_first(n_rows, rank, parts, d_out);
+  if (sum) {
+    launch_sum_z(zs, parts, n_rows, rank, z, st);
+    PM_CHECK_LAUNCH("pm_lora_fwd");
+  }
+  PM_BY_RANK(rank, (launch_expand<RT, kForward>(sum ? z : zs, sum ? 1 : parts, parts > 1 && !sum ? z : nullptr, nullptr, 0.f, b, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, base, ldbase, out, ldout, Join{}, 0, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
   return PM_OK;
 }
@@ -1448,7 +1458,7 @@ BwdPlan bwd_plan(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int ran
   const int rp = padded_rank(rank);
   p.tiles0 = (int)cdiv(d_out, kOuterCols), p.tiles1 = (int)cdiv(d_in, kOuterCols);
   p.fused = factors && rank <= 16 && n * d_out >= kFusedElements;
-  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank, false);
+  p.shrink = shrink_plan(n, n_adapters, (int)d_out, rank);
   if (p.fused) p.shrink.parts = 1;
   p.few = !p.fused && n <= (n_adapters > 1 ? kFewOuterRows : kFewOuterRows / 2) && few_tiles(d_in, d_out, rank) * n_adapters <= 1 << 20;
   p.range0 = outer_range(n, n_adapters, p.fused ? p.tiles0 : p.tiles0 + p.tiles1, rank);
@@ -1482,7 +1492,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
   BwdPlan p{};
   p.range0 = p.range1 = 1;
   float *dz = (float*)ws, *dz_parts = nullptr, *part0 = nullptr, *part1 = nullptr;
-  int blocks = 0;  // of few_rows
+  int blocks = 0, dz_count = 1;  // of few_rows; parts of dz
   if (n_rows > 0) {
     PM_REQUIRE(a && b && scales, PM_ERR_INVALID_ARG, "pm_lora_bwd: null pointer");
     PM_TRY(check_rows("pm_lora_bwd", "grad_out", grad_out, ldg, d_out));
@@ -1503,14 +1513,15 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     // outer reads x and grad_out after grad_x here
     if (grad_x && apart(grad_x, ldgx, d_in, grad_out, ldg, d_out, n_rows) && (!grad_a || apart(grad_x, ldgx, d_in, x, ldx, d_in, n_rows)))
       blocks = few_rows(n_rows, n_adapters, d_out, d_in, rank);
-    const int dz_count = blocks ? 1 : p.shrink.parts;
-    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
-    const OuterSide s1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
+    const bool sum = !blocks && p.shrink.parts > 1 && ((grad_a && !p.few) || (grad_x && sum_first(n_rows, rank, p.shrink.parts, d_in)));
+    dz_count = blocks || sum ? 1 : p.shrink.parts;
+    const OuterSide s0{z, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
+    const OuterSide s1{dz, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
     const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
     if (p.fused) {
       launch_outer<1, true>(s0, s0, p.tiles0, p.tiles0, splits0, streamed(n_rows, d_out), offsets, row_ids, n_rows, n_adapters, rank, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
-      hipLaunchKernelGGL(sum_dz_kernel, dim3((unsigned)cdiv(n_rows * 4, 256)), dim3(256), 0, st, dz_parts, p.tiles0, n_rows * 16, dz);
+      launch_sum_z(dz_parts, p.tiles0, n_rows, rank, dz, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
       launch_outer<1, false>(s1, s1, p.tiles1, p.tiles1, splits1, streamed(n_rows, d_in), offsets, row_ids, n_rows, n_adapters, rank, st);
       PM_CHECK_LAUNCH("pm_lora_bwd");
@@ -1521,6 +1532,10 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
         PM_BY_RANK(rank, (launch_shrink<RT>(p.shrink, grad_out, ldg, b, scales, offsets, row_ids, n_rows, n_adapters, (int)d_out, rank, dz, st)));
       }
       PM_CHECK_LAUNCH("pm_lora_bwd");
+      if (sum) {
+        launch_sum_z(dz, p.shrink.parts, n_rows, rank, dz, st);
+        PM_CHECK_LAUNCH("pm_lora_bwd");
+      }
       if (grad_a && p.few) {
         const int t0 = (int)cdiv(d_out, 128), t01 = t0 + (int)cdiv(d_in, 128);
         const FewSide f0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, grad_b}, f1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, grad_a};
@@ -1541,7 +1556,7 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     join_blocks = (unsigned)join.per_adapter * n_adapters;
   }
   if (n_rows > 0 && grad_x && !blocks) {
-    PM_BY_RANK(rank, (launch_expand<RT, kBackward>(dz, p.shrink.parts, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, join,
+    PM_BY_RANK(rank, (launch_expand<RT, kBackward>(dz, dz_count, nullptr, nullptr, 0.f, a, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, base, ldbase, grad_x, ldgx, join,
                                                    join_blocks, st)));
     PM_CHECK_LAUNCH("pm_lora_bwd");
   } else if (join_blocks) {
