@@ -848,7 +848,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(const bf16_t* 
 // DZ (rank <= 16, many rows): the same pass over dy also gives dz, so that dy is read once: the tile's 512 columns are contracted with the factor's (from registers), the
 // waves' results are added up through LDS while the next stage runs, and dz comes in one part for each column tile (6 % of the bytes of dy, written and read once).
 struct OuterSide {
-  const float* z;      // [n][rp]
+  const float* z;      // [parts][n][rp]
+  int parts;
   const bf16_t* t;     // [*, ldt]
   int64_t ldt;
   int d;
@@ -957,11 +958,11 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
           }
         }
       };
-      auto load_z = [&](int st, f32x4 (&zv)[kZp]) {
+      auto load_z = [&](int st, f32x4 (&zv)[kZp], int parts) {
 #pragma unroll
         for (int i = 0; i < kZp; ++i) {
           const int piece = (i * 512 + tid) % (SP * RT * 4), p = min(first + st * SP + piece / (RT * 4), last - 1), r = min(piece % (RT * 4) * 4, rp - 4);
-          zv[i] = *reinterpret_cast<const f32x4*>(s.z + (int64_t)p * rp + r);
+          zv[i] = sum_parts(s.z + (int64_t)p * rp + r, (int64_t)n * rp, parts);
         }
       };
       auto split_z = [&](int st, f32x4 (&zv)[kZp]) {
@@ -1046,7 +1047,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
             if (st > 0) store_dz(st - 1, true);
           fetch(st + 2, true);
           keep_order();
-          load_z(st + 3, next);
+          load_z(st + 3, next, 1);
         } else {
           wait_dma(0);
           lds_barrier();
@@ -1054,7 +1055,7 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
           if constexpr (DZ)
             if (st > 0) store_dz(st - 1, false);
           if (st + 2 < stages) fetch(st + 2, st + 2 < full);
-          if (st + 3 < stages) load_z(st + 3, next);
+          if (st + 3 < stages) load_z(st + 3, next, s.parts);
         }
         multiply(st);
         if constexpr (DZ) contract(st);
@@ -1062,27 +1063,27 @@ __global__ __launch_bounds__(512) void outer_kernel(OuterSide s0, OuterSide s1, 
       };
       // z and t are asked for in the order in which the loop goes on, every time: the compiler takes the least it sees on any way into the loop for the number of accesses younger than a
       // z that it waits for, and would drain everything in every second stage
-      if (full > 3) {
-        load_z(0, z0);
+      if (s.parts == 1 && full > 3) {
+        load_z(0, z0, 1);
         keep_order();
         fetch(0, true);
         keep_order();
-        load_z(1, zb);
+        load_z(1, zb, 1);
         keep_order();
         fetch(1, true);
         keep_order();
-        load_z(2, za);
+        load_z(2, za, 1);
         split_z(0, z0);
         do {
           stage(std::true_type{}, zb);
           stage(std::true_type{}, za);
         } while (st + 3 < full);
       } else {
-        load_z(0, z0);
+        load_z(0, z0, s.parts);
         fetch(0, full > 0);
-        load_z(min(1, stages - 1), zb);
+        load_z(min(1, stages - 1), zb, s.parts);
         if (stages > 1) fetch(1, full > 1);
-        load_z(min(2, stages - 1), za);
+        load_z(min(2, stages - 1), za, s.parts);
         split_z(0, z0);
       }
       while (st < stages) {
@@ -1215,10 +1216,13 @@ constexpr int kLdsBytes = 160 * 1024;  // of a CU
 // 16 384 rows 4096 -> 6144 105 -> 98 us, 4096 rows 34 -> 36).
 // A weight on its way to another buffer has not been touched before, and streams from 24 Mi as well (12288 x 4096: 40 -> 38 us).
 constexpr int64_t kStreamRows = (int64_t)24 << 20, kStreamBase = (int64_t)80 << 20;
-// Parts of z are added up by a launch of their own before outer, whose stages go on without a pause only over one part, and where expand's column tiles would read more than this of them
-// again and again (rank 64, 4096 rows 4096 -> 4096: forward 44 -> 35 us, backward 82 -> 68; rank 16, 1000 rows: backward 29 -> 27, but the forward, 14 MB, 15.6 -> 18.3).
-constexpr int64_t kPartsBytes = (int64_t)24 << 20;
-static inline bool sum_first(int64_t n, int rank, int parts, int64_t d) { return parts > 1 && n * padded_rank(rank) * 4 * parts * cdiv(d, 256) > kPartsBytes; }
+// Parts of z are added up by a launch of their own where the column tiles of expand (24 MB) or of outer (2 MB: its stages go on without a pause only over one part) would read more than this
+// of them again and again: rank 64, 4096 rows 4096 -> 4096 forward 44 -> 35 us, backward 82 -> 68; rank 16, 1000 rows (8 and 4 MB) forward 15.6 and 18.3, backward 29 -> 27; rank 8, 777 rows
+// 1024 -> 2048 (0.4 MB) the same on the card, and the host takes 2.6 us more.
+static inline bool sum_first(int64_t n, int rank, int parts, int64_t expand_cols, int64_t outer_cols) {
+  const int64_t bytes = n * padded_rank(rank) * 4 * parts;
+  return parts > 1 && (bytes * cdiv(expand_cols, 256) > (int64_t)24 << 20 || bytes * cdiv(outer_cols, 512) > (int64_t)2 << 20);
+}
 static void launch_sum_z(const float* from, int parts, int64_t n, int rank, float* z, hipStream_t stream) {
   const int64_t elems = n * padded_rank(rank);
   hipLaunchKernelGGL(sum_z_kernel, dim3((unsigned)cdiv(elems, 1024)), dim3(256), 0, stream, from, parts, elems, z);
@@ -1432,7 +1436,7 @@ extern "C" int pm_lora_fwd(const void* x, int64_t ldx, const void* a, const void
   float* zs = parts > 1 ? (float*)workspace : z;
   PM_BY_RANK(rank, (launch_shrink<RT>(plan, x, ldx, a, scales, offsets, row_ids, n_rows, n_adapters, (int)d_in, rank, zs, st)));
   PM_CHECK_LAUNCH("pm_lora_fwd");
-  const bool sum = sum_first(n_rows, rank, parts, d_out);
+  const bool sum = sum_first(n_rows, rank, parts, d_out, 0);
   if (sum) {
     launch_sum_z(zs, parts, n_rows, rank, z, st);
     PM_CHECK_LAUNCH("pm_lora_fwd");
@@ -1513,10 +1517,10 @@ extern "C" int pm_lora_bwd(const void* grad_out, int64_t ldg, const void* x, int
     // outer reads x and grad_out after grad_x here
     if (grad_x && apart(grad_x, ldgx, d_in, grad_out, ldg, d_out, n_rows) && (!grad_a || apart(grad_x, ldgx, d_in, x, ldx, d_in, n_rows)))
       blocks = few_rows(n_rows, n_adapters, d_out, d_in, rank);
-    const bool sum = !blocks && p.shrink.parts > 1 && ((grad_a && !p.few) || (grad_x && sum_first(n_rows, rank, p.shrink.parts, d_in)));
+    const bool sum = !blocks && sum_first(n_rows, rank, p.shrink.parts, grad_x ? d_in : 0, grad_a && !p.few ? d_in : 0);
     dz_count = blocks || sum ? 1 : p.shrink.parts;
-    const OuterSide s0{z, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
-    const OuterSide s1{dz, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
+    const OuterSide s0{z, 1, (const bf16_t*)grad_out, ldg, (int)d_out, part0, p.range0, (const bf16_t*)b, scales, dz_parts};
+    const OuterSide s1{dz, dz_count, (const bf16_t*)x, ldx, (int)d_in, part1, p.range1, nullptr, nullptr, nullptr};
     const unsigned splits0 = (unsigned)cdiv(n_rows, p.range0), splits1 = (unsigned)cdiv(n_rows, p.range1);
     if (p.fused) {
       launch_outer<1, true>(s0, s0, p.tiles0, p.tiles0, splits0, streamed(n_rows, d_out), offsets, row_ids, n_rows, n_adapters, rank, st);
