@@ -387,3 +387,53 @@ def test_lora_results_in_their_own_inputs_memory(ops, n):
         got = ops.lora_bwd(t["dy"], t["x"], z, *args, base=c["bx"], grad_x=t[name])
         assert got[0] is t[name]
         _check_bwd(c, z, *got)
+
+
+@pytest.mark.parametrize("n,ld,rank", [(40, 1 << 27, 16), (40, 1 << 27, 100), (300, 1 << 24, 16), (300, 1 << 24, 64), (300, 1 << 24, 100)])
+def test_lora_rows_gigabytes_apart(ops, n, ld, rank):
+    """Column slices of one buffer of more than 2^32 elements, in place."""
+    d_in, d_out = 264, 520
+    c = _case([n // 3, n - n // 3 - 2], d_in, d_out, rank, 2, True, seed=6)
+    storage = torch.empty(n * ld, dtype=BF16, device=DEV)
+    wide, at = {}, 0
+    for name in ("x", "base", "dy", "bx"):
+        w = c[name].shape[1]
+        wide[name] = storage.as_strided((n, w), (ld, 1), at)
+        wide[name].copy_(c[name])
+        at += w
+    args = (c["a"], c["b"], c["scales"], c["offsets"])
+    out, z = ops.lora_fwd(c["x"], *args, base=c["base"], row_ids=c["row_ids"])
+    got, zw = ops.lora_fwd(wide["x"], *args, base=wide["base"], out=wide["base"], row_ids=c["row_ids"])
+    assert got is wide["base"]
+    _check_fwd(c, got, zw)
+    _check_fwd(c, out, z)
+    want = ops.lora_bwd(c["dy"], c["x"], z, *args, base=c["bx"], row_ids=c["row_ids"])
+    back = ops.lora_bwd(wide["dy"], wide["x"], z, *args, base=wide["bx"], grad_x=wide["bx"], row_ids=c["row_ids"])
+    _check_bwd(c, z, *want)
+    _check_bwd(c, z, *back)
+    assert torch.equal(wide["x"], c["x"]) and torch.equal(wide["dy"], c["dy"])
+
+
+@pytest.mark.parametrize("counts,d_in,d_out,rank,mixed", [([350, 0, 240], 4096, 1032, 64, True), ([900], 4096, 4096, 64, False), ([500, 400], 4096, 4096, 128, False), ([700, 600], 4096, 4096, 9, True)])
+def test_lora_of_long_rows_in_parts(ops, counts, d_in, d_out, rank, mixed):
+    """The long axis cut into parts that are added up before they are used; in a graph as well."""
+    c = _case(counts, d_in, d_out, rank, 10, mixed, seed=8)
+
+    def step():
+        out, z = ops.lora_fwd(c["x"], c["a"], c["b"], c["scales"], c["offsets"], base=c["base"], row_ids=c["row_ids"])
+        return (out, z, *ops.lora_bwd(c["dy"], c["x"], z, c["a"], c["b"], c["scales"], c["offsets"], base=c["bx"], row_ids=c["row_ids"]))
+
+    out, z, *grads = step()
+    _check_fwd(c, out, z)
+    _check_bwd(c, z, *grads)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for turn in range(3):
+        c["x"].copy_(torch.randn_like(c["x"]))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        for i in (0, 2, 3, 4):  # (z of rows of no adapter is undefined)
+            assert torch.equal(held[i], eager[i]), turn
