@@ -13,7 +13,7 @@
 // tensor with 16-byte accesses, and the matrix cores are there to keep the arithmetic out of the way.  From rank 64 on the LDS has as much to do as the memory.  Measured, in the
 // kernels' own time (a large copy moves 5.7 TB/s, a read past the caches 6.7):
 //   shrink  16 384 x 4096 rank 16 23 us = 5.8 TB/s, 32 768 x 12288 rank 64 143 us = 5.6;   expand  16 384 x 6144 rank 16 66 us = 6.1, 32 768 x 4096 rank 64 107 us = 5.0
-//   outer   16 384 x 4096 rank 16 28 us = 4.8, with dz 16 384 x 6144 48 us = 4.5 (and dz's parts), 32 768 x (12288 + 4096) rank 64 220 us = 4.9
+//   outer   16 384 x 4096 rank 16 27 us = 5.0, with dz 16 384 x 6144 47 us = 4.6 (dz's parts among it), 32 768 x (12288 + 4096) rank 64 217 us = 4.9
 //
 // Numerics: z and dz are f32 in memory.  Where they feed the matrix cores they are split into bf16 terms that add up to the f32 value: two terms (16 bits)
 // in expand, whose result is rounded to bf16 (8 bits) anyway, three terms (24 bits: all of it) in outer, whose results are f32 gradients.  Everything else in
@@ -843,8 +843,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(const bf16_t* 
 // The positions are the contraction, so both operands are read transposed (ds_read_b64_tr_b16).  Stages of 32 positions go through LDS: t by DMA, a ring of three deep
 // (16-byte slot pairs permuted by the row's number, so that the 8 rows of half a transposed read lie in different banks), z through registers, where it is split into
 // three bf16 planes.  A wave takes 64 columns and all ranks.
-// Bound at rank 16 by memory, less what a workgroup waits for its first stage (7 us) and the spread of the ends (a fifth); at rank 64 by the LDS and the matrix cores, of which z's three terms
-// take two thirds (with rows that lie in the caches 32 768 x 12288 takes 173 us, without 194).
+// Bound at rank 16 by memory, less the 4 us until a workgroup's first stage is there; at rank 64 by the LDS and the matrix cores too, of which z's three terms take two thirds (with rows that
+// lie in the caches 32 768 x 12288 takes 173 us, without 190).
 // DZ (rank <= 16, many rows): the same pass over dy also gives dz, so that dy is read once: the tile's 512 columns are contracted with the factor's (from registers), the
 // waves' results are added up through LDS while the next stage runs, and dz comes in one part for each column tile (6 % of the bytes of dy, written and read once).
 struct OuterSide {
