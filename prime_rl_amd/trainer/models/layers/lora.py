@@ -195,14 +195,44 @@ def adapter_parameters(model: nn.Module) -> list[nn.Parameter]:
     return [p for m in model.modules() if isinstance(m, LoRAAdapters) for p in (m.a, m.b)]
 
 
+def adapter_state(model: nn.Module) -> LoRAState | None:
+    """The state that the model's adapters share; None for a model without."""
+    return next((m.state for m in model.modules() if isinstance(m, LoRAAdapters)), None)
+
+
+def pushed_adapter(model: nn.Module, adapter: int | None) -> int | None:
+    """Which adapter a push of `model` folds in: None for a model without adapters, the only one of a model with one, else the one that is named — the inference
+    engines know neither a frozen weight without its run's update nor the factors' names."""
+    state = adapter_state(model)
+    if state is None:
+        if adapter is not None:
+            raise ValueError(f"adapter {adapter} of a model without adapters")
+        return None
+    if adapter is None and state.n_adapters > 1:
+        raise ValueError(f"the model has {state.n_adapters} adapters: name the one whose run the weights are for (adapter=...)")
+    adapter = 0 if adapter is None else adapter
+    if not 0 <= adapter < state.n_adapters:
+        raise ValueError(f"adapter {adapter} of a model with {state.n_adapters}")
+    return adapter
+
+
+def adapter_linears(model: nn.Module) -> dict[str, nn.Linear]:
+    """The projections with adapters, by the names of their weights in the model's state dict."""
+    return {f"{name}.weight": m for name, m in model.named_modules(remove_duplicate=False) if isinstance(getattr(m, "lora", None), LoRAAdapters)}
+
+
+@torch.no_grad()
+def merged_weight(linear: nn.Linear, adapter: int) -> Tensor:
+    """The projection's weight with one run's adapter folded in (`ops.lora_merge`)."""
+    lora = linear.lora
+    return ops.lora_merge(linear.weight.detach(), lora.a[adapter].to(torch.bfloat16), lora.b[adapter].to(torch.bfloat16), float(lora.state.scales[adapter]))
+
+
 @torch.no_grad()
 def merged_state_dict(model: nn.Module, adapter: int) -> dict[str, Tensor]:
     """The model's state dict as a model without adapters has it, with one run's adapter folded into the projections (`ops.lora_merge`): what the weight push
     sends to that run's inference engine."""
+    adapter = pushed_adapter(model, adapter)
     sd = {k: v.detach() for k, v in model.state_dict().items() if ".lora." not in k}
-    for name, m in model.named_modules():
-        lora = getattr(m, "lora", None)
-        if isinstance(lora, LoRAAdapters):
-            scale = float(lora.state.scales[adapter])
-            sd[f"{name}.weight"] = ops.lora_merge(m.weight.detach(), lora.a[adapter].to(torch.bfloat16), lora.b[adapter].to(torch.bfloat16), scale)
+    sd.update({k: merged_weight(m, adapter) for k, m in adapter_linears(model).items()})
     return sd

@@ -39,6 +39,7 @@ from .. import _lib, ops
 from .._lib import LossParams, PrimeMI355XError
 from . import zero
 from .engine import LossConfig, OptimConfig, PackedBatch
+from .models.layers.lora import adapter_linears, merged_state_dict, merged_weight, pushed_adapter
 from .models.layers.moe import GroupedExperts
 
 
@@ -224,10 +225,12 @@ class ModuleEngine:
         """True when state_dict() runs collectives (every rank must call it, not only the rank that writes the checkpoint)."""
         return self.ep_size > 1
 
-    def state_dict(self) -> dict[str, Tensor]:
+    def state_dict(self, adapter: int | None = None) -> dict[str, Tensor]:
         """HF-named bf16 tensors of the WHOLE model (what the inference engine loads, transports/weights): expert shards are all-gathered
-        over the ep group, MoE names converted like the reference's `revert_weight_conversion` (transports/weights/nccl.py:87-98)."""
-        sd = {k: v.detach() for k, v in self.model.state_dict().items()}
+        over the ep group, MoE names converted like the reference's `revert_weight_conversion` (transports/weights/nccl.py:87-98).  A model with adapters
+        (layers/lora.py) has the names of one without, run `adapter`'s folded in; with several the run has to be named."""
+        adapter = pushed_adapter(self.model, adapter)
+        sd = {k: v.detach() for k, v in self.model.state_dict().items()} if adapter is None else merged_state_dict(self.model, adapter)
         sd = {k: (v if v.dtype == torch.bfloat16 or not v.is_floating_point() else v.to(torch.bfloat16)) for k, v in sd.items()}
         if self.ep_size > 1:
             for key in [k for k in sd if ".mlp.experts.w" in k]:
@@ -257,6 +260,8 @@ class ModuleEngine:
         groups: dict[str, list[dict]] = {}
         rr = 0
         for key, t in self.model.state_dict().items():
+            if ".lora." in key:  # a run's adapter travels inside its projection's weight (push_tensors)
+                continue
             gname = ".".join(key.split(".")[:3]) if key.startswith("model.layers.") else ""
             msgs = groups.setdefault(gname, [])
             hit = next(((wn, hf) for wn, hf in _PROJ if key.endswith(f".mlp.experts.{wn}")), None)
@@ -274,9 +279,10 @@ class ModuleEngine:
         order = [""] + sorted((g for g in groups if g), key=lambda g: int(g.split(".")[2]))
         return [dict(name=g or "non_layer", messages=groups[g]) for g in order if g in groups]
 
-    def push_tensors(self, plan: list[dict], rank: int) -> list[list[Tensor | None]]:
-        """The bf16 tensors this rank sends, aligned with `plan` (None where another rank is the source)."""
-        sd = self.model.state_dict()
+    def push_tensors(self, plan: list[dict], rank: int, adapter: int | None = None) -> list[list[Tensor | None]]:
+        """The bf16 tensors this rank sends, aligned with `plan` (None where another rank is the source); run `adapter`'s folded in as in `state_dict`."""
+        adapter = pushed_adapter(self.model, adapter)
+        sd, merged = self.model.state_dict(), adapter_linears(self.model)
         out = []
         for g in plan:
             row = []
@@ -284,7 +290,7 @@ class ModuleEngine:
                 if m["src"] != rank:
                     row.append(None)
                     continue
-                t = sd[m["key"]].detach()
+                t = merged_weight(merged[m["key"]], adapter) if m["key"] in merged else sd[m["key"]].detach()
                 if not t.is_floating_point():  # state_dict() keeps integer buffers as they are; the sharded push announces ONE dtype (bf16) per message
                     raise PrimeMI355XError(f"push_tensors: {m['key']} is {t.dtype}; the sharded weight push carries floating tensors as bf16 only")
                 row.append((t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16)).contiguous())

@@ -42,7 +42,8 @@ class WeightBroadcast(ABC):
         self.output_dir = Path(output_dir)
 
     @abstractmethod
-    def broadcast_weights(self, model, step: int) -> None: ...
+    def broadcast_weights(self, model, step: int, adapter: int | None = None) -> None:
+        """`adapter`: the run whose weights these are, where the model has several runs' adapters (trainer/models/layers/lora.py)."""
 
     def _notify_orchestrator(self, save_dir: Path) -> None:
         """Create the STABLE marker the orchestrator's weight watcher polls for (nccl.py:214-217)."""
@@ -50,14 +51,21 @@ class WeightBroadcast(ABC):
         (save_dir / STABLE_MARKER).touch()
 
 
-def _named_tensors(model) -> dict[str, torch.Tensor]:
-    """HF-named bf16 tensors of either a GRPOEngine / ParamStore (zero-copy views) or an nn.Module."""
+def _named_tensors(model, adapter: int | None = None) -> dict[str, torch.Tensor]:
+    """HF-named bf16 tensors of a GRPOEngine / ParamStore (zero-copy views), a ModuleEngine or an nn.Module; a run's adapter is folded in."""
     store = getattr(model, "store", model)
     if hasattr(model, "wait_params_ready"):
         model.wait_params_ready()  # the last optimizer step's parameter all-gathers run on the engine's comm stream
     if hasattr(store, "state_dict") and hasattr(store, "buckets"):
+        if adapter is not None:
+            raise ValueError(f"adapter {adapter} of an engine without adapters")
         return store.state_dict()
-    return {k: v.detach() for k, v in model.state_dict().items()}
+    if isinstance(model, torch.nn.Module):
+        from ...trainer.models.layers.lora import merged_state_dict, pushed_adapter
+
+        adapter = pushed_adapter(model, adapter)
+        return {k: v.detach() for k, v in model.state_dict().items()} if adapter is None else merged_state_dict(model, adapter)
+    return {k: v.detach() for k, v in (model.state_dict() if adapter is None else model.state_dict(adapter)).items()}
 
 
 class FileSystemWeightBroadcast(WeightBroadcast):
@@ -69,11 +77,11 @@ class FileSystemWeightBroadcast(WeightBroadcast):
         self.is_master, self.keep, self.group = is_master, keep, group
 
     @torch.no_grad()
-    def broadcast_weights(self, model, step: int) -> None:
+    def broadcast_weights(self, model, step: int, adapter: int | None = None) -> None:
         from safetensors.torch import save_file
 
         # an expert-parallel model assembles its full state dict with collectives: then every rank takes part, the master writes
-        named = _named_tensors(model) if (self.is_master or getattr(model, "collective_state_dict", False)) else None
+        named = _named_tensors(model, adapter) if (self.is_master or getattr(model, "collective_state_dict", False)) else None
         if self.is_master:
             save_dir = get_step_path(get_broadcast_dir(self.output_dir), step)
             save_dir.mkdir(parents=True, exist_ok=True)
@@ -252,9 +260,11 @@ class RCCLWeightBroadcast(WeightBroadcast):
         self._in_flight: tuple | None = None  # (completion event, None) of the previous asynchronous push (its temporaries are owned by record_stream)
 
     @torch.no_grad()
-    def broadcast_weights(self, model, step: int) -> None:
+    def broadcast_weights(self, model, step: int, adapter: int | None = None) -> None:
         store = getattr(model, "store", model)
         flat = hasattr(store, "buckets")  # GRPOEngine / ParamStore; otherwise an nn.Module engine (trainer/module_engine.py: MoE, expert parallel)
+        if flat and adapter is not None:
+            raise ValueError(f"adapter {adapter} of an engine without adapters")
         if not flat and self.protocol != "reference" and not hasattr(model, "push_plan"):
             raise NotImplementedError("the sharded push needs either the flat parameter buckets of the dense engine or an engine with push_plan() / push_tensors() "
                                       "(trainer/module_engine.py); anything else pushes with the reference byte protocol: PRIME_PUSH_PROTOCOL=reference")
@@ -266,9 +276,9 @@ class RCCLWeightBroadcast(WeightBroadcast):
         if flat or plan is not None:
             named = None
         else:
-            named = model.state_dict() if (self.rank == 0 or getattr(model, "collective_state_dict", False)) else None
+            named = _named_tensors(model, adapter) if (self.rank == 0 or getattr(model, "collective_state_dict", False)) else None
         if plan is not None:
-            named = {f"{gi}.{mi}": t for gi, row in enumerate(model.push_tensors(plan, self.rank)) for mi, t in enumerate(row) if t is not None}
+            named = {f"{gi}.{mi}": t for gi, row in enumerate(model.push_tensors(plan, self.rank, **({} if adapter is None else dict(adapter=adapter)))) for mi, t in enumerate(row) if t is not None}
         device = store.params.device if flat else torch.device(model.device)
         save_dir = get_step_path(get_broadcast_dir(self.output_dir), step)
         if self.rank == 0:
