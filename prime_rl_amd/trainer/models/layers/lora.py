@@ -24,25 +24,37 @@ from .linear import _adjacent_view
 
 class LoRARows:
     """Which rows of a pass belong to which adapter: `offsets` i32 [n + 1], adapter g owns positions [offsets[g], offsets[g + 1]); `row_ids` i32 [rows] or None
-    (position p is row p)."""
+    (position p is row p).  `n_rows`: the rows of the pass that the table is for, and `counts`: each adapter's rows, where the host knows them; a pass of another
+    length is refused by what is known (the kernels clamp a table that does not fit, which would leave rows to the wrong run)."""
 
-    def __init__(self, offsets: Tensor, row_ids: Tensor | None = None):
-        self.offsets, self.row_ids = offsets, row_ids
+    def __init__(self, offsets: Tensor, row_ids: Tensor | None = None, n_rows: int | None = None, counts: list[int] | None = None):
+        self.offsets, self.row_ids, self.n_rows, self.counts = offsets, row_ids, n_rows, counts
+        self._owned = None if counts is None else sum(counts)
+        if n_rows is not None and counts is not None and self._owned > n_rows:
+            raise ValueError(f"num_tokens: {self._owned} rows of adapters in a pass of {n_rows}")
 
     @classmethod
-    def packed(cls, num_tokens: Sequence[int] | Tensor, device) -> LoRARows:
-        """Runs packed one behind the other, `num_tokens[g]` rows of run g (`lora_num_tokens`); rows behind the last run belong to none."""
+    def packed(cls, num_tokens: Sequence[int] | Tensor, device, n_rows: int | None = None) -> LoRARows:
+        """Runs packed one behind the other, `num_tokens[g]` rows of run g (`lora_num_tokens`); rows behind the last run belong to none.  `n_rows`: the rows of the
+        pass; without it, and with `num_tokens` on the device, nothing tells a table that was left from another pass."""
         counts = torch.as_tensor(num_tokens, dtype=torch.int32).reshape(-1)
         if not counts.is_cuda and counts.numel() and int(counts.min()) < 0:
             raise ValueError(f"num_tokens: expected no negative counts, got {counts.tolist()}")
         offsets = torch.zeros(counts.numel() + 1, dtype=torch.int32, device=counts.device)
         offsets[1:] = counts.cumsum(0)
-        return cls(offsets.to(device))
+        return cls(offsets.to(device), n_rows=n_rows, counts=None if counts.is_cuda else counts.tolist())
 
     @classmethod
     def of(cls, adapter_ids: Tensor, n_adapters: int) -> LoRARows:
         """Rows in any order, `adapter_ids[row]` their adapter (outside [0, n_adapters): none)."""
-        return cls(*ops.lora_rows(adapter_ids, n_adapters))
+        return cls(*ops.lora_rows(adapter_ids, n_adapters), n_rows=adapter_ids.numel())
+
+    def check(self, n_rows: int) -> None:
+        """Raises where the table is known not to be that of a pass of `n_rows` rows."""
+        if self.n_rows is not None and self.n_rows != n_rows:
+            raise ValueError(f"the rows' table is for a pass of {self.n_rows} rows, this one has {n_rows}: LoRAState.set_rows comes before each pass")
+        if self._owned is not None and self._owned > n_rows:
+            raise ValueError(f"the rows' table holds {self._owned} rows of adapters, this pass has {n_rows}: LoRAState.set_rows comes before each pass")
 
 
 class LoRAState:
@@ -158,6 +170,7 @@ def lora_linear(x: Tensor, linears: Sequence[nn.Linear], adapters: Sequence[LoRA
         raise ValueError("LoRAState.set_rows says which rows of the pass belong to which adapter: call it before the model")
     if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise ValueError("a captured pass through adapters runs under torch.no_grad()")
+    state.rows.check(x.shape[0])
     x = x if x.is_contiguous() else x.contiguous()
     factors = [f for a in adapters if a is not None for f in (a.a, a.b)]
     return _LoRALinearFn.apply(x, state.rows, state.scales, [a is not None for a in adapters], [lin.weight.detach() for lin in linears],

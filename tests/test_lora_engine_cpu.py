@@ -135,3 +135,28 @@ def test_transports_push_one_of_several_runs(plain_ops, tmp_path):
             FileSystemWeightBroadcast(tmp_path).broadcast_weights(sender, step)
         FileSystemWeightBroadcast(tmp_path).broadcast_weights(sender, step, adapter=2)
         _same(load_file(tmp_path / "broadcasts" / f"step_{step}" / "model.safetensors"), want, plain)
+
+
+def test_a_table_of_another_pass_is_refused():
+    """A table that is longer than the pass, or was made for one of another length, raises before any kernel runs."""
+    from prime_rl_amd.trainer.models.layers.lora import LoRARows, attach_lora, lora_linear
+    from prime_rl_amd.trainer.models.layers.mlp import MLP, MLPConfig
+
+    mlp = MLP(MLPConfig(32, 64)).to(BF16)
+    state = attach_lora(mlp, 2, 4, 8.0, targets=("up_proj",))
+    x = torch.zeros(10, 32, dtype=BF16)
+
+    def run(rows):
+        state.set_rows(rows)
+        lora_linear(x, [mlp.up_proj])
+
+    offsets = torch.tensor([0, 3, 9], dtype=torch.int32)
+    for stale in (LoRARows.packed([6, 5], "cpu"), LoRARows.packed([6, 0], "cpu", n_rows=8), LoRARows.packed(torch.tensor([2, 9]), "cpu"), LoRARows(offsets, n_rows=12),
+                  LoRARows(offsets, torch.arange(9, dtype=torch.int32), n_rows=9)):
+        with pytest.raises(ValueError, match="set_rows"):
+            run(stale)
+    for fits in (LoRARows.packed([6, 4], "cpu"), LoRARows.packed([6, 0], "cpu"), LoRARows.packed([1, 2], "cpu", n_rows=10), LoRARows(offsets), LoRARows(offsets, n_rows=10)):
+        with pytest.raises(Exception, match="GPU"):  # what the kernels' entry says of tensors in host memory
+            run(fits)
+    with pytest.raises(ValueError, match="11 rows of adapters in a pass of 10"):
+        LoRARows.packed([6, 5], "cpu", n_rows=10)
