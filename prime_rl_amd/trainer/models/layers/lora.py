@@ -49,6 +49,13 @@ class LoRARows:
         """Rows in any order, `adapter_ids[row]` their adapter (outside [0, n_adapters): none)."""
         return cls(*ops.lora_rows(adapter_ids, n_adapters), n_rows=adapter_ids.numel())
 
+    def rows_of_adapters(self) -> list[int]:
+        """Each adapter's rows; waits for the device where only it knows them."""
+        if self.counts is None:
+            ends = self.offsets.tolist()
+            self.counts = [b - a for a, b in zip(ends, ends[1:])]
+        return self.counts
+
     def check(self, n_rows: int) -> None:
         """Raises where the table is known not to be that of a pass of `n_rows` rows."""
         if self.n_rows is not None and self.n_rows != n_rows:
@@ -114,7 +121,7 @@ class _LoRALinearFn(torch.autograd.Function):
         else:
             for w, b, part in zip(weights, biases, y.split(widths, dim=1)):
                 _product(x, w, b, part)
-        halves = [f.detach().to(torch.bfloat16) for f in factors]
+        halves = [f.detach().to(torch.bfloat16).contiguous() for f in factors]  # (a trainer engine keeps each run's share in a stretch of its own)
         zs, at = [], 0
         for i, part in enumerate(y.split(widths, dim=1)):
             if has_adapter[i]:

@@ -23,7 +23,10 @@ distributed/expert_parallel.py) maps as follows on a 288 GB part:
     experts — the experts are what is big, and expert parallelism already shards them.
 
 Parameters are re-pointed at one flat bf16 buffer (f32 parameters such as an f32 router gate at the f32 master buffer itself), so the
-optimizer is ONE fused `pm_adamw_step` launch and gradient reduction is one collective per class."""
+optimizer is ONE fused `pm_adamw_step` launch and gradient reduction is one collective per class.
+
+A model with the adapters of several runs (layers/lora.py): the runs share nothing but the passes.  Each run's share of every factor lies in one stretch of the flat
+buffers, and each has its own gradient norm, clipping factor, step count and update; a run without rows in a step (on any rank), or with gradients that are no numbers, is left as it is."""
 
 from __future__ import annotations
 
@@ -39,7 +42,7 @@ from .. import _lib, ops
 from .._lib import LossParams, PrimeMI355XError
 from . import zero
 from .engine import LossConfig, OptimConfig, PackedBatch
-from .models.layers.lora import adapter_linears, merged_state_dict, merged_weight, pushed_adapter
+from .models.layers.lora import LoRARows, adapter_linears, adapter_parameters, adapter_state, merged_state_dict, merged_weight, pushed_adapter
 from .models.layers.moe import GroupedExperts
 
 
@@ -92,14 +95,16 @@ class ModuleEngine:
         self.router_replay = router_replay
         self.step_count = 0
         self.cp_size = 1
-        # -- flat storage: replicated parameters first, expert parameters after them ---------------------------------------------------
+        # -- flat storage: replicated parameters first, expert parameters after them, then the runs' shares of the adapters one run behind the other --------
+        self.lora = adapter_state(model)
+        run_ids = {id(p) for p in adapter_parameters(model)}
         expert_ids = {id(p) for m in model.modules() if isinstance(m, GroupedExperts) for p in m.parameters(recurse=False)} if ep_size > 1 else set()
-        seen, replicated, experts = set(), [], []
+        seen, replicated, experts, runs = set(), [], [], []
         for pname, p in model.named_parameters():
             if id(p) in seen or not p.requires_grad:
                 continue
             seen.add(id(p))
-            (experts if id(p) in expert_ids else replicated).append((pname, p))
+            (experts if id(p) in expert_ids else runs if id(p) in run_ids else replicated).append((pname, p))
         self.entries: list[tuple[str, nn.Parameter, int]] = []
         cursor = 0
         for pname, p in replicated:
@@ -109,7 +114,18 @@ class ModuleEngine:
         for pname, p in experts:
             self.entries.append((pname, p, cursor))
             cursor = _align(cursor + p.numel())
-        self.total = _align(cursor, 256)
+        self.shared_total = _align(cursor, 256)
+        shared = list(self.entries)
+        cursor = 0
+        for pname, p in runs:  # the offset of a factor is that of run 0's share
+            self.entries.append((pname, p, self.shared_total + cursor))
+            cursor = _align(cursor + p[0].numel())
+        self.n_runs, self.run_size = (self.lora.n_adapters if runs else 0), _align(cursor, 256)
+        self.total = self.shared_total + self.n_runs * self.run_size
+        self.run_steps = [0] * self.n_runs  # updates of each run
+        self.run_norms: Tensor | None = None  # f32 [n_runs], of the last step before clipping; 0 for a run without rows, no number for one that was left out for it
+        self._run_rows = [0] * self.n_runs  # rows of the step so far
+        self._clip_plan = None  # of the runs' stretches
         dev = self.device
         self.params_bf16 = torch.zeros(self.total, dtype=torch.bfloat16, device=dev)
         self.master = torch.zeros(self.total, dtype=torch.float32, device=dev)
@@ -118,18 +134,24 @@ class ModuleEngine:
         self.exp_avg_sq = torch.zeros(n_v, dtype=torch.float32, device=dev)
         self.main_grad = torch.zeros(self.total, dtype=torch.float32, device=dev)
         self._grad_views: list[Tensor] = []
+
+        def home(flat: Tensor, p: nn.Parameter, off: int) -> Tensor:
+            if id(p) not in run_ids:
+                return flat[off:off + p.numel()].view(p.shape)
+            at = off - self.shared_total
+            return flat[self.shared_total:].view(self.n_runs, self.run_size)[:, at:at + p[0].numel()].view(p.shape)
+
         with torch.no_grad():
             for pname, p, off in self.entries:
-                n = p.numel()
                 if p.dtype not in (torch.bfloat16, torch.float32):
                     raise PrimeMI355XError(f"{pname}: parameters are bf16 (compute) or f32 (e.g. an f32 router gate), got {p.dtype}")
-                self.master[off:off + n].copy_(p.detach().reshape(-1).float())
+                home(self.master, p, off).copy_(p.detach().float())
                 if p.dtype == torch.bfloat16:
-                    self.params_bf16[off:off + n].copy_(p.detach().reshape(-1))
-                    p.data = self.params_bf16[off:off + n].view(p.shape)
+                    home(self.params_bf16, p, off).copy_(p.detach())
+                    p.data = home(self.params_bf16, p, off)
                 else:  # an f32 parameter IS its master copy; its bf16 shadow is scratch for the fused kernel
-                    p.data = self.master[off:off + n].view(p.shape)
-                self._grad_views.append(self.main_grad[off:off + n].view(p.shape))
+                    p.data = home(self.master, p, off)
+                self._grad_views.append(home(self.main_grad, p, off))
         # Expert parameters (97 % of an MoE model's weights) and the LM head get their gradient written / accumulated in f32 by the weight-gradient GEMM itself
         # (layers/moe.py `_main_grads`, layers/lm_head.py `_StoredLogitsLogProbEntropyFn`): no bf16 `.grad` tensor and no bf16 -> f32 accumulation pass over them.  PM_MOE_MAIN_GRAD=0 is the A/B switch.
         self._direct: list[nn.Parameter] = []
@@ -166,8 +188,8 @@ class ModuleEngine:
         # model) is never read.  Spans of consecutive entries of one kind, in flat-buffer order: (start, end, zero_grad).
         direct_ids = {id(p) for p in self._direct}
         self._update_spans: list[tuple[int, int, bool]] = []
-        for i, (pname, p, off) in enumerate(self.entries):
-            end = self.entries[i + 1][2] if i + 1 < len(self.entries) else self.total
+        for i, (pname, p, off) in enumerate(shared):
+            end = shared[i + 1][2] if i + 1 < len(shared) else self.shared_total
             zero = id(p) not in direct_ids
             if self._update_spans and self._update_spans[-1][2] == zero:
                 self._update_spans[-1] = (self._update_spans[-1][0], end, zero)
@@ -206,7 +228,7 @@ class ModuleEngine:
                     cur += n
                 covered.sort()
                 pos = 0
-                for a, b in covered + [(self.total, self.total)]:  # the complement of the covered ranges, cut at the partition boundary
+                for a, b in covered + [(self.shared_total, self.shared_total)]:  # the complement of the covered ranges, cut at the partition boundary
                     for lo, hi, part in ((pos, min(a, self.n_replicated), 0), (max(pos, self.n_replicated), a, 1)):
                         if hi > lo:
                             self._norm_rest.append((lo, hi, part))
@@ -318,13 +340,14 @@ class ModuleEngine:
             raise PrimeMI355XError("the model must return log-probs and entropy (inject_prime_lm_head with the fused head; trainer/model.py:setup_model does)")
         logprobs = out["logprobs"].reshape(n).float()
         entropy = out["entropy"].reshape(n).float().detach()
+        rows = self.lora.rows if self.lora is not None else None
         c = self.loss_cfg
         if c.type == "custom":  # LossFn plugin: per-sample Python under autograd on the detached log-probs (trainer/rl/loss.py)
             from .rl.loss import plugin_loss_over_pass
 
             loss, grad, per_mb, metrics = plugin_loss_over_pass(logprobs, b, scales, c.custom_fn, self.dims.vocab_size)
             return dict(loss=loss, grad_logprobs=grad, sample_stats=None, sample_metrics=dict(loss_per_micro_batch=per_mb, metrics=metrics),
-                        logprobs=logprobs, entropy=entropy)
+                        logprobs=logprobs, entropy=entropy, lora_rows=rows)
         params = LossParams(loss_type=_lib.PM_LOSS_IPO if c.type == "ipo" else _lib.PM_LOSS_DEFAULT, dppo_mask_low=c.dppo_mask_low,
                             dppo_mask_high=c.dppo_mask_high, adv_tau=c.adv_tau, kl_tau=c.kl_tau, ipo_threshold=c.ipo_threshold,
                             rl_scale=float(max(scales[0], 1)), ce_scale=float(max(scales[1], 1)), ref_kl_scale=float(max(scales[2], 1)), shift=1,
@@ -332,11 +355,13 @@ class ModuleEngine:
         loss, grad, stats, metrics = ops.grpo_loss_fwd_bwd(logprobs.detach().contiguous(), b.inference_logprobs, b.advantages, b.loss_mask, b.cu_samples,
                                                            params, ref_logprobs=b.ref_logprobs, rl_weights=b.rl_weights, ce_weights=b.ce_weights,
                                                            ref_kl_weights=b.ref_kl_weights, sample_starts_mb=b.sample_starts_mb)
-        return dict(loss=loss, grad_logprobs=grad, sample_stats=stats, sample_metrics=metrics, logprobs=logprobs, entropy=entropy)
+        return dict(loss=loss, grad_logprobs=grad, sample_stats=stats, sample_metrics=metrics, logprobs=logprobs, entropy=entropy, lora_rows=rows)
 
     def backward(self, ctx: dict) -> None:
         """d loss / d parameters through the autograd graph, seeded with the loss kernel's d loss / d log-prob; gradients land in f32."""
         ctx["logprobs"].backward(ctx["grad_logprobs"])
+        if self.n_runs:
+            self._run_rows = [a + b for a, b in zip(self._run_rows, ctx["lora_rows"].rows_of_adapters())]
         with torch.no_grad():
             for (pname, p, off), gv in zip(self.entries, self._grad_views):
                 if p.grad is None:
@@ -345,7 +370,7 @@ class ModuleEngine:
                 if st is not None and not st[0]:  # a direct parameter whose gradient came through autograd after all (a shape the f32-writing GEMM does not
                     gv.zero_()                    # take): its slice is not zeroed by the optimizer launch (_update_spans) and still holds the consumed gradient
                     st[0] = True
-                if p.grad.dtype == torch.bfloat16 and p.numel() % 8 == 0:
+                if p.grad.dtype == torch.bfloat16 and p.numel() % 8 == 0 and gv.is_contiguous():
                     ops.grad_accumulate(gv.view(-1), p.grad.contiguous().view(-1))
                 else:
                     gv.add_(p.grad)
@@ -358,15 +383,17 @@ class ModuleEngine:
             if self.device.type == "cuda":
                 torch.cuda.current_stream().wait_event(ev)
         self._param_readers.clear()
-        nr, g = self.n_replicated, self.main_grad
+        nr, end, g = self.n_replicated, self.shared_total, self.main_grad
         for p in self._direct:  # a direct parameter no backward pass of this step wrote (unused / frozen path): its slice still holds the previous step's gradient
             if not p.main_grad_written[0]:
                 p.main_grad.zero_()
         if self.dp_size > 1:
             if nr:
                 dist.all_reduce(g[:nr], op=dist.ReduceOp.SUM, group=self.dp_group)
-            if self.total > nr and (self.ep_size == 1 or self.dp_size > self.ep_size):
-                dist.all_reduce(g[nr:], op=dist.ReduceOp.SUM, group=self.ep_replica_group if self.ep_size > 1 else self.dp_group)
+            if self.n_runs:
+                dist.all_reduce(g[end:], op=dist.ReduceOp.SUM, group=self.dp_group)
+            if end > nr and (self.ep_size == 1 or self.dp_size > self.ep_size):
+                dist.all_reduce(g[nr:end], op=dist.ReduceOp.SUM, group=self.ep_replica_group if self.ep_size > 1 else self.dp_group)
         self._sumsq.zero_()
         if self._fused_norm and all(valid[0] for _, valid, _, _ in self._fused_norm):
             # every expert weight-gradient launch of this step left its tiles' sums of squares: read those (a few MB) and pass only over the rest
@@ -380,11 +407,11 @@ class ModuleEngine:
         else:
             if nr:
                 ops.sumsq_accumulate(g[:nr], self._sumsq[0:1])
-            if self.total > nr:
-                ops.sumsq_accumulate(g[nr:], self._sumsq[1:2])
+            if end > nr:
+                ops.sumsq_accumulate(g[nr:end], self._sumsq[1:2])
         for _, valid, _, _ in self._fused_norm:
             valid[0] = False
-        if self.total > nr and self.ep_size > 1:
+        if end > nr and self.ep_size > 1:
             dist.all_reduce(self._sumsq[1:2], op=dist.ReduceOp.SUM, group=self.ep_group)
         total = self._sumsq.sum().reshape(1)
         o = self.optim
@@ -394,15 +421,44 @@ class ModuleEngine:
                               g[a:b], self.params_bf16[a:b], self.step_count, coef, zero_grad=zero_grad)
         for p in self._direct:
             p.main_grad_written[0] = False  # consumed: the next step's first weight-gradient launch overwrites the slice (it is NOT zeroed, see _update_spans)
-        return norm
+        return self._update_runs(total) if self.n_runs else norm
 
-    def step(self, batch: PackedBatch | list[PackedBatch]) -> dict:
+    def _update_runs(self, shared_sumsq: Tensor) -> Tensor:
+        """Each run's own norm, clipping and update, over its stretch of the flat buffers; the norm of everything is returned."""
+        rows, self._run_rows = self._run_rows, [0] * self.n_runs
+        if self.dp_size > 1:  # a run has rows where any rank had some
+            t = torch.tensor(rows, dtype=torch.int64, device=self.device)
+            dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.dp_group)
+            rows = t.tolist()
+        o, spans = self.optim, [(a, a + self.run_size) for a in range(self.shared_total, self.total, self.run_size)]
+        if self._clip_plan is None:  # of gradients that stay where they are as long as the engine lives
+            self._clip_plan = ops.GradClipPlan([self.main_grad[a:b] for a, b in spans], groups=list(range(self.n_runs)))
+        coefs, self.run_norms = self._clip_plan.coefs(o.max_norm if o.max_norm else 0.0)
+        # A run without rows rests: neither its moments nor its weights move.  So does one whose gradients are no numbers (its norm tells): weights that are none would reach
+        # the other runs in the next pass, where attention multiplies rows of neighbouring documents by weights of zero.
+        for run, (norm, (a, b)) in enumerate(zip(self.run_norms.tolist(), spans)):
+            if not rows[run] or not math.isfinite(norm):
+                self.main_grad[a:b].zero_()
+                continue
+            self.run_steps[run] += 1
+            zero.apply_update(ops, o, self.master[a:b], self.exp_avg[a:b] if self.exp_avg.numel() else None, self.exp_avg_sq[a:b] if self.exp_avg_sq.numel() else None,
+                              self.main_grad[a:b], self.params_bf16[a:b], self.run_steps[run], coefs[run:run + 1], zero_grad=True)
+        return (shared_sumsq.double() + self.run_norms.double().square().sum()).sqrt().float()
+
+    def step(self, batch: PackedBatch | list[PackedBatch], rows: list[LoRARows] | None = None) -> dict:
+        """`rows`: for a model with adapters each pass's table (LoRAState.set_rows before each); one pass may have it set already."""
         passes = batch if isinstance(batch, list) else [batch]
+        if rows is not None and (self.lora is None or len(rows) != len(passes)):
+            raise PrimeMI355XError(f"rows: expected one table for each of {len(passes)} passes of a model with adapters, got {len(rows)}")
+        if rows is None and self.lora is not None and len(passes) > 1:
+            raise PrimeMI355XError(f"{len(passes)} passes through a model with adapters need a table each: step(passes, rows=[...])")
         counts = tuple(sum(p.local_counts[k] for p in passes) for k in range(3))
         scales = self.global_scales(counts)
         out = {"loss": [], "entropy": [], "logprobs": [], "sample_metrics": [], "sample_stats": [], "load_balance": []}
         moe = bool(getattr(self.model.config, "num_experts", None))
-        for p in passes:
+        for i, p in enumerate(passes):
+            if rows is not None:
+                self.lora.set_rows(rows[i])
             ctx = self.forward_loss(p, scales)
             if moe:  # per-layer load violation and routing confidence of this pass, counters reset (train.py:531-535, model.py:561-592); the reference
                 # reads them per micro-batch — a pass is `tokens_per_pass // seq_len` micro-batches routed together

@@ -160,3 +160,244 @@ def test_a_table_of_another_pass_is_refused():
             run(fits)
     with pytest.raises(ValueError, match="11 rows of adapters in a pass of 10"):
         LoRARows.packed([6, 5], "cpu", n_rows=10)
+
+
+def _fwd(x, a, b, scales, offsets, base=None, row_ids=None, out=None):
+    ends, z = offsets.tolist(), torch.zeros(x.shape[0], (a.shape[1] + 15) // 16 * 16)
+    y = base.float().clone()
+    for g in range(a.shape[0]):
+        rows = slice(ends[g], ends[g + 1])
+        z[rows, :a.shape[1]] = scales[g] * (x[rows].float() @ a[g].float().t())
+        y[rows] += z[rows, :a.shape[1]] @ b[g].float()
+    out = torch.empty_like(base) if out is None else out
+    out.copy_(y)
+    return out, z
+
+
+def _bwd(grad_out, x, z, a, b, scales, offsets, base=None, row_ids=None, grad_x=None, grad_a=None, grad_b=None, accumulate=False, want_x=True, want_factors=True):
+    ends, r = offsets.tolist(), a.shape[1]
+    da, db = torch.zeros(a.shape), torch.zeros(b.shape)
+    dx = base.float().clone() if want_x else None
+    for g in range(a.shape[0]):
+        rows = slice(ends[g], ends[g + 1])
+        dz = scales[g] * (grad_out[rows].float() @ b[g].float().t())
+        da[g], db[g] = dz.t() @ x[rows].float(), z[rows, :r].t() @ grad_out[rows].float()
+        if want_x:
+            dx[rows] += dz @ a[g].float()
+    if want_x:
+        grad_x.copy_(dx)
+    return grad_x, da, db
+
+
+class _Plan:
+    """GradClipPlan's factors by group, from the definition."""
+
+    def __init__(self, grads, groups):
+        self.grads, self.groups = grads, groups
+
+    def coefs(self, max_norm):
+        squares = torch.zeros(max(self.groups) + 1, dtype=torch.float64)
+        for t, g in zip(self.grads, self.groups):
+            squares[g] += t.double().square().sum()
+        norms = squares.sqrt().float()
+        return (max_norm / (norms + 1e-6)).clamp(max=1.0) if max_norm > 0 else torch.ones_like(norms), norms
+
+
+SEQ = 48
+
+
+@pytest.fixture
+def plain_adapters(plain_ops, monkeypatch):
+    from prime_rl_amd import ops
+
+    monkeypatch.setattr(ops, "lora_fwd", _fwd)
+    monkeypatch.setattr(ops, "lora_bwd", _bwd)
+    monkeypatch.setattr(ops, "GradClipPlan", _Plan)
+
+
+def _engine(n=2, extra=False, dtype=None, dp=None, **optim):
+    from prime_rl_amd.trainer.engine import OptimConfig
+    from prime_rl_amd.trainer.models.layers.lm_head import inject_prime_lm_head
+    from prime_rl_amd.trainer.models.layers.lora import LoRAAdapters
+    from prime_rl_amd.trainer.module_engine import ModuleEngine
+
+    model, _, state = _with_adapters(n)
+    if extra:
+        model.model.norm.weight.requires_grad_(True)  # a parameter that all runs share
+    for m in model.modules():
+        if dtype is not None and isinstance(m, LoRAAdapters):
+            m.to(dtype)
+    inject_prime_lm_head(model, chunk_size=32)
+    return model, state, ModuleEngine(model, "cpu", optim=OptimConfig(**{**dict(lr=2e-3, weight_decay=0.01, max_norm=0.01), **optim}), **(dp or {}))
+
+
+def _batches(step, n=2):
+    from prime_rl_amd.trainer.rl.data import FakeDataLoader, FakeDataLoaderConfig
+
+    dl = FakeDataLoader(FakeDataLoaderConfig(batch_size=n, generate_samples=True), seq_len=SEQ)
+    dl.batch_counter = step
+    mbs = dl.get_batch()
+    g = torch.Generator().manual_seed(step)
+    for mb in mbs:
+        mb["input_ids"] = mb["input_ids"] % 64
+        mb["inference_logprobs"] = -torch.rand(1, SEQ, generator=g) * 0.1 - 4.1
+    return mbs
+
+
+def _pass(engine, state, step, counts, mbs=None):
+    """Forward and backward of one pass, before the update."""
+    from prime_rl_amd.trainer.engine import pack_micro_batches
+    from prime_rl_amd.trainer.models.layers.lora import LoRARows
+
+    b = pack_micro_batches(mbs or _batches(step), "cpu")
+    state.set_rows(LoRARows.packed(counts, "cpu", n_rows=b.n_tokens))
+    engine.backward(engine.forward_loss(b, engine.global_scales(b.local_counts)))
+
+
+def _run_values(model, run):
+    from prime_rl_amd.trainer.models.layers.lora import adapter_parameters
+
+    return torch.cat([p[run].detach().float().reshape(-1) for p in adapter_parameters(model)])
+
+
+def _region(engine, run):
+    return slice(engine.shared_total + run * engine.run_size, engine.shared_total + (run + 1) * engine.run_size)
+
+
+@pytest.mark.parametrize("kind", ["adamw", "sgd", "sign_sgd"])
+@pytest.mark.parametrize("extra,dtype", [(False, None), (True, None), (False, BF16)])
+def test_a_run_does_not_notice_the_others(plain_adapters, kind, extra, dtype):
+    """Run 0 after two steps is the same to the bit whether run 1 has ordinary gradients, huge ones, none that are numbers, or no rows."""
+    results = []
+    for how in ("ordinary", "huge", "nan", "no rows"):
+        model, state, engine = _engine(extra=extra, dtype=dtype, type=kind)
+        for step in range(2):
+            _pass(engine, state, step, [SEQ, 0 if how == "no rows" else SEQ])
+            if extra:  # what the runs share follows all of them: held still here
+                engine.main_grad[:engine.shared_total].zero_()
+            before = _run_values(model, 1).clone()
+            assert engine.main_grad[_region(engine, 0)].any()
+            if how in ("huge", "nan"):
+                engine.main_grad[_region(engine, 1)].mul_(1e6 if how == "huge" else float("nan"))
+            engine.optimizer_step()
+            assert torch.equal(_run_values(model, 1), before) == (how in ("nan", "no rows"))  # of no numbers: nothing is done with them
+        assert not engine.main_grad.any() and engine.run_steps == [2, 0 if how in ("nan", "no rows") else 2]
+        results.append((_run_values(model, 0), engine.run_norms[0], engine.master[_region(engine, 0)].clone()))
+    for other in results[1:]:
+        assert all(torch.equal(u, v) for u, v in zip(results[0], other))
+
+
+def test_a_run_is_clipped_by_its_own_norm(plain_adapters):
+    """Two runs' updates against the definition: each with its own norm, factor, and first step of SGD without momentum."""
+    model, state, engine = _engine(type="sgd", momentum=0.0, weight_decay=0.0, lr=0.5, max_norm=1e-3)
+    _pass(engine, state, 0, [SEQ, SEQ])
+    engine.main_grad[_region(engine, 1)].mul_(100.0)
+    grads = [engine.main_grad[_region(engine, g)].double() for g in range(2)]
+    before = [engine.master[_region(engine, g)].double() for g in range(2)]
+    norm = engine.optimizer_step()
+    for g in range(2):
+        own = grads[g].norm()
+        assert own > 1e-3 and abs(engine.run_norms[g].double() - own) <= 1e-6 * own  # f32 sums of squares
+        want = before[g] - 0.5 * grads[g] * (1e-3 / (own + 1e-6))
+        assert ((engine.master[_region(engine, g)].double() - want).abs() <= 2.0**-23 * before[g].abs() + 1e-6 * (want - before[g]).abs()).all()
+    whole = torch.cat(grads).norm()
+    assert abs(norm.double() - whole) <= 1e-6 * whole
+
+
+def test_a_run_that_rests_goes_on_where_it_was(plain_adapters):
+    """Run 1 without rows in the second of three steps: its weights and moments wait, and its third update is the second of a run that never rested."""
+    model, state, engine = _engine()
+    _pass(engine, state, 0, [SEQ, SEQ])
+    engine.optimizer_step()
+    held = [t[_region(engine, 1)].clone() for t in (engine.master, engine.exp_avg, engine.exp_avg_sq)]
+    own = _run_values(model, 0).clone()
+    _pass(engine, state, 1, [SEQ, 0])
+    engine.optimizer_step()
+    assert all(torch.equal(t[_region(engine, 1)], h) for t, h in zip((engine.master, engine.exp_avg, engine.exp_avg_sq), held)) and engine.run_norms[1] == 0
+    assert not torch.equal(_run_values(model, 0), own) and engine.run_steps == [2, 1]
+    other_model, other_state, other = _engine()
+    _pass(other, other_state, 0, [SEQ, SEQ])
+    other.optimizer_step()
+    for e, st in ((engine, state), (other, other_state)):
+        _pass(e, st, 2, [0, SEQ])
+        e.optimizer_step()
+    assert torch.equal(_run_values(model, 1), _run_values(other_model, 1)) and other.run_steps == [1, 2]
+
+
+def test_rows_the_device_knows_alone(plain_adapters):
+    """A table whose counts the host was not told: the engine reads them."""
+    from prime_rl_amd.trainer.models.layers.lora import LoRARows
+
+    model, state, engine = _engine()
+    rows = LoRARows(torch.tensor([0, SEQ, SEQ], dtype=torch.int32))
+    from prime_rl_amd.trainer.engine import pack_micro_batches
+
+    held = _run_values(model, 1).clone()
+    engine.step(pack_micro_batches(_batches(0), "cpu"), rows=[rows])
+    assert engine.run_steps == [1, 0] and torch.equal(_run_values(model, 1), held)
+
+
+def test_passes_of_a_step_have_a_table_each(plain_adapters):
+    """Two passes of different rows against one pass of both; without tables, or with too few, the step is refused."""
+    from prime_rl_amd._lib import PrimeMI355XError
+    from prime_rl_amd.trainer.engine import pack_micro_batches
+    from prime_rl_amd.trainer.models.layers.lora import LoRARows
+
+    mbs = _batches(0)
+    model, state, engine = _engine(max_norm=1e9)
+    passes = [pack_micro_batches([mb], "cpu") for mb in mbs]
+    tables = [LoRARows.packed([SEQ, 0], "cpu"), LoRARows.packed([0, SEQ], "cpu")]
+    for rows in (None, tables[:1]):
+        with pytest.raises(PrimeMI355XError, match="table"):
+            engine.step(passes, rows=rows)
+    engine.step(passes, rows=tables)
+    norms = engine.run_norms
+    model, state, engine = _engine(max_norm=1e9)
+    engine.step([pack_micro_batches(mbs, "cpu")], rows=[LoRARows.packed([SEQ, SEQ], "cpu")])
+    assert ((engine.run_norms - norms).abs() <= 0.05 * norms).all() and engine.run_steps == [1, 1]  # bf16 activations of products of other sizes
+    from prime_rl_amd.trainer.engine import OptimConfig
+    from prime_rl_amd.trainer.module_engine import ModuleEngine
+
+    with pytest.raises(PrimeMI355XError, match="with adapters"):
+        ModuleEngine(_model(), "cpu", optim=OptimConfig()).step([passes[0]], rows=[tables[0]])
+
+
+def _two_ranks(rank, world, port, out):
+    """Rank r has run r's rows only: the ranks hold the same runs after each step, those of one process with both passes."""
+    import os
+
+    import torch.distributed as dist
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    torch.set_num_threads(2)
+    try:
+        from prime_rl_amd import ops
+        from tests.test_moe_ep_gloo_cpu import _patch_all_ops
+
+        _patch_all_ops()
+        ops.lora_fwd, ops.lora_bwd, ops.GradClipPlan = _fwd, _bwd, _Plan
+        from prime_rl_amd.trainer.engine import pack_micro_batches
+        from prime_rl_amd.trainer.models.layers.lora import LoRARows
+
+        model, _, engine = _engine(n=3, dp=dict(dp_group=dist.group.WORLD, dp_size=world))
+        ref_model, _, ref = _engine(n=3)
+        for step in range(2):
+            mbs = _batches(step)
+            tables = [LoRARows.packed([SEQ if g == r else 0 for g in range(3)], "cpu") for r in range(world)]
+            engine.step([pack_micro_batches([mbs[rank]], "cpu")], rows=[tables[rank]])
+            ref.step([pack_micro_batches([mb], "cpu") for mb in mbs], rows=tables)
+            assert engine.run_steps == [step + 1, step + 1, 0] and ref.run_steps == engine.run_steps
+            assert torch.equal(engine.run_norms, ref.run_norms), (step, engine.run_norms, ref.run_norms)
+        for g in range(3):
+            assert torch.equal(_run_values(model, g), _run_values(ref_model, g)), g
+    finally:
+        dist.destroy_process_group()
+
+
+def test_runs_on_other_ranks(tmp_path):
+    import torch.multiprocessing as mp
+
+    from tests._ports import free_port
+
+    mp.spawn(_two_ranks, args=(2, free_port(), str(tmp_path)), nprocs=2, join=True)
