@@ -326,6 +326,8 @@ class ModuleEngine:
 
     # -- one pass -------------------------------------------------------------------------------------------------------------------
     def forward_loss(self, b: PackedBatch, scales: tuple[int, int, int]) -> dict:
+        if adapter_state(self.model) is not self.lora:
+            raise PrimeMI355XError("adapters are attached before the engine takes the model's parameters (attach_lora, then ModuleEngine)")
         n = b.n_tokens
         seq_lens = (b.cu_seqlens[1:] - b.cu_seqlens[:-1]).to(torch.int64)
         kw = {}

@@ -362,6 +362,19 @@ def test_passes_of_a_step_have_a_table_each(plain_adapters):
         ModuleEngine(_model(), "cpu", optim=OptimConfig()).step([passes[0]], rows=[tables[0]])
 
 
+def test_adapters_come_before_the_engine(plain_ops):
+    from prime_rl_amd._lib import PrimeMI355XError
+    from prime_rl_amd.trainer.engine import OptimConfig, pack_micro_batches
+    from prime_rl_amd.trainer.models.layers.lora import attach_lora
+    from prime_rl_amd.trainer.module_engine import ModuleEngine
+
+    model = _model()
+    engine = ModuleEngine(model, "cpu", optim=OptimConfig())
+    attach_lora(model, 2, 4, 8.0)
+    with pytest.raises(PrimeMI355XError, match="before the engine"):
+        engine.step(pack_micro_batches(_batches(0), "cpu"))
+
+
 def _two_ranks(rank, world, port, out):
     """Rank r has run r's rows only: the ranks hold the same runs after each step, those of one process with both passes."""
     import os
