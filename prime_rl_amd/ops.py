@@ -1244,8 +1244,9 @@ class GradClipPlan:
 
     `grads`: contiguous f32 | bf16 GPU tensors; `groups[i]` in [0, n_groups) is the group of grads[i] (None: one group).  `out[i]`, f32 | bf16 of the same size,
     receives the clipped grads[i] — e.g. a slice of the flat f32 gradient that `adamw_step` reads; without `out` the gradients are clipped in place.  The plan
-    holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are, and keep it as long as a captured graph of
-    its calls."""
+    holds the table of all tensors on the device and keeps their memory; build it once for gradients that stay where they are (flat buffers, `zero_grad(set_to_none=False)`),
+    and keep it as long as a captured graph of its calls.  Gradients that autograd makes anew are not followed: the plan goes on clipping the memory it has.  `check` raises for
+    them.  Of 2016 tensors, building takes the host 6.4 ms, a check 0.44."""
 
     _CHUNK_MOST, _PIECE = 65536, 2048
 
@@ -1274,6 +1275,7 @@ class GradClipPlan:
         if any(t.device != self.device for t in (*grads, *dst)):
             raise PrimeMI355XError(f"GradClipPlan: expected all tensors on {self.device}")
         self._held = [t.detach() for t in (*grads, *dst)]
+        self._at = [(t.data_ptr(), t.numel(), t.dtype) for t in grads]
         src = np.array([(t.data_ptr(), t.numel() * t.element_size(), i) for i, t in enumerate(grads) if t.numel()], dtype=np.int64).reshape(-1, 3)
         own = np.array([(o.data_ptr(), o.numel() * o.element_size(), i) for i, o in enumerate(dst) if o.numel()], dtype=np.int64).reshape(-1, 3)
         spans = src if out is None else np.concatenate([src, own[own[:, 0] != src[:, 0]]])
@@ -1304,6 +1306,15 @@ class GradClipPlan:
         self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
         self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)  # the tables' own
         self._offsets = torch.from_numpy(np.searchsorted(np.array(groups, dtype=np.int64)[of], np.arange(self.n_groups + 1)).astype(np.int32)).to(self.device)
+
+    def check(self, grads: list[Tensor | None]) -> None:
+        """Raises unless `grads` (say each parameter's `.grad` as it is now) are what the plan was built for, in the same places."""
+        if len(grads) != len(self._at):
+            raise PrimeMI355XError(f"grads: a plan of {len(self._at)} gradients, got {len(grads)}")
+        for i, (t, at) in enumerate(zip(grads, self._at)):
+            if t is None or (t.data_ptr(), t.numel(), t.dtype) != at or not t.is_contiguous():
+                raise PrimeMI355XError(f"grads[{i}]: {'none' if t is None else 'not where the plan has it'}; a plan is for gradients that stay in place (zero_grad(set_to_none=False)), "
+                                       "others need a plan of their own")
 
     def _run(self, max_norm, sumsq: Tensor | None, want_sumsq: bool, scale: bool) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
         lib = _lib.load()
