@@ -81,6 +81,12 @@ class LoRAState:
             raise ValueError(f"rows of {rows.offsets.numel() - 1} adapters for a model of {self.n_adapters}")
         self.rows = rows
 
+    def scales_on(self, device) -> Tensor:
+        """The scales beside the rows of a pass: a model may have moved since it got its adapters."""
+        if self.scales.device != device:
+            self.scales = self.scales.to(device)
+        return self.scales
+
 
 class LoRAAdapters(nn.Module):
     """The adapters of one projection; `a` starts uniform (as nn.Linear's weight does), `b` at zero: the update starts at zero."""
@@ -180,7 +186,7 @@ def lora_linear(x: Tensor, linears: Sequence[nn.Linear], adapters: Sequence[LoRA
     state.rows.check(x.shape[0])
     x = x if x.is_contiguous() else x.contiguous()
     factors = [f for a in adapters if a is not None for f in (a.a, a.b)]
-    return _LoRALinearFn.apply(x, state.rows, state.scales, [a is not None for a in adapters], [lin.weight.detach() for lin in linears],
+    return _LoRALinearFn.apply(x, state.rows, state.scales_on(x.device), [a is not None for a in adapters], [lin.weight.detach() for lin in linears],
                                [None if lin.bias is None else lin.bias.detach() for lin in linears], *factors)
 
 
