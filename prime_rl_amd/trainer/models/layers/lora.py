@@ -145,8 +145,8 @@ class _LoRALinearFn(torch.autograd.Function):
         n_factors, n_weights = len(ctx.dtypes), len(ctx.widths)
         weights, halves, zs = rest[:n_weights], rest[n_weights:n_weights + n_factors], rest[n_weights + n_factors:]
         joined = _adjacent_view(weights)
-        # rows that overlap (a gradient that is one row for all, say) are written out
-        dy = dy if dy.stride(1) == 1 and dy.stride(0) >= dy.shape[1] and dy.stride(0) % 8 == 0 and dy.data_ptr() % 16 == 0 else dy.contiguous()
+        # rows that overlap (a gradient that is one row for all, say) or begin at odd places are written out
+        dy = dy if dy.stride(1) == 1 and dy.stride(0) >= dy.shape[1] and dy.stride(0) % 8 == 0 and dy.data_ptr() % 16 == 0 else dy.clone(memory_format=torch.contiguous_format)
         want_x, want_factors = ctx.needs_input_grad[0], any(ctx.needs_input_grad[6:])
         dx, parts = None, dy.split(ctx.widths, dim=1)
         if want_x:
@@ -184,7 +184,7 @@ def lora_linear(x: Tensor, linears: Sequence[nn.Linear], adapters: Sequence[LoRA
     if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise ValueError("a captured pass through adapters runs under torch.no_grad()")
     state.rows.check(x.shape[0])
-    x = x if x.is_contiguous() else x.contiguous()
+    x = x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
     factors = [f for a in adapters if a is not None for f in (a.a, a.b)]
     return _LoRALinearFn.apply(x, state.rows, state.scales_on(x.device), [a is not None for a in adapters], [lin.weight.detach() for lin in linears],
                                [None if lin.bias is None else lin.bias.detach() for lin in linears], *factors)
