@@ -12,6 +12,7 @@ bf16): adapters are small, and their gradients arrive in f32 without a rounding.
 from __future__ import annotations
 
 import math
+import warnings
 from collections.abc import Iterable, Sequence
 
 import torch
@@ -195,15 +196,20 @@ TARGETS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down
 
 def attach_lora(model: nn.Module, n_adapters: int, rank: int, alpha: float | Sequence[float], targets: Sequence[str] = TARGETS) -> LoRAState:
     """Hangs adapters on every projection of the attention and dense MLP seams that `targets` names, freezes all other parameters, and returns the state whose
-    `set_rows` describes each pass.  A model has one set of adapters: it is attached once."""
+    `set_rows` describes each pass.  A model has one set of adapters: it is attached once.  Experts of MoE layers, routed and shared, get none (a warning says so where
+    `targets` names their projections)."""
     from .attn import HipVarlenAttention
     from .mlp import MLP
+    from .moe import BCFeedForward, GroupedExperts
 
     unknown = set(targets) - set(TARGETS)
     if unknown:
         raise ValueError(f"targets: expected names among {TARGETS}, got {sorted(unknown)}")
     if any(isinstance(m, LoRAAdapters) for m in model.modules()):
         raise ValueError("the model has adapters already")
+    experts = [name for name, m in model.named_modules() if isinstance(m, (GroupedExperts, BCFeedForward))]
+    if experts and set(targets) & {"gate_proj", "up_proj", "down_proj"}:
+        warnings.warn(f"attach_lora: {len(experts)} expert modules ({experts[0]}, ...) are frozen without adapters: only attention and dense MLP projections have them", stacklevel=2)
     device = next(model.parameters()).device
     state = LoRAState(n_adapters, rank, alpha, device)
     linears = [lin for m in model.modules() if isinstance(m, (HipVarlenAttention, MLP)) for name, lin in m.named_children() if name in targets]

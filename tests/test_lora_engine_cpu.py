@@ -414,3 +414,19 @@ def test_runs_on_other_ranks(tmp_path):
     from tests._ports import free_port
 
     mp.spawn(_two_ranks, args=(2, free_port(), str(tmp_path)), nprocs=2, join=True)
+
+
+def test_experts_without_adapters_are_named():
+    """A MoE model's experts get none: a warning says so where their projections were asked for, and only there."""
+    import warnings
+
+    from prime_rl_amd.trainer.models.layers.lora import adapter_linears, attach_lora
+
+    model = _model(moe=True)
+    with pytest.warns(UserWarning, match="layers.1.mlp.experts"):
+        attach_lora(model, 2, 4, 8.0)
+    assert {k.split(".")[-2] for k in adapter_linears(model)} == {*ATTENTION, "gate_proj", "up_proj", "down_proj"}  # layer 0 is dense
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        attach_lora(_model(moe=True), 2, 4, 8.0, targets=ATTENTION)
+        attach_lora(_model(), 2, 4, 8.0)
