@@ -11,7 +11,7 @@
 //
 // All of it is bound by HBM traffic of the row tensors (2 r operations per 2-byte element, far under the MFMA rate), so each kernel makes one pass over its row
 // tensor with 16-byte accesses, and the matrix cores are there to keep the arithmetic out of the way.  From rank 64 on the LDS has as much to do as the memory.  Measured, in the
-// kernels' own time (a large copy moves 5.7 TB/s, a read past the caches 6.7):
+// kernels' own time, the least of twelve launches (medians of the long ones are up to 25 % above it; a large copy moves 5.7 TB/s, a read past the caches 6.7):
 //   shrink  16 384 x 4096 rank 16 23 us = 5.8 TB/s, 32 768 x 12288 rank 64 143 us = 5.6;   expand  16 384 x 6144 rank 16 66 us = 6.1, 32 768 x 4096 rank 64 107 us = 5.0
 //   outer   16 384 x 4096 rank 16 27 us = 5.0, with dz 16 384 x 6144 47 us = 4.6 (dz's parts among it), 32 768 x (12288 + 4096) rank 64 217 us = 4.9
 //
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const float* __restrict_
 
 // The same for rank > 64.  There the LDS bounds it, and z's fragments are most of what goes through it: a wave keeps those of 32 positions in registers, straight from memory, and
 // takes the factor's tiles of 128 columns one after the other, which the four waves of a workgroup share.  Tiles come by DMA, one ahead; base and out move in the fragments' order.
-// 16 384 x 6144 at rank 128: 128 us against 216 in the way of smaller ranks (a copy takes 75); at rank 64 that way is the faster one (32 768 x 4096: 125 us against 164).
+// 16 384 x 6144 at rank 128: 128 us against 216 in the way of smaller ranks (a copy takes 75); at rank 64 that way is the faster one (32 768 x 4096: 107 us; this way took 164).
 constexpr int kDeepRows = 128, kDeepCols = 128;
 // the transposed fragments of 64 ranks at 8 columns (two halves of 4): rows of 256 bytes, [2 k][2 halves][16 rows, 16 more].  One block with its own wait: the compiler would wait for
 // the tile in flight before such a read.
@@ -1283,8 +1283,8 @@ static inline int outer_range(int64_t n, int n_adapters, int col_tiles, int rank
 }
 
 // Few rows: column blocks of a wave (1 or 4) where both products run in one launch, 0 where they take one each.  All workgroups have to run at once, and what each reads of the first
-// factor must not be much: the card takes about as long either way (in a graph: 1 row 4096 -> 4096 rank 16 7.9 us against 8.8, 64 rows of 32 adapters 9.0 against 9.9, 64 of one 10.9
-// against 10.4, 32 rows 2048 -> 8192 rank 20 7.7 against 10.2; but 1 row of 12288 columns rank 16 16.8 against 9.1, of 4096 rank 64 19.6 against 12.0), the host less (11.5 us a call
+// factor must not be much: the card takes about as long either way (in a graph: 1 row 4096 -> 4096 rank 16 7.9 us against 8.8, 64 rows of 32 adapters 9.0 against 9.9, 64 of one, where the
+// card alone is slower this way, 10.9 against 10.4, 32 rows 2048 -> 8192 rank 20 7.7 against 10.2; but 1 row of 12288 columns rank 16 16.8 against 9.1, of 4096 rank 64 19.6 against 12.0), the host less (11.5 us a call
 // against 16.3).
 static inline int few_rows(int64_t n, int n_adapters, int64_t d_in, int64_t d_out, int rank) {
   if (n > 64 || rank > 64 || rank_tiles(rank) * 16 * d_in > 96 << 10) return 0;
