@@ -229,7 +229,10 @@ def adapter_parameters(model: nn.Module) -> list[nn.Parameter]:
 
 def adapter_state(model: nn.Module) -> LoRAState | None:
     """The state that the model's adapters share; None for a model without."""
-    return next((m.state for m in model.modules() if isinstance(m, LoRAAdapters)), None)
+    states = {id(m.state): m.state for m in model.modules() if isinstance(m, LoRAAdapters)}
+    if len(states) > 1:
+        raise ValueError(f"the model's adapters belong to {len(states)} different states")
+    return next(iter(states.values()), None)
 
 
 def pushed_adapter(model: nn.Module, adapter: int | None) -> int | None:

@@ -430,3 +430,17 @@ def test_experts_without_adapters_are_named():
         warnings.simplefilter("error")
         attach_lora(_model(moe=True), 2, 4, 8.0, targets=ATTENTION)
         attach_lora(_model(), 2, 4, 8.0)
+
+
+def test_adapters_of_two_states_are_no_set(plain_ops):
+    """Adapters hung on by hand with a state each: whose rows a pass has would be guessed, so engine and push refuse them."""
+    from prime_rl_amd.trainer.engine import OptimConfig
+    from prime_rl_amd.trainer.models.layers.lora import LoRAAdapters, LoRAState, merged_state_dict
+    from prime_rl_amd.trainer.module_engine import ModuleEngine
+
+    model, _, _ = _with_adapters(2)
+    mlp = model.model.layers[0].mlp
+    mlp.down_proj.lora = LoRAAdapters(mlp.down_proj, LoRAState(2, 4, 8.0, "cpu"))
+    for call in (lambda: ModuleEngine(model, "cpu", optim=OptimConfig()), lambda: merged_state_dict(model, 0)):
+        with pytest.raises(ValueError, match="2 different states"):
+            call()
